@@ -266,6 +266,79 @@ int vits_op_attention(const float* qkv, const float* emb_k, const float* emb_v, 
 int vits_op_attention_prec(const float* qkv, const float* emb_k, const float* emb_v, const int* lengths, float* out, int B,
                            int H, int DK, int L, int window, int precision, void* stream);
 
+/* ---- a paged key-value cache and the attention that reads it ----
+ * For an autoregressive model that is served beside the synthesiser (a text or prosody model whose tokens, durations
+ * or pitch go to the stages above).  No counterpart in the reference, whose attention (reference attentions.py:179-332)
+ * takes whole rows; vits_op_attention is that one.  These entry points take other types and layouts than the rest of
+ * this header: fp32, fp16 or bf16 values (VITS_TYPE_*), rows of tokens, [rows][heads][dim] with the strides given (in
+ * elements; the channels of a head are contiguous).
+ *
+ * The cache: two tensors [pages][kv_heads][page_size][dim], page_stride elements from page to page (so both may lie in
+ * one [pages][2][...] tensor), the rest contiguous.  page_size is a multiple of 16, at most 65536.  Token t of request
+ * s lies in page table[s][t / page_size] at t % page_size; its slot is page id * page_size + t % page_size.
+ *
+ * A row is one new token.  vits_op_page_plan names each row's request, position and slot; vits_op_rotary_store puts the
+ * rows' keys and values there; vits_op_paged_attention lets every row see its request's tokens up to and with its own.
+ * A row of a request < 0 (slot < 0) is no row: its outputs stay as they were.  So a program that replays a captured
+ * graph sizes its rows once and lets the plan say how many there are.
+ *
+ * err_flag (device int32 zeroed by the caller, or NULL): ids on the device that lie outside what the host described -- a
+ * slot or a page outside the cache, a request or a position outside the table -- are left out, never followed, and OR 1
+ * into it. */
+#define VITS_TYPE_F32 0
+#define VITS_TYPE_F16 1
+#define VITS_TYPE_BF16 2
+
+/* Page plan of one step.  lengths [requests]: tokens each request has in the cache; grow [requests]: how many it gets
+ * now (0 and more), or -1: it ends, its pages go back and its length becomes 0.  table [requests][table_stride], width
+ * of it usable: the page ids, in and out (entries of new pages are written, the others left as they are).  ring [pages]
+ * and cursor {head, tail}: the free pages are ring[i % pages] for i = head .. tail - 1; head and tail only ever grow.  A
+ * page that a request gives back in this call is free from the next call on.
+ * Out: lengths_out [requests], cursor_out [2] (both beside the inputs, not over them: the step can be taken again);
+ * row_start [requests + 1]: where each request's rows begin, and their number; for rows 0 .. rows - 1 row_request,
+ * row_position (0 for a request's first token) and row_slot, -1 behind the last; requests' rows follow each other in
+ * order, and so do the pages they take.  status [1]: 0, or the OR of VITS_PLAN_*; then nothing is taken: lengths_out and
+ * cursor_out repeat the inputs, row_start is 0, every row is -1, table and ring are left as they were.
+ * At most 65535 requests, 2^30 rows and 2^30 pages. */
+#define VITS_PLAN_BAD_LENGTH 1 /* a length below 0, a growth below -1, or their sum beyond int32 */
+#define VITS_PLAN_TABLE_FULL 2 /* a request needs more pages than its row of the table has       */
+#define VITS_PLAN_ROWS_FULL 4  /* more new tokens than rows                                      */
+#define VITS_PLAN_NO_PAGES 8   /* fewer free pages than needed                                   */
+#define VITS_PLAN_BAD_RING 16  /* cursor and lengths contradict the size of the ring             */
+int vits_op_page_plan(const int* lengths, const int* grow, int requests, int* table, int64_t table_stride, int width,
+                      int* ring, int pages, const int64_t* cursor, int page_size, int* lengths_out, int64_t* cursor_out,
+                      int* row_start, int* row_request, int* row_position, int64_t* row_slot, int rows, int* status,
+                      void* stream);
+
+/* Rotary positions, and the write to the cache.  The first 2 * pairs channels of every head of q and k turn by the angle
+ * position * freq[i] (radians; freq in 64 bits, [pairs], the product too): channels i and i + pairs (interleaved == 0) or
+ * 2i and 2i + 1 are (a, b) -> scale * (a cos - b sin, b cos + a sin); the other channels pass through.  q's rows go to
+ * out (may be q itself, with the same strides), k's and v's to slot [rows] of the caches.  q may be NULL (no queries), or
+ * k, v and the caches (then slot may be NULL too: every row is one).  Computed in fp32, rounded once.  The slots of one
+ * call have to differ: where two rows share one, each stored value is either row's.  Scaled positions are scaled
+ * frequencies (vits_amd/ops.py: rotary_frequencies); the gradient with respect to q is the same call on the gradient of
+ * out with -freq.  dim 2 .. 256. */
+int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out, int64_t out_row, int64_t out_head,
+                         int heads, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                         int64_t v_head, void* k_cache, void* v_cache, int64_t page_stride, int pages, int page_size,
+                         int kv_heads, int dim, int dtype, const int* position, const int64_t* slot, int rows,
+                         const double* freq, int pairs, float scale, int interleaved, int* err_flag, void* stream);
+
+/* Attention of single rows: out[r][h] = sum_t w_t v_t with w = softmax_t(scale * q[r][h] . k_t) over the tokens t of row
+ * r's request with position - window < t <= position (window 0: from the first token on), keys and values of head
+ * h / (heads / kv_heads).  A row that sees no token (position < 0) gives 0.  lse [rows][heads] fp32 or NULL: log of the sum
+ * of exp(scale * q . k_t), -inf for such a row.  Scores, softmax and sums in fp32.  What lies in the cache behind a row's
+ * position, and in pages the table does not name for it, has no influence whatever it holds.
+ * dim: 32, 64, ... 256; caches and pages begin on 16-byte addresses.  max_keys: how many tokens the host knows a row to see
+ * at most (0: as many as the table holds); it only guides how the work is split, a row that sees more is right all
+ * the same.  ws: vits_op_paged_attention_workspace_bytes of the same numbers (-1 for a shape that is refused). */
+int64_t vits_op_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int dim, int64_t max_keys);
+int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, const void* v_cache,
+                            int64_t page_stride, int pages, int page_size, const int* table, int64_t table_stride, int width,
+                            int requests, const int* row_request, const int* row_position, int rows, int heads, int kv_heads,
+                            int dim, int dtype, float scale, int window, int64_t max_keys, void* out, int64_t out_row,
+                            int64_t out_head, float* lse, int* err_flag, void* ws, int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

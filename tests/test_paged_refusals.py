@@ -1,0 +1,145 @@
+"""What the paged-cache operators refuse, through the C ABI and the Python functions, and what they compute on the host.
+No GPU: a refused call touches none of its pointers, and none of these calls gets further than its checks."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from vits_amd import _native as N
+from vits_amd import ops
+
+P = 1 << 20            # stands for a device address on a 16-byte boundary; never followed
+INVALID, WORKSPACE = -1, -4
+
+
+def refused(rc, word, code=INVALID):
+    assert rc == code
+    assert word in N.lib.vits_last_error().decode()
+
+
+PLAN = dict(lengths=P, grow=P + 64, requests=4, table=P, table_stride=8, width=8, ring=P, pages=32, cursor=P, page_size=16,
+            lengths_out=P + 4096, cursor_out=P + 8192, row_start=P, row_request=P, row_position=P, row_slot=P, rows=10, status=P, stream=0)
+
+
+@pytest.mark.parametrize("change,word", [
+    *[({n: 0}, "null") for n in ("lengths", "grow", "table", "ring", "cursor", "lengths_out", "cursor_out", "row_start", "status",
+                                 "row_request", "row_position", "row_slot")],
+    (dict(requests=0), "requests"), (dict(requests=65536), "requests"), (dict(rows=-1), "rows"), (dict(rows=(1 << 30) + 1), "rows"),
+    (dict(pages=0), "pages"), (dict(pages=(1 << 30) + 1), "pages"), (dict(width=0), "table"), (dict(table_stride=7), "overlap"),
+    (dict(page_size=0), "page_size"), (dict(page_size=8), "page_size"), (dict(page_size=24), "page_size"), (dict(page_size=-16), "page_size"),
+    (dict(page_size=65552), "page_size"), (dict(lengths_out=P), "in place"), (dict(lengths_out=P + 64), "in place"),
+    (dict(cursor_out=P), "in place"),
+])
+def test_page_plan_refuses(change, word):
+    refused(N.lib.vits_op_page_plan(*{**PLAN, **change}.values()), word)
+
+
+ROTARY = dict(q=P, q_row=512, q_head=128, out=P + 4096, out_row=512, out_head=128, heads=4, k=P, k_row=256, k_head=128, v=P, v_row=256,
+              v_head=128, k_cache=P, v_cache=P, page_stride=2 * 16 * 128, pages=9, page_size=16, kv_heads=2, dim=128, dtype=2, position=P,
+              slot=P, rows=3, freq=P, pairs=64, scale=1.0, interleaved=0, err_flag=0, stream=0)
+
+
+@pytest.mark.parametrize("change,word", [
+    *[({n: 0}, "null") for n in ("position", "freq", "out", "v", "k_cache", "v_cache", "slot")], (dict(q=0, k=0), "null"),
+    (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(rows=-1), "required"), (dict(dim=1, pairs=1), "required"),
+    (dict(dim=258), "required"), (dict(pairs=0), "required"), (dict(pairs=65), "required"), (dict(heads=0), "required"),
+    (dict(heads=1025), "required"), (dict(kv_heads=0), "required"), (dict(pages=0), "required"), (dict(page_size=20), "page_size"),
+    (dict(page_stride=2 * 16 * 128 - 1), "overlap"), (dict(out=P, out_row=640), "in place"), (dict(out=P, out_head=64), "in place"),
+])
+def test_rotary_store_refuses(change, word):
+    refused(N.lib.vits_op_rotary_store(*{**ROTARY, **change}.values()), word)
+
+
+ATTEND = dict(q=P, q_row=512, q_head=128, k_cache=P, v_cache=P, page_stride=2 * 16 * 128, pages=9, page_size=16, table=P, table_stride=8,
+              width=8, requests=3, row_request=P, row_position=P, rows=3, heads=4, kv_heads=2, dim=128, dtype=2, scale=0.1, window=0,
+              max_keys=128, out=P + 65536, out_row=512, out_head=128, lse=0, err_flag=0, ws=P, ws_bytes=1 << 40, stream=0)
+
+
+@pytest.mark.parametrize("change,word", [
+    *[({n: 0}, "null") for n in ("q", "k_cache", "v_cache", "table", "row_request", "row_position", "out")],
+    (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(rows=-1), "required"), (dict(heads=3), "required"), (dict(heads=0), "required"),
+    (dict(kv_heads=0), "required"), (dict(heads=2048, kv_heads=2048), "required"), (dict(dim=0), "required"), (dict(dim=48), "required"),
+    (dict(dim=288), "required"), (dict(page_size=8), "page_size"), (dict(pages=0), "required"), (dict(width=0), "required"),
+    (dict(table_stride=7), "required"), (dict(requests=0), "required"), (dict(window=-1), "required"), (dict(page_stride=100), "overlap"),
+    (dict(k_cache=P + 8), "16-byte"), (dict(v_cache=P + 2), "16-byte"), (dict(page_stride=2 * 16 * 128 + 4), "16-byte"),
+    (dict(out=P), "in place"),
+])
+def test_paged_attention_refuses(change, word):
+    refused(N.lib.vits_op_paged_attention(*{**ATTEND, **change}.values()), word)
+
+
+def test_paged_attention_workspace():
+    size = N.lib.vits_op_paged_attention_workspace_bytes
+    for bad in ((-1, 4, 2, 128, 0), (1, 4, 3, 128, 0), (1, 0, 1, 128, 0), (1, 4, 2, 40, 0), (1, 4, 2, 512, 0)):
+        assert size(*bad) == -1
+    need = size(3, 4, 2, 128, 1 << 20)
+    assert need >= 0 and size(0, 4, 2, 128, 0) >= 0
+    if need:
+        refused(N.lib.vits_op_paged_attention(*{**ATTEND, "max_keys": 1 << 20, "ws_bytes": need - 1}.values()), "workspace", WORKSPACE)
+        refused(N.lib.vits_op_paged_attention(*{**ATTEND, "max_keys": 1 << 20, "ws": 0}.values()), "workspace", WORKSPACE)
+        refused(N.lib.vits_op_paged_attention(*{**ATTEND, "max_keys": 1 << 20, "ws": P + 8}.values()), "workspace", WORKSPACE)
+
+
+def test_python_functions_refuse_host_tensors():
+    pages = ops.new_pages(3, 4, 20, device="cpu")
+    with pytest.raises(ValueError, match="GPU"):
+        ops.page_plan(pages.lengths, torch.zeros(3, dtype=torch.int32), pages.table, pages.ring, pages.cursor, 16, rows=4)
+    with pytest.raises(ValueError, match="rows or out"):
+        ops.page_plan(pages.lengths, torch.zeros(3, dtype=torch.int32), pages.table, pages.ring, pages.cursor, 16)
+    q, cache = torch.zeros(2, 4, 64), torch.zeros(20, 2, 16, 64)
+    i32 = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.rotary_store(q, None, None, None, None, i32, None, ops.rotary_frequencies(64, device="cpu"))
+    with pytest.raises(ValueError, match="neither"):
+        ops.rotary_store(None, None, None, None, None, i32, None, ops.rotary_frequencies(64, device="cpu"))
+    with pytest.raises(ValueError, match="GPU"):
+        ops.paged_attention(q, cache, cache, pages.table, i32, i32)
+
+
+def test_python_checks():
+    """The functions that the operators' argument checks are made of, on host tensors."""
+    x = torch.zeros(4, 3, 8)
+    ops._rows("t", "x", x, 4, 3, 8, torch.float32)
+    for bad in (x.half(), x[:3], x[:, :2], x[..., :7], x.transpose(1, 2).contiguous().transpose(1, 2)):
+        with pytest.raises(ValueError, match="t: x must be"):
+            ops._rows("t", "x", bad, 4, 3, 8, torch.float32)
+    n = torch.zeros(6, dtype=torch.int32)
+    ops._flat("t", "n", n, torch.int32, 6)
+    for bad in (n.long(), n[:5], n.view(2, 3), torch.zeros(12, dtype=torch.int32)[::2]):
+        with pytest.raises(ValueError, match="t: n must be"):
+            ops._flat("t", "n", bad, torch.int32, 6)
+    cache = torch.zeros(5, 2, 2, 16, 8)                        # keys and values of a page side by side
+    ops._caches("t", cache[:, 0], cache[:, 1])
+    for k, v in ((cache[:, 0], cache[:4, 1]), (cache[:, 0], cache[:, 1].half()), (cache[:, 0], cache[:, 1].contiguous()),
+                 (cache[0], cache[0][:1]), (cache[:, 0].transpose(1, 2), cache[:, 1].transpose(1, 2)), (cache[:, 0].long(), cache[:, 1].long())):
+        with pytest.raises(ValueError, match="t: "):
+            ops._caches("t", k, v)
+    with pytest.raises(ValueError, match="table"):
+        ops._table("t", torch.zeros(4, 6, dtype=torch.int32)[:, ::2])
+    buf = torch.zeros(100)
+    ops._apart("t", buf[:50], buf[50:])
+    ops._apart("t", buf[10:10], buf)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops._apart("t", buf[:51], buf[50:])
+
+
+def test_rotary_frequencies():
+    f = ops.rotary_frequencies(8, device="cpu")
+    assert f.dtype == torch.float64 and f.tolist() == pytest.approx([1.0, 0.1, 0.01, 0.001], rel=1e-14)
+    assert ops.rotary_frequencies(8, factor=4, scaling="linear", device="cpu").tolist() == pytest.approx([x / 4 for x in f.tolist()], rel=1e-14)
+    raised = ops.rotary_frequencies(8, factor=4, scaling="base", device="cpu")
+    assert raised[0] == 1.0 and float(raised[3]) == pytest.approx(0.001 / 4, rel=1e-12)
+    # pairs that turn more than 32 times in 4096 positions stay, those that turn less than once are divided, those between lie between
+    plain = ops.rotary_frequencies(128, device="cpu")
+    ramp = ops.rotary_frequencies(128, factor=8, scaling="ramp", device="cpu")
+    turns = 4096 * plain / (2 * math.pi)
+    assert torch.equal(ramp[turns > 32], plain[turns > 32])
+    assert torch.allclose(ramp[turns < 1], plain[turns < 1] / 8, rtol=1e-14)
+    between = (turns > 1) & (turns < 32)
+    assert between.any() and bool(((ramp < plain) & (ramp > plain / 8))[between].all())
+    assert ops.rotary_frequencies(2, factor=3, scaling="base", device="cpu").tolist() == [1.0]
+    for bad in (dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_dim=8, factor=0.5), dict(rotary_dim=8, base=1.0),
+                dict(rotary_dim=8, scaling="other"), dict(rotary_dim=8, scaling="ramp", fast=1.0, slow=1.0), dict(rotary_dim=8, factor=math.nan)):
+        with pytest.raises(ValueError):
+            ops.rotary_frequencies(**bad, device="cpu")

@@ -11,7 +11,7 @@ BASE="$(basename "$SRC" .hip)"
   -Xclang -target-feature -Xclang -packed-fp32-ops $EXTRA \
   -c "$R/vits_amd/csrc/$BASE.hip" -o "$V/${BASE}_$NAME.o"
 OBJS=""
-for o in kernels_conv kernels_gl16 kernels_chain kernels_misc model; do
+for o in kernels_conv kernels_gl16 kernels_chain kernels_misc kernels_paged model; do
   if [ "$o" == "$BASE" ]; then OBJS="$OBJS $V/${BASE}_$NAME.o"; else OBJS="$OBJS $L/$o.o"; fi
 done
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o "$V/libvits_$NAME.so" $OBJS

@@ -96,6 +96,12 @@ def _load():
         "vits_op_layer_norm": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, vp]),
         "vits_op_attention": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp]),
         "vits_op_attention_prec": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
+        "vits_op_page_plan": (i32, [vp, vp, i32, vp, i64, i32, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, i32, vp, vp]),
+        "vits_op_rotary_store": (i32, [vp, i64, i64, vp, i64, i64, i32, vp, i64, i64, vp, i64, i64, vp, vp, i64, i32, i32, i32,
+                                       i32, i32, vp, vp, i32, vp, i32, f32, i32, vp, vp]),
+        "vits_op_paged_attention_workspace_bytes": (i64, [i32, i32, i32, i32, i64]),
+        "vits_op_paged_attention": (i32, [vp, i64, i64, vp, vp, i64, i32, i32, vp, i64, i32, i32, vp, vp, i32, i32, i32, i32,
+                                          i32, f32, i32, i64, vp, i64, i64, vp, vp, vp, i64, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)      # AttributeError here means the library does not match include/vits_amd.h
@@ -111,6 +117,8 @@ PREC_F32, PREC_BF16X3, PREC_BF16, PREC_F16X2 = 0, 1, 2, 3
 PRECISIONS = {"fp32": PREC_F32, "bf16x3": PREC_BF16X3, "bf16": PREC_BF16, "f16x2": PREC_F16X2}
 F_IN_LRELU, F_IN_MASK, F_RELU, F_MASK_PRE, F_RES, F_RES_SUB, F_ACCUM, F_MASK_POST = (1 << i for i in range(8))
 F_OUT_STAGED, F_IN_STAGED = 1 << 8, 1 << 9
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+PLAN_BAD_LENGTH, PLAN_TABLE_FULL, PLAN_ROWS_FULL, PLAN_NO_PAGES, PLAN_BAD_RING = 1, 2, 4, 8, 16
 
 
 def check(rc: int, what: str = "") -> None:

@@ -10,7 +10,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libvits_amd.so")
-SOURCES = ["kernels_conv.hip", "kernels_gl16.hip", "kernels_chain.hip", "kernels_misc.hip", "model.hip"]
+SOURCES = ["kernels_conv.hip", "kernels_gl16.hip", "kernels_chain.hip", "kernels_misc.hip", "kernels_paged.hip",
+           "model.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # no packed fp32 arithmetic (v_pk_add_f32 and its like, which -O3 makes of ordinary float code): some of its forms have
 # given wrong results now and then.  The host pass does not know the feature and says so; that is harmless.
@@ -28,12 +29,14 @@ def _stale(target: str, deps) -> bool:
 def build(force: bool = False, verbose: bool = True) -> str:
     os.makedirs(LIBDIR, exist_ok=True)
     headers = [os.path.join(CSRC, "common.h"), os.path.join(os.path.dirname(HERE), "include", "vits_amd.h")]
+    paged = [os.path.join(CSRC, "paged.h")] + headers[1:]
+    deps = {"kernels_paged.hip": paged, "model.hip": headers + paged}
     objs, jobs = [], []
     for src in SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(LIBDIR, src.replace(".hip", ".o"))
         objs.append(o)
-        if force or _stale(o, [s] + headers):
+        if force or _stale(o, [s] + deps.get(src, headers[:1])):
             jobs.append([HIPCC, *FLAGS, "-c", s, "-o", o])
 
     def run(cmd):

@@ -1,7 +1,8 @@
 // Host side of libvits_amd.so: model registry, stage orchestration and the C ABI declared in include/vits_amd.h.
-// Each stage function enqueues hand-written kernels (kernels_conv.hip, kernels_misc.hip) on the caller's stream and
+// Each stage function enqueues hand-written kernels (kernels_*.hip) on the caller's stream and
 // allocates nothing; activations live in the caller's workspace.
 #include "common.h"
+#include "paged.h"
 #include "../../include/vits_amd.h"
 
 #include <cmath>
@@ -338,6 +339,23 @@ ConvDesc need_conv(vits_model* m, const std::string& name, int cin, int rows, in
     return ConvDesc();
   }
   return d;
+}
+
+}  // namespace
+
+namespace {
+// shared checks of the paged-cache operators
+int check_page_size(int page_size) {
+  if (page_size < PAGED_PAGE_UNIT || page_size % PAGED_PAGE_UNIT || page_size > 65536)
+    return fail(VITS_ERR_INVALID, "page_size must be a multiple of 16 and at most 65536");
+  return VITS_OK;
+}
+
+int check_att_shape(int rows, int heads, int kv_heads, int dim) {
+  if (rows < 0 || kv_heads < 1 || heads < 1 || heads > PAGED_MAX_HEADS || heads % kv_heads || dim < 32 || dim > PAGED_MAX_DIM || dim % 32)
+    return fail(VITS_ERR_INVALID, "paged attention: 1 to 1024 query heads in equal groups over the key-value heads, and heads of "
+                                  "32, 64, ... 256 channels required");
+  return VITS_OK;
 }
 
 }  // namespace
@@ -1410,6 +1428,100 @@ int vits_op_attention_prec(const float* qkv, const float* emb_k, const float* em
     return fail(VITS_ERR_INVALID, "attention: precision must be bf16x3 (1) or f16x2 (3)");
   HIP_TRY(launch_attention(qkv, emb_k, emb_v, lengths, out, B, H, DK, L, window, (hipStream_t)stream,
                            precision == PREC_F16X2, g_range_flag));
+  return VITS_OK;
+}
+
+int vits_op_page_plan(const int* lengths, const int* grow, int requests, int* table, int64_t table_stride, int width,
+                      int* ring, int pages, const int64_t* cursor, int page_size, int* lengths_out, int64_t* cursor_out,
+                      int* row_start, int* row_request, int* row_position, int64_t* row_slot, int rows, int* status,
+                      void* stream) {
+  if (!lengths || !grow || !table || !ring || !cursor || !lengths_out || !cursor_out || !row_start || !status ||
+      (rows > 0 && (!row_request || !row_position || !row_slot)))
+    return fail(VITS_ERR_INVALID, "page plan: null argument");
+  if (requests < 1 || requests > 65535 || rows < 0 || rows > (1 << 30) || pages < 1 || pages > (1 << 30) || width < 1 ||
+      table_stride < width)
+    return fail(VITS_ERR_INVALID, "page plan: 1 to 65535 requests, up to 2^30 rows and pages, a table of at least one page "
+                                  "a request and rows that do not overlap required");
+  TRY(check_page_size(page_size));
+  if (lengths_out == lengths || lengths_out == grow || cursor_out == cursor)
+    return fail(VITS_ERR_INVALID, "page plan: cannot run in place (every block reads all lengths and the cursor)");
+  PagePlanArgs a{};
+  a.lengths = lengths; a.grow = grow; a.requests = requests;
+  a.table = table; a.table_stride = table_stride; a.width = width;
+  a.ring = ring; a.pages = pages; a.cursor = cursor; a.page_size = page_size;
+  a.lengths_out = lengths_out; a.cursor_out = cursor_out;
+  a.row_start = row_start; a.row_request = row_request; a.row_position = row_position; a.row_slot = row_slot;
+  a.rows = rows; a.status = status;
+  HIP_TRY(launch_page_plan(a, (hipStream_t)stream));
+  return VITS_OK;
+}
+
+int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out, int64_t out_row, int64_t out_head,
+                         int heads, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                         int64_t v_head, void* k_cache, void* v_cache, int64_t page_stride, int pages, int page_size,
+                         int kv_heads, int dim, int dtype, const int* position, const int64_t* slot, int rows,
+                         const double* freq, int pairs, float scale, int interleaved, int* err_flag, void* stream) {
+  // (no rows: an empty tensor's address may be null)
+  if (rows != 0 && (!position || !freq || (!q && !k) || (q && !out) || (k && (!v || !k_cache || !v_cache || !slot))))
+    return fail(VITS_ERR_INVALID, "rotary store: null argument");
+  if (dtype < VITS_TYPE_F32 || dtype > VITS_TYPE_BF16)
+    return fail(VITS_ERR_INVALID, "rotary store: dtype must be fp32 (0), fp16 (1) or bf16 (2)");
+  if (rows < 0 || dim < 2 || dim > PAGED_MAX_DIM || pairs < 1 || 2 * pairs > dim || (q && (heads < 1 || heads > PAGED_MAX_HEADS)) ||
+      (k && (kv_heads < 1 || kv_heads > PAGED_MAX_HEADS || pages < 1)))
+    return fail(VITS_ERR_INVALID, "rotary store: heads of 2 to 256 channels, 1 to 1024 of them, at least one turning pair and no "
+                                  "more pairs than channels hold required");
+  if (k) {
+    TRY(check_page_size(page_size));
+    if (page_stride < (int64_t)kv_heads * page_size * dim) return fail(VITS_ERR_INVALID, "rotary store: pages overlap");
+  }
+  if (q == out && q && (q_row != out_row || q_head != out_head))
+    return fail(VITS_ERR_INVALID, "rotary store: in place needs the same strides on both sides");
+  if (rows == 0) return VITS_OK;
+  RotaryArgs a{};
+  a.q = q; a.q_row = q_row; a.q_head = q_head; a.out = out; a.out_row = out_row; a.out_head = out_head; a.heads = heads;
+  a.k = k; a.k_row = k_row; a.k_head = k_head; a.v = v; a.v_row = v_row; a.v_head = v_head;
+  a.k_cache = k_cache; a.v_cache = v_cache; a.page_stride = page_stride;
+  a.pages = pages; a.page_size = page_size; a.kv_heads = kv_heads; a.dim = dim; a.dtype = dtype;
+  a.position = position; a.slot = slot; a.rows = rows;
+  a.freq = freq; a.pairs = pairs; a.scale = scale; a.interleaved = interleaved != 0; a.err_flag = err_flag;
+  HIP_TRY(launch_rotary_store(a, (hipStream_t)stream));
+  return VITS_OK;
+}
+
+int64_t vits_op_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int dim, int64_t max_keys) {
+  if (check_att_shape(rows, heads, kv_heads, dim) != VITS_OK) return -1;
+  return paged_attention_workspace(rows, heads, kv_heads, dim, max_keys);
+}
+
+int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, const void* v_cache,
+                            int64_t page_stride, int pages, int page_size, const int* table, int64_t table_stride, int width,
+                            int requests, const int* row_request, const int* row_position, int rows, int heads, int kv_heads,
+                            int dim, int dtype, float scale, int window, int64_t max_keys, void* out, int64_t out_row,
+                            int64_t out_head, float* lse, int* err_flag, void* ws, int64_t ws_bytes, void* stream) {
+  if (rows != 0 && (!q || !k_cache || !v_cache || !table || !row_request || !row_position || !out))
+    return fail(VITS_ERR_INVALID, "paged attention: null argument");
+  if (dtype < VITS_TYPE_F32 || dtype > VITS_TYPE_BF16)
+    return fail(VITS_ERR_INVALID, "paged attention: dtype must be fp32 (0), fp16 (1) or bf16 (2)");
+  TRY(check_att_shape(rows, heads, kv_heads, dim));
+  TRY(check_page_size(page_size));
+  if (pages < 1 || width < 1 || table_stride < width || requests < 1 || window < 0)
+    return fail(VITS_ERR_INVALID, "paged attention: at least one page, request and table column, rows of the table that do not "
+                                  "overlap and a window that is not negative required");
+  if (page_stride < (int64_t)kv_heads * page_size * dim) return fail(VITS_ERR_INVALID, "paged attention: pages overlap");
+  if (q && q == out) return fail(VITS_ERR_INVALID, "paged attention: cannot run in place");
+  const int size = dtype == VITS_TYPE_F32 ? 4 : 2;
+  if ((((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) || (page_stride * size) % 16)
+    return fail(VITS_ERR_INVALID, "paged attention: the caches and their pages must begin on 16-byte addresses");
+  if (ws_bytes < paged_attention_workspace(rows, heads, kv_heads, dim, max_keys) || (ws_bytes > 0 && !ws) || ((uintptr_t)ws & 15))
+    return fail(VITS_ERR_WORKSPACE, "paged attention: workspace too small or not on a 16-byte address");
+  if (rows == 0) return VITS_OK;
+  PagedAttArgs a{};
+  a.q = q; a.q_row = q_row; a.q_head = q_head; a.k_cache = k_cache; a.v_cache = v_cache; a.page_stride = page_stride;
+  a.pages = pages; a.page_size = page_size; a.table = table; a.table_stride = table_stride; a.width = width;
+  a.requests = requests; a.row_request = row_request; a.row_position = row_position;
+  a.rows = rows; a.heads = heads; a.kv_heads = kv_heads; a.dim = dim; a.dtype = dtype; a.scale = scale; a.window = window;
+  a.out = out; a.out_row = out_row; a.out_head = out_head; a.lse = lse; a.err_flag = err_flag;
+  HIP_TRY(launch_paged_attention(a, max_keys, ws, (hipStream_t)stream));
   return VITS_OK;
 }
 

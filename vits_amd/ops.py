@@ -1,0 +1,286 @@
+"""Operators around a paged key-value cache, on torch tensors: what an autoregressive model needs that is served beside
+the synthesiser (a text or prosody model whose tokens, durations or pitch go to `SynthesizerTrn.infer_batches`).
+
+    pages = ops.new_pages(requests=64, width=512, pages=20000, page_size=16, device="cuda")  # table, ring, cursor, lengths
+    k_cache, v_cache = (torch.empty(20000, kv_heads, 16, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))   # a layer
+    freq = ops.rotary_frequencies(dim, device="cuda")
+    ...
+    plan = ops.page_plan(lengths, grow, table, ring, cursor, 16, rows=R)        # once a step: which rows, pages and slots
+    q = ops.rotary_store(q, k, v, k_cache, v_cache, plan.position, plan.slot, freq)                # every layer
+    o = ops.paged_attention(q, k_cache, v_cache, table, plan.request, plan.position)
+    lengths, cursor = plan.lengths, plan.cursor
+
+The kernels are in libvits_amd.so (vits_op_page_plan, vits_op_rotary_store, vits_op_paged_attention; include/vits_amd.h has
+the formulas and the layouts); there is no fallback.  Everything runs on the current stream of the tensors' device, nothing
+waits for the GPU, and with the outputs given (`out=`, `lse=`) a call can be captured into a graph.  Wrong shapes and types
+raise ValueError, a library error VitsError; ids on the device that are out of range are left out and OR 1 into `err_flag`
+(an int32 tensor of one element), where one is given.  The reference has no counterpart (its attention, attentions.py:179-332, takes
+whole rows)."""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple, Optional, Sequence
+
+import torch
+
+from . import _native as N
+
+_TYPES = {torch.float32: N.TYPE_F32, torch.float16: N.TYPE_F16, torch.bfloat16: N.TYPE_BF16}
+
+
+class PagePlan(NamedTuple):
+    """What `page_plan` gives, in the order of its `out`."""
+    lengths: torch.Tensor    # int32 [requests]      tokens in the cache after the step
+    cursor: torch.Tensor     # int64 [2]             head and tail of the ring after the step
+    start: torch.Tensor      # int32 [requests + 1]  where each request's rows begin, and how many there are
+    request: torch.Tensor    # int32 [rows]          -1 behind the last
+    position: torch.Tensor   # int32 [rows]
+    slot: torch.Tensor       # int64 [rows]
+    status: torch.Tensor     # int32 [1]             0, or the OR of _native.PLAN_*: nothing was taken
+
+
+class Pages(NamedTuple):
+    """An empty cache's bookkeeping."""
+    lengths: torch.Tensor    # int32 [requests]
+    table: torch.Tensor      # int32 [requests, width]
+    ring: torch.Tensor       # int32 [pages]
+    cursor: torch.Tensor     # int64 [2]
+
+
+def new_pages(requests: int, width: int, pages: int, device="cuda") -> Pages:
+    """No request holds a token, and every page is free; a request can hold `width` pages."""
+    i32 = dict(dtype=torch.int32, device=device)
+    return Pages(torch.zeros(requests, **i32), torch.full((requests, width), -1, **i32), torch.arange(pages, **i32),
+                 torch.tensor([0, pages], dtype=torch.int64, device=device))
+
+
+def _on_gpu(what: str, first: torch.Tensor, *more) -> torch.device:
+    device = first.device
+    if device.type != "cuda":
+        raise ValueError(f"{what}: tensors must be on a GPU (vits_amd has no CPU path)")
+    for t in more:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: all tensors must be on one GPU, got {t.device} and {device}")
+    return device
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _flat(what: str, name: str, t: torch.Tensor, dtype, n: Optional[int] = None) -> None:
+    if t.dtype != dtype or t.dim() != 1 or (n is not None and t.numel() != n) or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be contiguous {dtype} [{'n' if n is None else n}], got {t.dtype} {list(t.shape)}")
+
+
+def _rows(what: str, name: str, t: torch.Tensor, rows: int, heads: Optional[int], dim: int, dtype) -> None:
+    if t.dtype != dtype or t.dim() != 3 or t.shape[0] != rows or (heads is not None and t.shape[1] != heads) or t.shape[2] != dim \
+            or (t.stride(2) != 1 and dim > 1):
+        raise ValueError(f"{what}: {name} must be {dtype} [{rows}, {'heads' if heads is None else heads}, {dim}] with contiguous "
+                         f"channels, got {t.dtype} {list(t.shape)}, strides {list(t.stride())}")
+
+
+def _table(what: str, table: torch.Tensor) -> None:
+    if table.dtype != torch.int32 or table.dim() != 2 or (table.stride(1) != 1 and table.shape[1] > 1):
+        raise ValueError(f"{what}: table must be int32 [requests, width] with contiguous rows, got {table.dtype} {list(table.shape)}")
+
+
+def _caches(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
+    for t in (k_cache, v_cache):
+        if t.dim() != 4 or t.dtype not in _TYPES:
+            raise ValueError(f"{what}: caches must be fp32, fp16 or bf16 [pages, kv_heads, page_size, dim], got {t.dtype} {list(t.shape)}")
+    _, _, page, dim = k_cache.shape
+    if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype or k_cache.stride() != v_cache.stride() \
+            or k_cache.stride()[1:] != (page * dim, dim, 1):
+        raise ValueError(f"{what}: k_cache and v_cache must be alike and contiguous within a page, got {list(k_cache.shape)} and "
+                         f"{list(v_cache.shape)}, strides {list(k_cache.stride())} and {list(v_cache.stride())}")
+
+
+def _err_flag(what: str, flag: Optional[torch.Tensor]) -> int:
+    if flag is None:
+        return 0
+    _flat(what, "err_flag", flag, torch.int32, 1)
+    return flag.data_ptr()
+
+
+def _span(t: torch.Tensor):
+    """First and last byte of a tensor's elements, as a half-open range."""
+    n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def _apart(what: str, a: torch.Tensor, b: torch.Tensor) -> None:
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a0 < b1 and b0 < a1:
+        raise ValueError(f"{what}: an output overlaps an input")
+
+
+def page_plan(lengths: torch.Tensor, grow: torch.Tensor, table: torch.Tensor, ring: torch.Tensor, cursor: torch.Tensor, page_size: int,
+              rows: Optional[int] = None, out: Optional[Sequence[torch.Tensor]] = None) -> PagePlan:
+    """One step of a serving loop, planned on the GPU: request s gets grow[s] new tokens (or ends: -1), `table` its new
+    pages from `ring`, and every new token a row with its request, position and slot; -1 in rows behind the last.
+    `rows` is how many there may be (default: as `out` holds).  table and ring are changed in place; the new lengths and
+    cursor are returned beside the old ones, so the caller decides when the step counts.  Where the step does not fit,
+    `status` says why and nothing is changed."""
+    what = "page_plan"
+    n = lengths.numel()
+    if out is None:
+        if rows is None:
+            raise ValueError("page_plan: give rows or out")
+        i32 = dict(dtype=torch.int32, device=lengths.device)
+        i64 = dict(dtype=torch.int64, device=lengths.device)
+        out = (torch.empty(n, **i32), torch.empty(2, **i64), torch.empty(n + 1, **i32), torch.empty(rows, **i32),
+               torch.empty(rows, **i32), torch.empty(rows, **i64), torch.empty(1, **i32))
+    elif len(out) != 7:
+        raise ValueError("page_plan: out must hold a PagePlan's seven tensors")
+    plan = PagePlan(*out)
+    if rows is None:
+        rows = plan.request.numel()
+    i32, i64 = torch.int32, torch.int64
+    device = _on_gpu(what, lengths, grow, table, ring, cursor, *plan)
+    for name, t, dtype, k in (("lengths", lengths, i32, n), ("grow", grow, i32, n), ("ring", ring, i32, None), ("cursor", cursor, i64, 2),
+                              ("out.lengths", plan.lengths, i32, n), ("out.cursor", plan.cursor, i64, 2),
+                              ("out.start", plan.start, i32, n + 1), ("out.request", plan.request, i32, rows),
+                              ("out.position", plan.position, i32, rows), ("out.slot", plan.slot, i64, rows),
+                              ("out.status", plan.status, i32, 1)):
+        _flat(what, name, t, dtype, k)
+    _table(what, table)
+    if table.shape[0] != n:
+        raise ValueError(f"page_plan: table has {table.shape[0]} rows for {n} requests")
+    for i in (lengths, grow, cursor):
+        for o in (table, ring, *plan):
+            _apart(what, i, o)
+    with torch.cuda.device(device):
+        N.check(N.lib.vits_op_page_plan(
+            lengths.data_ptr(), grow.data_ptr(), n, table.data_ptr(), table.stride(0), table.shape[1], ring.data_ptr(), ring.numel(),
+            cursor.data_ptr(), page_size, plan.lengths.data_ptr(), plan.cursor.data_ptr(), plan.start.data_ptr(),
+            plan.request.data_ptr(), plan.position.data_ptr(), plan.slot.data_ptr(), rows, plan.status.data_ptr(), _stream(device)), what)
+    return plan
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original_length: int = 4096,
+                       fast: float = 32.0, slow: float = 1.0, device="cuda") -> torch.Tensor:
+    """Radians a position for each of the rotary_dim / 2 pairs, in 64 bits: base^(-2i / rotary_dim), for contexts `factor`
+    times as long as the trained ones as they are ("none"), divided by the factor ("linear": positions are interpolated),
+    with the base raised so that the slowest pair is divided by the factor and the fastest kept ("base"), or ("ramp")
+    divided by it for pairs that turn less than `slow` times within original_length, kept for those that turn more than
+    `fast` times, and blended linearly in the number of turns between (`rotary_store`'s `scale` takes the factor on the
+    vectors that goes with it)."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rotary_frequencies: rotary_dim must be even and positive")
+    if not factor >= 1.0 or not base > 1.0:
+        raise ValueError("rotary_frequencies: factor must be at least 1 and base above 1")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    if scaling == "base" and rotary_dim > 2:
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    freq = base ** (-i / rotary_dim)
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "ramp":
+        if not fast > slow:
+            raise ValueError("rotary_frequencies: fast must be above slow")
+        keep = ((original_length * freq / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+        freq = freq / factor * (1 - keep) + freq * keep
+    elif scaling not in ("none", "base"):
+        raise ValueError("rotary_frequencies: scaling must be 'none', 'linear', 'base' or 'ramp'")
+    return freq.to(device)
+
+
+def rotary_store(q: Optional[torch.Tensor], k: Optional[torch.Tensor], v: Optional[torch.Tensor], k_cache: Optional[torch.Tensor],
+                 v_cache: Optional[torch.Tensor], position: torch.Tensor, slot: Optional[torch.Tensor], freq: torch.Tensor,
+                 interleaved: bool = False, scale: float = 1.0, out: Optional[torch.Tensor] = None,
+                 err_flag: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Turns q [rows, heads, dim] by its rows' positions into `out` (new, given, or q itself), and k [rows, kv_heads, dim]
+    into k_cache at the rows' slots, where v goes too, unturned.  The first 2 * freq.numel() channels of a head turn.
+    Rows of slot < 0 are left as they were.  q may be None (nothing is returned), or k, v and the caches (then slot may be
+    too).  With q alone and -freq it is its own gradient.  The slots of one call have to differ."""
+    what = "rotary_store"
+    if q is None and k is None:
+        raise ValueError("rotary_store: neither queries nor keys")
+    first = q if q is not None else k
+    if first.dim() != 3 or first.dtype not in _TYPES:
+        raise ValueError(f"rotary_store: rows must be fp32, fp16 or bf16 [rows, heads, dim], got {first.dtype} {list(first.shape)}")
+    rows, _, dim = first.shape
+    device = _on_gpu(what, first, k, v, k_cache, v_cache, position, slot, freq, out, err_flag)
+    _flat(what, "position", position, torch.int32, rows)
+    _flat(what, "freq", freq, torch.float64)
+    if slot is not None:
+        _flat(what, "slot", slot, torch.int64, rows)
+    qa = oa = (0, 0, 0)
+    heads = 0
+    if q is not None:
+        heads = q.shape[1]
+        _rows(what, "q", q, rows, heads, dim, first.dtype)
+        if out is None:
+            out = torch.empty((rows, heads, dim), dtype=q.dtype, device=device)
+            if slot is not None:
+                out.zero_()                     # rows that are no rows are left as they were: not as the allocator found them
+        else:
+            _rows(what, "out", out, rows, heads, dim, first.dtype)
+            if out.data_ptr() != q.data_ptr() or out.stride() != q.stride():
+                _apart(what, q, out)
+        qa, oa = ((t.data_ptr(), t.stride(0), t.stride(1)) for t in (q, out))
+    elif out is not None:
+        raise ValueError("rotary_store: out without q")
+    ka = va = (0, 0, 0)
+    kc = vc = page_stride = pages = page_size = kv_heads = 0
+    if k is not None:
+        if v is None or k_cache is None or v_cache is None or slot is None:
+            raise ValueError("rotary_store: keys need values, both caches and slots")
+        _caches(what, k_cache, v_cache)
+        pages, kv_heads, page_size, _ = k_cache.shape
+        for name, t in (("k", k), ("v", v)):
+            _rows(what, name, t, rows, kv_heads, dim, first.dtype)
+        if k_cache.dtype != first.dtype or k_cache.shape[3] != dim:
+            raise ValueError(f"rotary_store: caches of {k_cache.dtype} with {k_cache.shape[3]} channels for rows of {first.dtype} with {dim}")
+        ka, va = ((t.data_ptr(), t.stride(0), t.stride(1)) for t in (k, v))
+        kc, vc, page_stride = k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0)
+    elif v is not None or k_cache is not None or v_cache is not None:
+        raise ValueError("rotary_store: values or caches without keys")
+    with torch.cuda.device(device):
+        N.check(N.lib.vits_op_rotary_store(
+            *qa, *oa, heads, *ka, *va, kc, vc, page_stride, pages, page_size, kv_heads, dim, _TYPES[first.dtype], position.data_ptr(),
+            N.ptr(slot), rows, freq.data_ptr(), freq.numel(), scale, int(interleaved), _err_flag(what, err_flag), _stream(device)), what)
+    return out
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, request: torch.Tensor,
+                    position: torch.Tensor, scale: Optional[float] = None, window: int = 0, max_keys: Optional[int] = None,
+                    out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                    err_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Every row of q [rows, heads, dim] attends to its request's tokens up to and with its own position (the last `window` of
+    them, where that is not 0); heads / kv_heads query heads share a key-value head.  scale: 1 / sqrt(dim) by default.  A row
+    that sees nothing gives 0, a row of request < 0 is left as it was (0 in an `out` made here).  lse (fp32 [rows, heads],
+    optional) receives the log of the sum of the exponentials.  max_keys: the most tokens a row can see as far as the host
+    knows, which guides how the work is split; the result does not depend on it beyond rounding."""
+    what = "paged_attention"
+    if q.dim() != 3:
+        raise ValueError(f"paged_attention: q must be [rows, heads, dim], got {list(q.shape)}")
+    rows, heads, dim = q.shape
+    device = _on_gpu(what, q, k_cache, v_cache, table, request, position, out, lse, err_flag)
+    _caches(what, k_cache, v_cache)
+    pages, kv_heads, page_size, _ = k_cache.shape
+    _rows(what, "q", q, rows, heads, k_cache.shape[3], k_cache.dtype)
+    _flat(what, "request", request, torch.int32, rows)
+    _flat(what, "position", position, torch.int32, rows)
+    _table(what, table)
+    if out is None:
+        out = torch.zeros((rows, heads, dim), dtype=q.dtype, device=device)
+    else:
+        _rows(what, "out", out, rows, heads, dim, q.dtype)
+        _apart(what, q, out)
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous()):
+        raise ValueError(f"paged_attention: lse must be contiguous float32 [{rows}, {heads}], got {lse.dtype} {list(lse.shape)}")
+    keys = table.shape[1] * page_size if max_keys is None else max_keys
+    nbytes = N.lib.vits_op_paged_attention_workspace_bytes(rows, heads, kv_heads, dim, keys)
+    if nbytes < 0:
+        N.check(-1, what)
+    # a workspace of this call's own: calls on different streams, and graphs that run side by side, share none
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    with torch.cuda.device(device):
+        N.check(N.lib.vits_op_paged_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), pages, page_size,
+            table.data_ptr(), table.stride(0), table.shape[1], table.shape[0], request.data_ptr(), position.data_ptr(), rows, heads,
+            kv_heads, dim, _TYPES[q.dtype], 1.0 / math.sqrt(dim) if scale is None else scale, window, keys, out.data_ptr(),
+            out.stride(0), out.stride(1), N.ptr(lse), _err_flag(what, err_flag), N.ptr(ws), nbytes, _stream(device)), what)
+    return out
