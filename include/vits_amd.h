@@ -317,7 +317,7 @@ int vits_op_page_plan(const int* lengths, const int* grow, int requests, int* ta
  * k, v and the caches (then slot may be NULL too: every row is one).  Computed in fp32, rounded once.  The slots of one
  * call have to differ: where two rows share one, each stored value is either row's.  Scaled positions are scaled
  * frequencies (vits_amd/ops.py: rotary_frequencies); the gradient with respect to q is the same call on the gradient of
- * out with -freq.  dim 2 .. 256. */
+ * out with -freq.  dim 2 .. 256, at most 2^23 rows. */
 int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out, int64_t out_row, int64_t out_head,
                          int heads, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                          int64_t v_head, void* k_cache, void* v_cache, int64_t page_stride, int pages, int page_size,
@@ -329,7 +329,7 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
  * h / (heads / kv_heads).  A row that sees no token (position < 0) gives 0.  lse [rows][heads] fp32 or NULL: log of the sum
  * of exp(scale * q . k_t), -inf for such a row.  Scores, softmax and sums in fp32.  What lies in the cache behind a row's
  * position, and in pages the table does not name for it, has no influence whatever it holds.
- * dim: 32, 64, ... 256; caches and pages begin on 16-byte addresses.  max_keys: how many tokens the host knows a row to see
+ * dim: 32, 64, ... 256; at most 2^23 rows and, by the table, 2^30 tokens a request; caches and pages begin on 16-byte addresses.  max_keys: how many tokens the host knows a row to see
  * at most (0: as many as the table holds); it only guides how the work is split, a row that sees more is right all
  * the same.  ws: vits_op_paged_attention_workspace_bytes of the same numbers (-1 for a shape that is refused). */
 int64_t vits_op_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int dim, int64_t max_keys);

@@ -355,71 +355,646 @@ hipError_t start_rotary_t(RotaryArgs a, hipStream_t s) {
 
 // ---------------------------------------------------------------------------------------------------------
 // attention of single rows over the cache
+//
+// Per key-value head the query heads of its group, for up to 16 / group rows of one request that stand beside each other (a
+// single new token, drafted tokens, a prompt's rows), are the 16 columns of a matrix product: S^T = K Q^T with 16 keys as
+// rows, then O^T = V^T P^T.  In both the result's column is lane & 15, so a column's maximum, sum and rescaling factor
+// stay in the lanes that hold its scores and its output.  The contraction of the second product runs over the keys in
+// the order the first one leaves them in the lanes (lane group g = lane / 16 holds keys 4g .. 4g + 3 of each 16), so the
+// weights go from one to the other without leaving their lane; V's rows are loaded to match: lane group g loads those
+// same rows, lane n of it the channels n * DIM / 16 and on, whole rows in one instruction.  Nothing of the cache passes
+// through LDS, and no wave waits for another inside the loop over the keys.
+// 16-bit types: v_mfma_f32_16x16x32, 32 keys a step; v_perm pairs the rows' channels to operands.  fp32: v_mfma_f32_16x16x4,
+// 16 keys a step.  bf16 weights go in as two terms (w = h + l, 2^-17 relative): the product's matrix time is a small part of the
+// load time; fp16 weights as one (2^-12 relative).
 // ---------------------------------------------------------------------------------------------------------
-constexpr int ATT_WAVES = 4;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x3a __attribute__((ext_vector_type(3), aligned(4)));
+typedef unsigned u32x2a __attribute__((ext_vector_type(2), aligned(4)));
+typedef unsigned u32x4a __attribute__((ext_vector_type(4), aligned(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// One block per row and query head; the waves take keys in turn, lanes hold channels lane, lane + 64, ...
-template <typename T>
-__global__ __launch_bounds__(ATT_WAVES * WAVE) void paged_attention_kernel(PagedAttArgs a) {
-  __shared__ float part[ATT_WAVES][PAGED_MAX_DIM + 2];
-  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+constexpr int ATT_WAVES = 4;
+constexpr int ATT_THREADS = ATT_WAVES * WAVE;
+constexpr int ATT_COLS = 16;                 // columns of the products: (row of a run, query head)
+constexpr int ATT_MIN_STEPS = 8;             // the least a block takes of a split length: two steps a wave
+constexpr float ATT_SLACK = 8.f;             // the running maximum follows once it is exceeded by 2^8: weights stay below 256
+
+// max and sum over the four lanes of a column (lane, lane ^ 16, lane ^ 32, lane ^ 48)
+__device__ __forceinline__ float col_max(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float col_sum(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Work is laid out on one line, in steps of STEP keys: run after run (a run: rows of one request, up to rows_per_run of
+// them beside each other), for each run its units (key-value head, 16 query heads of its group) one after the other, for
+// each unit the run's keys.  A run that sees no key has one step, in which everything is masked.
+struct AttPlan {
+  int rows_per_run;        // 16 / group, at least 1
+  int tiles;               // 16-column tiles of a group
+  int units;               // kv_heads * tiles
+  int blocks;              // blocks the line is cut for (split form)
+  int wide_q;              // queries lie on 16-byte addresses
+};
+
+struct Run {
+  int row, n, req;
+  int begin, end;          // keys that any of its rows sees: begin a multiple of 16
+};
+
+template <typename T> constexpr int att_step() { return sizeof(T) == 2 ? 32 : 16; }
+
+// a row's keys [begin, end); true if its position lies outside the table
+__device__ __forceinline__ bool att_row_keys(const PagedAttArgs& a, int row, int& begin, int& end) {
+  const long long cap = (long long)a.width * a.page_size, stop = (long long)a.row_position[row] + 1;
+  const long long first = a.window > 0 && stop > a.window ? stop - a.window : 0;
+  end = (int)(stop < 0 ? 0 : stop < cap ? stop : cap);
+  begin = (int)(first < end ? first : end);
+  return stop > cap;
+}
+
+// whether a run begins at `row`, and what it is
+__device__ __forceinline__ bool att_run(const PagedAttArgs& a, const AttPlan& p, int row, Run& r) {
   const int req = a.row_request[row];
-  if (req < 0) return;
-  if (req >= a.requests) {
-    if (a.err_flag && threadIdx.x == 0) atomicOr(a.err_flag, 1);
+  if (req < 0 || req >= a.requests) return false;
+  const int in = row % p.rows_per_run;
+  if (in > 0 && a.row_request[row - 1] == req) return false;
+  r.row = row;
+  r.req = req;
+  const int most = min(p.rows_per_run - in, a.rows - row);
+  int n = 1;
+  att_row_keys(a, row, r.begin, r.end);
+  if (r.begin == r.end) r.begin = 0x7fffffff;
+  for (; n < most && a.row_request[row + n] == req; ++n) {
+    int b, e;
+    att_row_keys(a, row + n, b, e);
+    if (b < e) r.begin = min(r.begin, b);
+    r.end = max(r.end, e);
+  }
+  r.n = n;
+  r.begin = r.begin >= r.end ? 0 : r.begin & ~15;
+  return true;
+}
+
+template <int STEP>
+__device__ __forceinline__ int att_run_steps(const Run& r) {
+  return max(1, (r.end - r.begin + STEP - 1) / STEP);
+}
+
+// what a block leaves of a unit that it has not taken whole: [0] for the one it begins in the middle of, [1] for the one
+// it ends in the middle of; joined by paged_join_kernel
+__host__ __device__ __forceinline__ float* att_slot(float* ws, int block, int which, int dim) {
+  return ws + ((long long)block * 2 + which) * ATT_COLS * (dim + 4);
+}
+struct AttJoin {           // a unit that begins in a block and ends in a later one
+  int row, n, unit, parts; // parts: the blocks behind this one that hold some of it; 0: there is none
+};
+
+// Column m of a unit: its row (of the run's n) and head, false if there is none
+__device__ __forceinline__ bool att_column(int m, int n, int group, int tile, int& row, int& head) {
+  if (group <= ATT_COLS) {
+    row = m / group;
+    head = m - row * group;
+    return row < n;
+  }
+  row = 0;
+  head = tile * ATT_COLS + m;
+  return head < group;
+}
+
+__device__ __forceinline__ float att_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <typename T, int DIM>
+struct AttTile {
+  static constexpr bool HALF = sizeof(T) == 2;
+  static constexpr int SUB = HALF ? 2 : 1;              // 16-key parts of a step
+  static constexpr int STEP = 16 * SUB;
+  static constexpr int KL = DIM * (int)sizeof(T) / 64;   // 16-byte loads of a lane for 16 keys
+  static constexpr int CH = DIM / 16;                   // channels of a lane in V and in the output
+  static constexpr int VW = CH * (int)sizeof(T) / 4;     // dwords of a lane for one row of V
+  static constexpr int ROW = DIM + 4;                   // floats of a column in LDS and in the workspace, padded
+
+  u32x4 q[KL], k[SUB][KL];
+  unsigned v[SUB][4][VW];
+  f32x4 o[CH];
+  float top, sum;                                       // of this lane's column: running maximum (base 2), and this lane's part of the sum
+
+  __device__ __forceinline__ void load_k(int s, const T* page, int lane) {
+    const char* p = (const char*)page + (lane & 15) * (DIM * sizeof(T)) + (lane >> 4) * 16;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) k[s][i] = *(const u32x4*)(p + 64 * i);
+  }
+  __device__ __forceinline__ void load_v(int s, const T* page, int lane) {
+    const char* p = (const char*)page + (lane >> 4) * (4 * DIM * sizeof(T)) + (lane & 15) * (VW * 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const char* r = p + j * (DIM * sizeof(T));
+      int w = 0;
+#pragma unroll
+      for (; w + 4 <= VW; w += 4) {
+        const u32x4a x = *(const u32x4a*)(r + 4 * w);
+        v[s][j][w] = x[0]; v[s][j][w + 1] = x[1]; v[s][j][w + 2] = x[2]; v[s][j][w + 3] = x[3];
+      }
+      if constexpr (VW % 4 == 3) {
+        const u32x3a x = *(const u32x3a*)(r + 4 * w);
+        v[s][j][w] = x[0]; v[s][j][w + 1] = x[1]; v[s][j][w + 2] = x[2];
+      } else if constexpr (VW % 4 == 2) {
+        const u32x2a x = *(const u32x2a*)(r + 4 * w);
+        v[s][j][w] = x[0]; v[s][j][w + 1] = x[1];
+      } else if constexpr (VW % 4 == 1) {
+        v[s][j][w] = *(const unsigned*)(r + 4 * w);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void scores(f32x4 (&s)[SUB]) const {
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
+        if constexpr (!HALF) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[u][i][e]), __uint_as_float(q[i][e]), c, 0, 0, 0);
+        } else if constexpr (__is_same(T, __bf16)) {
+          c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[u][i]), __builtin_bit_cast(bf16x8, q[i]), c, 0, 0, 0);
+        } else {
+          c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[u][i]), __builtin_bit_cast(f16x8, q[i]), c, 0, 0, 0);
+        }
+      }
+      s[u] = c;
+    }
+    // The scores are read in another block of the program than this one, which the compiler (ROCm 7.2) reaches over a taken branch
+    // without the wait that a matrix instruction's result needs (up to 11 issue slots): the fp32 form at 64 channels read
+    // scores of the step before.  So they are waited for here.
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) asm volatile("s_nop 15" : "+v"(s[u]));
+  }
+
+  // acc += V^T P^T, with the rows of V that `see` (one bit a key of this lane: 4 * part + row) leaves out taken as zero
+  template <bool MASKED>
+  __device__ __forceinline__ void weigh(f32x4 (&acc)[CH], const f32x4 (&p)[SUB], unsigned see) const {
+    if constexpr (!HALF) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const unsigned x = MASKED && !(see >> j & 1) ? 0u : v[0][j][c];
+          acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x), p[0][j], acc[c], 0, 0, 0);
+        }
+    } else {
+      u32x4 hi, lo;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const f32x2 w = {p[u][2 * e], p[u][2 * e + 1]};
+          if constexpr (__is_same(T, __bf16)) {
+            const bf16x2 h = __builtin_convertvector(w, bf16x2);
+            hi[2 * u + e] = __builtin_bit_cast(unsigned, h);
+            lo[2 * u + e] = __builtin_bit_cast(unsigned, __builtin_convertvector(w - __builtin_convertvector(h, f32x2), bf16x2));
+          } else {
+            hi[2 * u + e] = __builtin_bit_cast(unsigned, __builtin_convertvector(w, f16x2));
+          }
+        }
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        u32x4 even, odd;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            unsigned x = v[u][2 * e][w], y = v[u][2 * e + 1][w];
+            if (MASKED) {
+              x = see >> (4 * u + 2 * e) & 1 ? x : 0u;
+              y = see >> (4 * u + 2 * e + 1) & 1 ? y : 0u;
+            }
+            even[2 * u + e] = __builtin_amdgcn_perm(y, x, 0x05040100);
+            odd[2 * u + e] = __builtin_amdgcn_perm(y, x, 0x07060302);
+          }
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const u32x4 x = z ? odd : even;
+          f32x4& c = acc[2 * w + z];
+          if constexpr (__is_same(T, __bf16)) {
+            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, lo), c, 0, 0, 0);
+            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, hi), c, 0, 0, 0);
+          } else {
+            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, hi), c, 0, 0, 0);
+          }
+        }
+      }
+    }
+  }
+
+  // the running softmax over one step's scores (base 2, -inf where masked); s becomes the weights
+  __device__ __forceinline__ void soften(f32x4 (&s)[SUB]) {
+    float t = s[0][0];
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t = fmaxf(t, s[u][e]);
+    t = col_max(t);
+    if (__ballot(t > top + ATT_SLACK)) {                // seldom after the first steps
+      const float next = fmaxf(top, t);
+      const float keep = next == -INFINITY ? 1.f : att_exp2(top - next);
+      sum *= keep;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) o[c] *= keep;
+      top = next;
+    }
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[u][e] = att_exp2(s[u][e] - base);
+        sum += s[u][e];
+      }
+  }
+};
+
+// Steps [t0, t1) of unit `unit` of run r, by the block: its waves take steps in turn and are joined in LDS.  whole: the
+// unit's every step; then the result is written, else this part goes to `slot`.
+template <typename T, int DIM>
+__device__ __forceinline__ void att_part(const PagedAttArgs& a, const AttPlan& p, const Run& r, int unit, int t0, int t1, bool whole,
+                                         float* slot, float* lds) {
+  using Tile = AttTile<T, DIM>;
+  constexpr int SUB = Tile::SUB, STEP = Tile::STEP, KL = Tile::KL, CH = Tile::CH, ROW = Tile::ROW;
+  const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int col = lane & 15, lg = lane >> 4;
+  const int group = a.heads / a.kv_heads, hk = unit / p.tiles, tile = unit - hk * p.tiles;
+  Tile w;
+  int my_row, my_head, begin = 0, end = 0;
+  const bool real = att_column(col, r.n, group, tile, my_row, my_head);
+  if (real && att_row_keys(a, r.row + my_row, begin, end) && a.err_flag) atomicOr(a.err_flag, 1);
+  // keys that every column of the run sees (a column that is none does not count)
+  int all_from = real ? begin : 0, all_to = real ? end : 0x7fffffff;
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) {
+    all_from = max(all_from, __shfl_xor(all_from, d, WAVE));
+    all_to = min(all_to, __shfl_xor(all_to, d, WAVE));
+  }
+  all_from = __builtin_amdgcn_readfirstlane(all_from);
+  all_to = __builtin_amdgcn_readfirstlane(all_to);
+  {
+    const T* q = (const T*)a.q + (long long)(r.row + my_row) * a.q_row + (long long)(hk * group + my_head) * a.q_head;
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      Pack<T, N> x;
+      const int c = (64 * i + 16 * lg) / (int)sizeof(T);
+      w.q[i] = u32x4{0, 0, 0, 0};
+      if (real && p.wide_q) {
+        w.q[i] = *(const u32x4*)(q + c);
+      } else if (real) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x.v[e] = q[c + e];
+        w.q[i] = __builtin_bit_cast(u32x4, x);
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < CH; ++c) w.o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  w.top = -INFINITY;
+  w.sum = 0.f;
+  const float scale = a.scale * 1.4426950408889634f;     // scores in powers of two
+
+  // Where the 16-key parts of this wave's next 64 / SUB steps lie, one part a lane: elements from the cache's beginning
+  // (16 keys never straddle a page), 0 and a bit in `out` for a part that no row sees or whose page is none.
+  const int per_page = a.page_size / 16;
+  const long long head_off = (long long)hk * a.page_size * DIM;
+  long long at = 0;
+  unsigned long long out = 0;
+  auto locate = [&](int first) {
+    const int t = first + (lane / SUB) * ATT_WAVES;
+    const int key = r.begin + t * STEP + 16 * (lane % SUB);
+    at = 0;
+    bool bad = true;
+    if (t < t1 && key < r.end) {
+      const int part = key / 16, page = part / per_page;
+      const int id = a.table[(long long)r.req * a.table_stride + page];
+      bad = id < 0 || id >= a.pages;
+      if (!bad) at = (long long)id * a.page_stride + head_off + (long long)(part - page * per_page) * 16 * DIM;
+      else if (a.err_flag) atomicOr(a.err_flag, 1);
+    }
+    out = __ballot(bad);
+  };
+  auto part_at = [&](int i) -> long long {               // the part that lane i has located, the same for the wave
+    const unsigned lo = __builtin_amdgcn_readlane((unsigned)at, i), hi = __builtin_amdgcn_readlane((unsigned)(at >> 32), i);
+    return (long long)((unsigned long long)hi << 32 | lo);
+  };
+  const T *kc = (const T*)a.k_cache, *vc = (const T*)a.v_cache;
+  constexpr int ROUND = WAVE / SUB;                      // steps that one call of locate() serves
+  int t = t0 + wave, in = 0;
+  if (t < t1) {
+    locate(t);
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) w.load_k(u, kc + part_at(u), lane);
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) w.load_v(u, vc + part_at(u), lane);
+  }
+  while (t < t1) {
+    const int key0 = r.begin + t * STEP;
+    const unsigned bad = (unsigned)(out >> (in * SUB)) & ((1u << SUB) - 1);
+    f32x4 s[SUB];
+    w.scores(s);
+    t += ATT_WAVES;
+    ++in;
+    long long next[SUB];
+    if (t < t1) {
+      if (in == ROUND) {
+        locate(t);
+        in = 0;
+      }
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        next[u] = part_at(in * SUB + u);
+        w.load_k(u, kc + next[u], lane);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) s[u] *= scale;
+    if (bad == 0 && key0 >= all_from && key0 + STEP <= all_to) {
+      w.soften(s);
+      w.template weigh<false>(w.o, s, 0);
+    } else {
+      // this lane's keys, as its own column sees them and, below, as each row of the run does: what a row does not see has
+      // to be left out of V too, or a weight of 0 would meet an infinity or a NaN there
+      auto sees = [&](int from, int to) {
+        unsigned m = 0;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + 16 * u + 4 * lg + e;
+            m |= (unsigned)(key >= from && key < to && !(bad >> u & 1)) << (4 * u + e);
+          }
+        return m;
+      };
+      const unsigned mine = sees(begin, end);
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[u][e] = mine >> (4 * u + e) & 1 ? s[u][e] : -INFINITY;
+      w.soften(s);
+      if (r.n == 1) {
+        w.template weigh<true>(w.o, s, sees(all_from, all_to));
+      } else {
+        for (int i = 0; i < r.n; ++i) {
+          int from, to;
+          att_row_keys(a, r.row + i, from, to);
+          f32x4 add[CH];
+#pragma unroll
+          for (int c = 0; c < CH; ++c) add[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+          w.template weigh<true>(add, s, sees(from, to));
+          const bool own = real && my_row == i;
+#pragma unroll
+          for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w.o[c][e] += own ? add[c][e] : 0.f;
+        }
+      }
+    }
+    if (t < t1) {
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) w.load_v(u, vc + next[u], lane);
+    }
+  }
+  w.sum = col_sum(w.sum);
+
+  // the waves' parts, a column of DIM sums with its maximum and sum behind it each
+  float* mine = lds + (wave * ATT_COLS + col) * ROW;
+  if (real) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine[(4 * lg + e) * CH + c] = w.o[c][e];
+    if (lg == 0) {
+      mine[DIM] = w.top;
+      mine[DIM + 1] = w.sum;
+    }
+  }
+  __syncthreads();
+  for (int m = wave; m < ATT_COLS; m += ATT_WAVES) {      // a wave a column
+    int row, head;
+    if (!att_column(m, r.n, group, tile, row, head)) continue;
+    float top = -INFINITY, sum = 0.f, f[ATT_WAVES];
+#pragma unroll
+    for (int i = 0; i < ATT_WAVES; ++i) top = fmaxf(top, lds[(i * ATT_COLS + m) * ROW + DIM]);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int i = 0; i < ATT_WAVES; ++i) {
+      f[i] = att_exp2(lds[(i * ATT_COLS + m) * ROW + DIM] - base);
+      sum += f[i] * lds[(i * ATT_COLS + m) * ROW + DIM + 1];
+    }
+    int from, to;
+    att_row_keys(a, r.row + row, from, to);
+    const int h = hk * group + head;
+    for (int c = lane; c < DIM; c += WAVE) {
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < ATT_WAVES; ++i) x += f[i] * lds[(i * ATT_COLS + m) * ROW + c];
+      if (whole) ((T*)a.out)[(long long)(r.row + row) * a.out_row + (long long)h * a.out_head + c] = Conv<T>::from(from < to ? x / sum : 0.f);
+      else slot[m * ROW + c] = x;
+    }
+    if (lane == 0) {
+      if (!whole) {
+        slot[m * ROW + DIM] = top;
+        slot[m * ROW + DIM + 1] = sum;
+      } else if (a.lse) {
+        a.lse[(long long)(r.row + row) * a.heads + h] = from < to ? (base + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+      }
+    }
+  }
+  __syncthreads();                                       // before the LDS is written again
+}
+
+// requests outside the table are not followed
+__device__ __forceinline__ void att_flag_request(const PagedAttArgs& a, int row) {
+  if (a.err_flag && a.row_request[row] >= a.requests) atomicOr(a.err_flag, 1);
+}
+
+// A block a unit: for lengths that a block takes in a short time, and for so many units that their lengths even out.
+template <typename T, int DIM>
+__global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attention_kernel(PagedAttArgs a, AttPlan p) {
+  __shared__ float lds[ATT_WAVES * ATT_COLS * AttTile<T, DIM>::ROW];
+  const int unit = blockIdx.x % p.units, row = blockIdx.x / p.units;
+  Run r;
+  if (!att_run(a, p, row, r)) {
+    if (unit == 0 && threadIdx.x == 0) att_flag_request(a, row);
     return;
   }
-  long long end = (long long)a.row_position[row] + 1;
-  const long long cap = (long long)a.width * a.page_size;
-  if (end > cap) {
-    end = cap;
-    if (a.err_flag && threadIdx.x == 0) atomicOr(a.err_flag, 1);
+  att_part<T, DIM>(a, p, r, unit, 0, att_run_steps<AttTile<T, DIM>::STEP>(r), true, nullptr, lds);
+}
+
+// The line of work cut into p.blocks equal pieces, a block a piece: a long row beside short ones, or alone, costs every
+// block the same.  Each block sums up the rows' steps itself to find where its piece begins.
+template <typename T, int DIM>
+__global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attention_split_kernel(PagedAttArgs a, AttPlan p, float* ws, AttJoin* joins) {
+  constexpr int STEP = AttTile<T, DIM>::STEP;
+  __shared__ float lds[ATT_WAVES * ATT_COLS * AttTile<T, DIM>::ROW];
+  __shared__ long long wave_sum[ATT_WAVES];
+  __shared__ long long found_at;
+  __shared__ int found_row;
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+  const int each = (a.rows + ATT_THREADS - 1) / ATT_THREADS;
+  const int row0 = min(tid * each, a.rows), row1 = min(row0 + each, a.rows);
+  long long mine = 0;
+  for (int row = row0; row < row1; ++row) {
+    Run r;
+    if (att_run(a, p, row, r)) mine += att_run_steps<STEP>(r);
+    else if (blockIdx.x == 0) att_flag_request(a, row);
   }
-  const long long begin = a.window > 0 && end > a.window ? end - a.window : 0;
-  const int hk = h / (a.heads / a.kv_heads);
-  const T* q = (const T*)a.q + row * a.q_row + h * a.q_head;
-  float qv[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
+  long long upto = mine;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) qv[i] = lane + 64 * i < a.dim ? Conv<T>::to(q[lane + 64 * i]) * a.scale : 0.f;
-  for (long long t = begin + wave; t < end; t += ATT_WAVES) {
-    const int id = a.table[req * a.table_stride + t / a.page_size];
-    if (id < 0 || id >= a.pages) {
-      if (a.err_flag && lane == 0) atomicOr(a.err_flag, 1);
-      continue;
-    }
-    const long long cell = id * a.page_stride + ((long long)hk * a.page_size + t % a.page_size) * a.dim;
-    float d = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 64 * i < a.dim) d += qv[i] * Conv<T>::to(((const T*)a.k_cache)[cell + lane + 64 * i]);
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) d += __shfl_xor(d, x, 64);
-    const float top = fmaxf(m, d), base = top == -INFINITY ? 0.f : top;
-    const float keep = __expf(m - base), p = __expf(d - base);
-    l = l * keep + p;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 64 * i < a.dim) o[i] = o[i] * keep + p * Conv<T>::to(((const T*)a.v_cache)[cell + lane + 64 * i]);
-    m = top;
+  for (int d = 1; d < WAVE; d <<= 1) {
+    const long long x = __shfl_up(upto, d, WAVE);
+    if (lane >= d) upto += x;
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) part[wave][lane + 64 * i] = o[i];
-  if (lane == 0) { part[wave][PAGED_MAX_DIM] = m; part[wave][PAGED_MAX_DIM + 1] = l; }
+  if (lane == WAVE - 1) wave_sum[wave] = upto;
+  if (tid == 0) found_row = -1;
   __syncthreads();
-  float top = -INFINITY, sum = 0, w[ATT_WAVES];
-  for (int i = 0; i < ATT_WAVES; ++i) top = fmaxf(top, part[i][PAGED_MAX_DIM]);
+  long long before = upto - mine, total = 0;
+  for (int w = 0; w < ATT_WAVES; ++w) {
+    if (w < wave) before += wave_sum[w];
+    total += wave_sum[w];
+  }
+  total *= p.units;
+  long long piece = (total + p.blocks - 1) / p.blocks;
+  if (piece < ATT_MIN_STEPS) piece = ATT_MIN_STEPS;
+  const long long first = blockIdx.x * piece, last = first + piece < total ? first + piece : total;
+  if (tid == 0) joins[blockIdx.x].parts = 0;
+  if (first < last && before * p.units <= first && first < (before + mine) * p.units) {   // one thread
+    long long run_at = before;
+    for (int row = row0; row < row1; ++row) {
+      Run r;
+      if (!att_run(a, p, row, r)) continue;
+      const int steps = att_run_steps<STEP>(r);
+      if (first < (run_at + steps) * p.units) {
+        found_row = row;
+        found_at = run_at;
+        break;
+      }
+      run_at += steps;
+    }
+  }
+  __syncthreads();
+  if (first >= last) return;
+  int row = found_row;
+  long long run_at = found_at * p.units, pos = first;
+  Run r;
+  att_run(a, p, row, r);
+  for (;;) {
+    const int steps = att_run_steps<STEP>(r);
+    for (int unit = (int)((pos - run_at) / steps); unit < p.units && pos < last; ++unit) {
+      const long long unit_at = run_at + (long long)unit * steps;
+      const int t0 = (int)(pos - unit_at), t1 = (int)(last - unit_at < steps ? last - unit_at : steps);
+      const bool whole = t0 == 0 && t1 == steps;
+      if (t0 == 0 && t1 < steps && tid == 0) {
+        const long long end_block = (unit_at + steps - 1) / piece;
+        joins[blockIdx.x] = AttJoin{r.row, r.n, unit, (int)(end_block - blockIdx.x)};
+      }
+      att_part<T, DIM>(a, p, r, unit, t0, t1, whole, att_slot(ws, blockIdx.x, t0 == 0, DIM), lds);
+      pos = unit_at + t1;
+    }
+    if (pos >= last) return;
+    run_at += (long long)steps * p.units;
+    do ++row; while (!att_run(a, p, row, r));             // pos < total: there is one
+  }
+}
+
+// Joins the parts of the unit that begins in block blockIdx.x of the split: a wave a column, one after the other in the
+// order of the keys, so that the result does not depend on which block was done first.
+template <typename T>
+__global__ __launch_bounds__(ATT_THREADS) void paged_join_kernel(PagedAttArgs a, AttPlan p, const float* ws, const AttJoin* joins) {
+  const AttJoin j = joins[blockIdx.x];
+  if (j.parts == 0) return;
+  const int lane = threadIdx.x & (WAVE - 1), m = blockIdx.y * ATT_WAVES + threadIdx.x / WAVE;
+  const int group = a.heads / a.kv_heads, hk = j.unit / p.tiles, ROW = a.dim + 4;
+  int row, head;
+  if (!att_column(m, j.n, group, j.unit - hk * p.tiles, row, head)) return;
+  auto part = [&](int i) { return att_slot(const_cast<float*>(ws), blockIdx.x + i, i == 0, a.dim) + m * ROW; };
+  float top = -INFINITY;
+  for (int i = lane; i <= j.parts; i += WAVE) top = fmaxf(top, part(i)[a.dim]);
+#pragma unroll
+  for (int d = 1; d < WAVE; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, WAVE));
   const float base = top == -INFINITY ? 0.f : top;
-  for (int i = 0; i < ATT_WAVES; ++i) {
-    w[i] = __expf(part[i][PAGED_MAX_DIM] - base);
-    sum += w[i] * part[i][PAGED_MAX_DIM + 1];
+  float x[PAGED_MAX_DIM / WAVE] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll 4
+  for (int i = 0; i <= j.parts; ++i) {
+    const float* q = part(i);
+    const float f = att_exp2(q[a.dim] - base);
+    sum += f * q[a.dim + 1];
+#pragma unroll
+    for (int c = 0; c < PAGED_MAX_DIM / WAVE; ++c)
+      if (lane + WAVE * c < a.dim) x[c] += f * q[lane + WAVE * c];
   }
-  const bool none = end <= 0;
-  for (int c = threadIdx.x; c < a.dim; c += ATT_WAVES * WAVE) {
-    float v = 0;
-    for (int i = 0; i < ATT_WAVES; ++i) v += w[i] * part[i][c];
-    ((T*)a.out)[row * a.out_row + h * a.out_head + c] = Conv<T>::from(none ? 0.f : v / sum);
+  int from, to;
+  att_row_keys(a, j.row + row, from, to);
+  const int h = hk * group + head;
+#pragma unroll
+  for (int c = 0; c < PAGED_MAX_DIM / WAVE; ++c)
+    if (lane + WAVE * c < a.dim)
+      ((T*)a.out)[(long long)(j.row + row) * a.out_row + (long long)h * a.out_head + lane + WAVE * c] = Conv<T>::from(from < to ? x[c] / sum : 0.f);
+  if (a.lse && lane == 0) a.lse[(long long)(j.row + row) * a.heads + h] = from < to ? (base + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+}
+
+constexpr int ATT_BLOCKS = 512;              // two blocks a CU
+
+AttPlan att_plan(int rows, int heads, int kv_heads, long long max_keys, bool& split) {
+  const int group = heads / kv_heads;
+  AttPlan p;
+  p.rows_per_run = group <= ATT_COLS ? ATT_COLS / group : 1;
+  p.tiles = (group + ATT_COLS - 1) / ATT_COLS;
+  p.units = kv_heads * p.tiles;
+  p.blocks = ATT_BLOCKS;
+  p.wide_q = 0;
+  split = max_keys <= 0 || max_keys > 512 || (long long)rows * p.units > 65536;
+  return p;
+}
+
+template <typename T, int DIM>
+hipError_t start_attention(const PagedAttArgs& a, const AttPlan& p, bool split, void* ws, hipStream_t s) {
+  if (!split) {
+    hipLaunchKernelGGL((paged_attention_kernel<T, DIM>), dim3((unsigned)a.rows * p.units), dim3(ATT_THREADS), 0, s, a, p);
+    return hipGetLastError();
   }
-  if (a.lse && threadIdx.x == 0) a.lse[(long long)row * a.heads + h] = none ? -INFINITY : base + logf(sum);
+  float* parts = (float*)ws;
+  AttJoin* joins = (AttJoin*)att_slot(parts, p.blocks, 0, DIM);
+  hipLaunchKernelGGL((paged_attention_split_kernel<T, DIM>), dim3(p.blocks), dim3(ATT_THREADS), 0, s, a, p, parts, joins);
+  const int cols = min(ATT_COLS, a.heads / a.kv_heads * p.rows_per_run);
+  hipLaunchKernelGGL((paged_join_kernel<T>), dim3(p.blocks, (cols + ATT_WAVES - 1) / ATT_WAVES), dim3(ATT_THREADS), 0, s, a, p, parts, joins);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t start_attention_t(const PagedAttArgs& a, const AttPlan& p, bool split, void* ws, hipStream_t s) {
+  switch (a.dim) {
+    case 32: return start_attention<T, 32>(a, p, split, ws, s);
+    case 64: return start_attention<T, 64>(a, p, split, ws, s);
+    case 96: return start_attention<T, 96>(a, p, split, ws, s);
+    case 128: return start_attention<T, 128>(a, p, split, ws, s);
+    case 160: return start_attention<T, 160>(a, p, split, ws, s);
+    case 192: return start_attention<T, 192>(a, p, split, ws, s);
+    case 224: return start_attention<T, 224>(a, p, split, ws, s);
+    case 256: return start_attention<T, 256>(a, p, split, ws, s);
+  }
+  return hipErrorInvalidValue;
 }
 
 }  // namespace
@@ -435,14 +1010,19 @@ hipError_t launch_rotary_store(const RotaryArgs& a, hipStream_t s) {
   return a.dtype == VITS_TYPE_F16 ? start_rotary_t<_Float16>(a, s) : start_rotary_t<__bf16>(a, s);
 }
 
-int64_t paged_attention_workspace(int, int, int, int, long long) { return 0; }
+int64_t paged_attention_workspace(int rows, int heads, int kv_heads, int dim, long long max_keys) {
+  bool split;
+  const AttPlan p = att_plan(rows, heads, kv_heads, max_keys, split);
+  return split ? (int64_t)p.blocks * (2 * ATT_COLS * (dim + 4) * sizeof(float) + sizeof(AttJoin)) : 0;
+}
 
-hipError_t launch_paged_attention(const PagedAttArgs& a, long long, void*, hipStream_t s) {
-  const dim3 grid(a.rows, a.heads), block(ATT_WAVES * WAVE);
-  if (a.dtype == VITS_TYPE_F32) hipLaunchKernelGGL(paged_attention_kernel<float>, grid, block, 0, s, a);
-  else if (a.dtype == VITS_TYPE_F16) hipLaunchKernelGGL(paged_attention_kernel<_Float16>, grid, block, 0, s, a);
-  else hipLaunchKernelGGL(paged_attention_kernel<__bf16>, grid, block, 0, s, a);
-  return hipGetLastError();
+hipError_t launch_paged_attention(const PagedAttArgs& a, long long max_keys, void* ws, hipStream_t s) {
+  bool split;
+  AttPlan p = att_plan(a.rows, a.heads, a.kv_heads, max_keys, split);
+  const int size = a.dtype == VITS_TYPE_F32 ? 4 : 2;
+  p.wide_q = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_row * size % 16 == 0 && a.q_head * size % 16 == 0;
+  if (a.dtype == VITS_TYPE_F32) return start_attention_t<float>(a, p, split, ws, s);
+  return a.dtype == VITS_TYPE_F16 ? start_attention_t<_Float16>(a, p, split, ws, s) : start_attention_t<__bf16>(a, p, split, ws, s);
 }
 
 }  // namespace vits

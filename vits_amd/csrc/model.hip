@@ -352,8 +352,8 @@ int check_page_size(int page_size) {
 }
 
 int check_att_shape(int rows, int heads, int kv_heads, int dim) {
-  if (rows < 0 || kv_heads < 1 || heads < 1 || heads > PAGED_MAX_HEADS || heads % kv_heads || dim < 32 || dim > PAGED_MAX_DIM || dim % 32)
-    return fail(VITS_ERR_INVALID, "paged attention: 1 to 1024 query heads in equal groups over the key-value heads, and heads of "
+  if (rows < 0 || rows > PAGED_MAX_ROWS || kv_heads < 1 || heads < 1 || heads > PAGED_MAX_HEADS || heads % kv_heads || dim < 32 || dim > PAGED_MAX_DIM || dim % 32)
+    return fail(VITS_ERR_INVALID, "paged attention: at most 2^23 rows, 1 to 1024 query heads in equal groups over the key-value heads, and heads of "
                                   "32, 64, ... 256 channels required");
   return VITS_OK;
 }
@@ -1466,9 +1466,9 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
     return fail(VITS_ERR_INVALID, "rotary store: null argument");
   if (dtype < VITS_TYPE_F32 || dtype > VITS_TYPE_BF16)
     return fail(VITS_ERR_INVALID, "rotary store: dtype must be fp32 (0), fp16 (1) or bf16 (2)");
-  if (rows < 0 || dim < 2 || dim > PAGED_MAX_DIM || pairs < 1 || 2 * pairs > dim || (q && (heads < 1 || heads > PAGED_MAX_HEADS)) ||
+  if (rows < 0 || rows > PAGED_MAX_ROWS || dim < 2 || dim > PAGED_MAX_DIM || pairs < 1 || 2 * pairs > dim || (q && (heads < 1 || heads > PAGED_MAX_HEADS)) ||
       (k && (kv_heads < 1 || kv_heads > PAGED_MAX_HEADS || pages < 1)))
-    return fail(VITS_ERR_INVALID, "rotary store: heads of 2 to 256 channels, 1 to 1024 of them, at least one turning pair and no "
+    return fail(VITS_ERR_INVALID, "rotary store: at most 2^23 rows, heads of 2 to 256 channels, 1 to 1024 of them, at least one turning pair and no "
                                   "more pairs than channels hold required");
   if (k) {
     TRY(check_page_size(page_size));
@@ -1504,9 +1504,9 @@ int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const 
     return fail(VITS_ERR_INVALID, "paged attention: dtype must be fp32 (0), fp16 (1) or bf16 (2)");
   TRY(check_att_shape(rows, heads, kv_heads, dim));
   TRY(check_page_size(page_size));
-  if (pages < 1 || width < 1 || table_stride < width || requests < 1 || window < 0)
-    return fail(VITS_ERR_INVALID, "paged attention: at least one page, request and table column, rows of the table that do not "
-                                  "overlap and a window that is not negative required");
+  if (pages < 1 || width < 1 || table_stride < width || (int64_t)width * page_size > (1 << 30) || requests < 1 || window < 0)
+    return fail(VITS_ERR_INVALID, "paged attention: at least one page, request and table column, a table of at most 2^30 tokens a "
+                                  "request whose rows do not overlap and a window that is not negative required");
   if (page_stride < (int64_t)kv_heads * page_size * dim) return fail(VITS_ERR_INVALID, "paged attention: pages overlap");
   if (q && q == out) return fail(VITS_ERR_INVALID, "paged attention: cannot run in place");
   const int size = dtype == VITS_TYPE_F32 ? 4 : 2;

@@ -8,6 +8,7 @@ namespace vits {
 
 constexpr int PAGED_MAX_DIM = 256;          // channels of a head
 constexpr int PAGED_MAX_HEADS = 1024;
+constexpr int PAGED_MAX_ROWS = 1 << 23;
 constexpr int PAGED_PAGE_UNIT = 16;         // page_size is a multiple of it: 16 keys never straddle two pages
 
 struct PagePlanArgs {
