@@ -382,7 +382,8 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr int ATT_WAVES = 4;
 constexpr int ATT_THREADS = ATT_WAVES * WAVE;
 constexpr int ATT_COLS = 16;                 // columns of the products: (row of a run, query head)
-constexpr int ATT_MIN_STEPS = 8;             // the least a block takes of a split length: two steps a wave
+constexpr int ATT_PIECES = 2048;             // the most pieces a call's work is cut into: two waves a SIMD
+constexpr int ATT_MIN_STEPS = 2;             // the least a piece holds
 constexpr float ATT_SLACK = 8.f;             // the running maximum follows once it is exceeded by 2^8: weights stay below 256
 
 // max and sum over the four lanes of a column (lane, lane ^ 16, lane ^ 32, lane ^ 48)
@@ -406,13 +407,14 @@ struct AttPlan {
   int rows_per_run;        // 16 / group, at least 1
   int tiles;               // 16-column tiles of a group
   int units;               // kv_heads * tiles
-  int blocks;              // blocks the line is cut for (split form)
-  int wide_q;              // queries lie on 16-byte addresses
+  int pieces;              // waves that the line is cut for (split form), a multiple of ATT_WAVES
+  int wide_q, wide_out;    // queries, outputs lie on 16-byte addresses
 };
 
 struct Run {
   int row, n, req;
   int begin, end;          // keys that any of its rows sees: begin a multiple of 16
+  int from;                // where its first row's keys begin
 };
 
 template <typename T> constexpr int att_step() { return sizeof(T) == 2 ? 32 : 16; }
@@ -428,16 +430,18 @@ __device__ __forceinline__ bool att_row_keys(const PagedAttArgs& a, int row, int
 
 // whether a run begins at `row`, and what it is
 __device__ __forceinline__ bool att_run(const PagedAttArgs& a, const AttPlan& p, int row, Run& r) {
-  const int req = a.row_request[row];
+  const int req = a.row_request[row], before = a.row_request[row > 0 ? row - 1 : 0];
+  int end;
+  att_row_keys(a, row, r.from, end);                     // loaded beside the requests, not after them
   if (req < 0 || req >= a.requests) return false;
   const int in = row % p.rows_per_run;
-  if (in > 0 && a.row_request[row - 1] == req) return false;
+  if (in > 0 && before == req) return false;
   r.row = row;
   r.req = req;
+  r.begin = r.from < end ? r.from : 0x7fffffff;
+  r.end = end;
   const int most = min(p.rows_per_run - in, a.rows - row);
   int n = 1;
-  att_row_keys(a, row, r.begin, r.end);
-  if (r.begin == r.end) r.begin = 0x7fffffff;
   for (; n < most && a.row_request[row + n] == req; ++n) {
     int b, e;
     att_row_keys(a, row + n, b, e);
@@ -454,8 +458,8 @@ __device__ __forceinline__ int att_run_steps(const Run& r) {
   return max(1, (r.end - r.begin + STEP - 1) / STEP);
 }
 
-// what a block leaves of a unit that it has not taken whole: [0] for the one it begins in the middle of, [1] for the one
-// it ends in the middle of; joined by paged_join_kernel
+// what a block's pieces leave of a unit that they do not hold whole: [0] for the one the block begins in the middle of, [1]
+// for the one it ends in the middle of; joined by paged_join_kernel
 __host__ __device__ __forceinline__ float* att_slot(float* ws, int block, int which, int dim) {
   return ws + ((long long)block * 2 + which) * ATT_COLS * (dim + 4);
 }
@@ -628,20 +632,36 @@ struct AttTile {
   }
 };
 
-// Steps [t0, t1) of unit `unit` of run r, by the block: its waves take steps in turn and are joined in LDS.  whole: the
-// unit's every step; then the result is written, else this part goes to `slot`.
+// x / sum as the result of a column's quad of channels
+template <typename T>
+__device__ __forceinline__ void att_write(const PagedAttArgs& a, int row, int head, int c, f32x4 x, float sum, bool none) {
+  T* to = (T*)a.out + (long long)row * a.out_row + (long long)head * a.out_head + c;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) to[e] = Conv<T>::from(none ? 0.f : x[e] / sum);
+}
+__device__ __forceinline__ void att_write_lse(const PagedAttArgs& a, int row, int head, float top, float sum, bool none) {
+  const float base = top == -INFINITY ? 0.f : top;
+  a.lse[(long long)row * a.heads + head] = none ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
+}
+
+// Steps [t0, t1) of unit `unit` of run r, by one wave.  whole: that is the unit's every step and the result is written, else
+// this part goes to `slot`, in LDS.
 template <typename T, int DIM>
-__device__ __forceinline__ void att_part(const PagedAttArgs& a, const AttPlan& p, const Run& r, int unit, int t0, int t1, bool whole,
-                                         float* slot, float* lds) {
+__device__ __forceinline__ void att_part(const PagedAttArgs& a, const AttPlan& p, const Run& r, int unit, int t0, int t1, bool whole, float* slot) {
   using Tile = AttTile<T, DIM>;
   constexpr int SUB = Tile::SUB, STEP = Tile::STEP, KL = Tile::KL, CH = Tile::CH, ROW = Tile::ROW;
-  const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int lane = threadIdx.x & (WAVE - 1);
   const int col = lane & 15, lg = lane >> 4;
   const int group = a.heads / a.kv_heads, hk = unit / p.tiles, tile = unit - hk * p.tiles;
   Tile w;
   int my_row, my_head, begin = 0, end = 0;
   const bool real = att_column(col, r.n, group, tile, my_row, my_head);
-  if (real && att_row_keys(a, r.row + my_row, begin, end) && a.err_flag) atomicOr(a.err_flag, 1);
+  if (real && r.n == 1) {
+    begin = r.from;
+    end = r.end;
+  } else if (real) {
+    att_row_keys(a, r.row + my_row, begin, end);
+  }
   // keys that every column of the run sees (a column that is none does not count)
   int all_from = real ? begin : 0, all_to = real ? end : 0x7fffffff;
 #pragma unroll
@@ -674,14 +694,14 @@ __device__ __forceinline__ void att_part(const PagedAttArgs& a, const AttPlan& p
   w.sum = 0.f;
   const float scale = a.scale * 1.4426950408889634f;     // scores in powers of two
 
-  // Where the 16-key parts of this wave's next 64 / SUB steps lie, one part a lane: elements from the cache's beginning
+  // Where the 16-key parts of the next 64 / SUB steps lie, one part a lane: elements from the cache's beginning
   // (16 keys never straddle a page), 0 and a bit in `out` for a part that no row sees or whose page is none.
   const int per_page = a.page_size / 16;
   const long long head_off = (long long)hk * a.page_size * DIM;
   long long at = 0;
   unsigned long long out = 0;
   auto locate = [&](int first) {
-    const int t = first + (lane / SUB) * ATT_WAVES;
+    const int t = first + lane / SUB;
     const int key = r.begin + t * STEP + 16 * (lane % SUB);
     at = 0;
     bool bad = true;
@@ -700,7 +720,7 @@ __device__ __forceinline__ void att_part(const PagedAttArgs& a, const AttPlan& p
   };
   const T *kc = (const T*)a.k_cache, *vc = (const T*)a.v_cache;
   constexpr int ROUND = WAVE / SUB;                      // steps that one call of locate() serves
-  int t = t0 + wave, in = 0;
+  int t = t0, in = 0;
   if (t < t1) {
     locate(t);
 #pragma unroll
@@ -713,7 +733,7 @@ __device__ __forceinline__ void att_part(const PagedAttArgs& a, const AttPlan& p
     const unsigned bad = (unsigned)(out >> (in * SUB)) & ((1u << SUB) - 1);
     f32x4 s[SUB];
     w.scores(s);
-    t += ATT_WAVES;
+    ++t;
     ++in;
     long long next[SUB];
     if (t < t1) {
@@ -776,89 +796,84 @@ __device__ __forceinline__ void att_part(const PagedAttArgs& a, const AttPlan& p
     }
   }
   w.sum = col_sum(w.sum);
-
-  // the waves' parts, a column of DIM sums with its maximum and sum behind it each
-  float* mine = lds + (wave * ATT_COLS + col) * ROW;
-  if (real) {
+  if (!real) return;
+  // the lane's DIM / 4 channels lie beside each other: 4 lg * CH and on
+  if (!whole) {
+    float* to = slot + col * ROW;
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int c = 0; c < 4 * CH; c += 4) {
+      f32x4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mine[(4 * lg + e) * CH + c] = w.o[c][e];
+      for (int e = 0; e < 4; ++e) x[e] = w.o[(c + e) % CH][(c + e) / CH];
+      *(f32x4*)(to + 4 * lg * CH + c) = x;
+    }
     if (lg == 0) {
-      mine[DIM] = w.top;
-      mine[DIM + 1] = w.sum;
+      to[DIM] = w.top;
+      to[DIM + 1] = w.sum;
     }
-  }
-  __syncthreads();
-  for (int m = wave; m < ATT_COLS; m += ATT_WAVES) {      // a wave a column
-    int row, head;
-    if (!att_column(m, r.n, group, tile, row, head)) continue;
-    float top = -INFINITY, sum = 0.f, f[ATT_WAVES];
-#pragma unroll
-    for (int i = 0; i < ATT_WAVES; ++i) top = fmaxf(top, lds[(i * ATT_COLS + m) * ROW + DIM]);
-    const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int i = 0; i < ATT_WAVES; ++i) {
-      f[i] = att_exp2(lds[(i * ATT_COLS + m) * ROW + DIM] - base);
-      sum += f[i] * lds[(i * ATT_COLS + m) * ROW + DIM + 1];
-    }
-    int from, to;
-    att_row_keys(a, r.row + row, from, to);
-    const int h = hk * group + head;
-    for (int c = lane; c < DIM; c += WAVE) {
-      float x = 0.f;
-#pragma unroll
-      for (int i = 0; i < ATT_WAVES; ++i) x += f[i] * lds[(i * ATT_COLS + m) * ROW + c];
-      if (whole) ((T*)a.out)[(long long)(r.row + row) * a.out_row + (long long)h * a.out_head + c] = Conv<T>::from(from < to ? x / sum : 0.f);
-      else slot[m * ROW + c] = x;
-    }
-    if (lane == 0) {
-      if (!whole) {
-        slot[m * ROW + DIM] = top;
-        slot[m * ROW + DIM + 1] = sum;
-      } else if (a.lse) {
-        a.lse[(long long)(r.row + row) * a.heads + h] = from < to ? (base + log2f(sum)) * 0.6931471805599453f : -INFINITY;
-      }
-    }
-  }
-  __syncthreads();                                       // before the LDS is written again
-}
-
-// requests outside the table are not followed
-__device__ __forceinline__ void att_flag_request(const PagedAttArgs& a, int row) {
-  if (a.err_flag && a.row_request[row] >= a.requests) atomicOr(a.err_flag, 1);
-}
-
-// A block a unit: for lengths that a block takes in a short time, and for so many units that their lengths even out.
-template <typename T, int DIM>
-__global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attention_kernel(PagedAttArgs a, AttPlan p) {
-  __shared__ float lds[ATT_WAVES * ATT_COLS * AttTile<T, DIM>::ROW];
-  const int unit = blockIdx.x % p.units, row = blockIdx.x / p.units;
-  Run r;
-  if (!att_run(a, p, row, r)) {
-    if (unit == 0 && threadIdx.x == 0) att_flag_request(a, row);
     return;
   }
-  att_part<T, DIM>(a, p, r, unit, 0, att_run_steps<AttTile<T, DIM>::STEP>(r), true, nullptr, lds);
+  const bool none = begin >= end;
+  const int h = hk * group + my_head;
+  T* to = (T*)a.out + (long long)(r.row + my_row) * a.out_row + (long long)h * a.out_head + 4 * lg * CH;
+  constexpr int N = 16 / sizeof(T);
+#pragma unroll
+  for (int c = 0; c < 4 * CH; c += N) {
+    Pack<T, N> x;
+#pragma unroll
+    for (int e = 0; e < N; ++e) x.v[e] = Conv<T>::from(none ? 0.f : w.o[(c + e) % CH][(c + e) / CH] / w.sum);
+    if (p.wide_out) {
+      *(Pack<T, N>*)(to + c) = x;
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) to[c + e] = x.v[e];
+    }
+  }
+  if (a.lse && lg == 0) att_write_lse(a, r.row + my_row, h, w.top, w.sum, none);
 }
 
-// The line of work cut into p.blocks equal pieces, a block a piece: a long row beside short ones, or alone, costs every
-// block the same.  Each block sums up the rows' steps itself to find where its piece begins.
+// requests and positions outside the table are not followed
+__device__ __forceinline__ void att_flag_row(const PagedAttArgs& a, int row) {
+  const int req = a.row_request[row];
+  int b, e;
+  if (a.err_flag && (req >= a.requests || (req >= 0 && att_row_keys(a, row, b, e)))) atomicOr(a.err_flag, 1);
+}
+
+// A wave a unit: for lengths that a wave takes in a short time, and for so many units that their lengths even out.
+template <typename T, int DIM>
+__global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attention_kernel(PagedAttArgs a, AttPlan p) {
+  const long long n = (long long)blockIdx.x * ATT_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int row = (int)(n / p.units), unit = (int)(n - (long long)row * p.units);
+  if (row >= a.rows) return;
+  if (unit == 0 && threadIdx.x % WAVE == 0) att_flag_row(a, row);
+  Run r;
+  if (att_run(a, p, row, r)) att_part<T, DIM>(a, p, r, unit, 0, att_run_steps<AttTile<T, DIM>::STEP>(r), true, nullptr);
+}
+
+// The line of work cut into p.pieces equal pieces, a wave a piece, a block four that follow each other: a long row beside
+// short ones, or alone, costs every wave the same.  Each block sums up the rows' steps itself to find where its waves' pieces
+// begin.  What its waves hold of one unit is joined in the block, and goes to the workspace only where the unit reaches
+// into another block.
 template <typename T, int DIM>
 __global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attention_split_kernel(PagedAttArgs a, AttPlan p, float* ws, AttJoin* joins) {
-  constexpr int STEP = AttTile<T, DIM>::STEP;
-  __shared__ float lds[ATT_WAVES * ATT_COLS * AttTile<T, DIM>::ROW];
+  constexpr int STEP = AttTile<T, DIM>::STEP, ROW = AttTile<T, DIM>::ROW;
+  struct Part {             // what a wave leaves of a unit: [0] one that began in an earlier wave, [1] one that goes on in the next
+    int live, row, n, unit, from, to;
+    int more;               // [0]: it goes on in the next wave; [1]: blocks behind this one that hold some of it
+  };
+  __shared__ float lds[ATT_WAVES][2][ATT_COLS * ROW];
+  __shared__ Part left[ATT_WAVES][2];
   __shared__ long long wave_sum[ATT_WAVES];
-  __shared__ long long found_at;
-  __shared__ int found_row;
-  const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+  __shared__ long long found_at[ATT_WAVES];
+  __shared__ Run found[ATT_WAVES];
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int each = (a.rows + ATT_THREADS - 1) / ATT_THREADS;
   const int row0 = min(tid * each, a.rows), row1 = min(row0 + each, a.rows);
   long long mine = 0;
+  Run r;
   for (int row = row0; row < row1; ++row) {
-    Run r;
     if (att_run(a, p, row, r)) mine += att_run_steps<STEP>(r);
-    else if (blockIdx.x == 0) att_flag_request(a, row);
+    if (blockIdx.x == 0) att_flag_row(a, row);
   }
   long long upto = mine;
 #pragma unroll
@@ -867,7 +882,7 @@ __global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attenti
     if (lane >= d) upto += x;
   }
   if (lane == WAVE - 1) wave_sum[wave] = upto;
-  if (tid == 0) found_row = -1;
+  if (tid < 2 * ATT_WAVES) left[tid >> 1][tid & 1].live = 0;
   __syncthreads();
   long long before = upto - mine, total = 0;
   for (int w = 0; w < ATT_WAVES; ++w) {
@@ -875,86 +890,155 @@ __global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attenti
     total += wave_sum[w];
   }
   total *= p.units;
-  long long piece = (total + p.blocks - 1) / p.blocks;
-  if (piece < ATT_MIN_STEPS) piece = ATT_MIN_STEPS;
-  const long long first = blockIdx.x * piece, last = first + piece < total ? first + piece : total;
+  long long size = (total + p.pieces - 1) / p.pieces;
+  if (size < ATT_MIN_STEPS) size = ATT_MIN_STEPS;
   if (tid == 0) joins[blockIdx.x].parts = 0;
-  if (first < last && before * p.units <= first && first < (before + mine) * p.units) {   // one thread
+  if (blockIdx.x * ATT_WAVES * size >= total) return;      // the whole block
+  for (int w = 0; w < ATT_WAVES; ++w) {                  // the thread whose rows hold the beginning of wave w's piece
+    const long long first = (blockIdx.x * ATT_WAVES + w) * size;
+    if (first >= total || before * p.units > first || first >= (before + mine) * p.units) continue;
     long long run_at = before;
     for (int row = row0; row < row1; ++row) {
-      Run r;
-      if (!att_run(a, p, row, r)) continue;
+      if (each > 1 && !att_run(a, p, row, r)) continue;    // with a row a thread, r is still that row's
       const int steps = att_run_steps<STEP>(r);
       if (first < (run_at + steps) * p.units) {
-        found_row = row;
-        found_at = run_at;
+        found[w] = r;
+        found_at[w] = run_at;
         break;
       }
       run_at += steps;
     }
   }
   __syncthreads();
-  if (first >= last) return;
-  int row = found_row;
-  long long run_at = found_at * p.units, pos = first;
-  Run r;
-  att_run(a, p, row, r);
-  for (;;) {
-    const int steps = att_run_steps<STEP>(r);
-    for (int unit = (int)((pos - run_at) / steps); unit < p.units && pos < last; ++unit) {
-      const long long unit_at = run_at + (long long)unit * steps;
-      const int t0 = (int)(pos - unit_at), t1 = (int)(last - unit_at < steps ? last - unit_at : steps);
-      const bool whole = t0 == 0 && t1 == steps;
-      if (t0 == 0 && t1 < steps && tid == 0) {
-        const long long end_block = (unit_at + steps - 1) / piece;
-        joins[blockIdx.x] = AttJoin{r.row, r.n, unit, (int)(end_block - blockIdx.x)};
+  const int piece = blockIdx.x * ATT_WAVES + wave;
+  const long long first = piece * size, last = first + size < total ? first + size : total;
+  if (first < last) {
+    auto same = [](int x) { return __builtin_amdgcn_readfirstlane(x); };     // the same for the wave: kept in scalar registers
+    const Run f = found[wave];
+    r = Run{same(f.row), same(f.n), same(f.req), same(f.begin), same(f.end), same(f.from)};
+    const long long at = found_at[wave];
+    long long run_at = (long long)((unsigned long long)(unsigned)same((int)(at >> 32)) << 32 | (unsigned)same((int)at)) * p.units;
+    long long pos = first;
+    int row = r.row;
+    for (;;) {
+      const int steps = att_run_steps<STEP>(r);
+      for (int unit = (int)((pos - run_at) / steps); unit < p.units && pos < last; ++unit) {
+        const long long unit_at = run_at + (long long)unit * steps;
+        const int t0 = (int)(pos - unit_at), t1 = (int)(last - unit_at < steps ? last - unit_at : steps);
+        const bool whole = t0 == 0 && t1 == steps;
+        if (!whole && lane == 0)
+          left[wave][t0 == 0] = Part{1, r.row, r.n, unit, r.from, r.end,
+                                     t0 == 0 ? (int)((unit_at + steps - 1) / (size * ATT_WAVES)) - (int)blockIdx.x : t1 < steps};
+        att_part<T, DIM>(a, p, r, unit, t0, t1, whole, lds[wave][t0 == 0]);
+        pos = unit_at + t1;
       }
-      att_part<T, DIM>(a, p, r, unit, t0, t1, whole, att_slot(ws, blockIdx.x, t0 == 0, DIM), lds);
-      pos = unit_at + t1;
+      if (pos >= last) break;
+      run_at += (long long)steps * p.units;
+      do ++row; while (!att_run(a, p, row, r));           // pos < total: there is one
     }
-    if (pos >= last) return;
-    run_at += (long long)steps * p.units;
-    do ++row; while (!att_run(a, p, row, r));             // pos < total: there is one
+  }
+  __syncthreads();
+
+  // A chain: what the block holds of one unit, beginning with a wave's [1], or (k == 0) with what an earlier block began,
+  // and going on in the [0] of the waves behind
+  const int group = a.heads / a.kv_heads;
+  for (int k = 0; k <= ATT_WAVES; ++k) {
+    const Part head = k == 0 ? left[0][0] : left[k - 1][1];
+    if (!head.live) continue;
+    int w1 = k == 0 ? 1 : k;                              // one past the last wave with a [0] of the chain
+    bool ends = k == 0 ? !left[0][0].more : false;
+    while (!ends && w1 < ATT_WAVES) ends = !left[w1++][0].more;
+    const bool whole = ends && k > 0;
+    if (k > 0 && !ends && tid == 0) joins[blockIdx.x] = AttJoin{head.row, head.n, head.unit, head.more};
+    float* slot = att_slot(ws, blockIdx.x, k > 0, DIM);
+    const int hk = head.unit / p.tiles, tile = head.unit - hk * p.tiles;
+    for (int i = tid; i < ATT_COLS * (DIM / 4); i += ATT_THREADS) {
+      const int m = i / (DIM / 4), c = i % (DIM / 4) * 4;
+      int row, hd;
+      if (!att_column(m, head.n, group, tile, row, hd)) continue;
+      const float* part[ATT_WAVES + 1];
+      int n = 0;
+      if (k > 0) part[n++] = lds[k - 1][1] + m * ROW;
+      for (int w = k; w < w1; ++w) part[n++] = lds[w][0] + m * ROW;
+      float top = -INFINITY, sum = 0.f;
+      for (int j = 0; j < n; ++j) top = fmaxf(top, part[j][DIM]);
+      const float base = top == -INFINITY ? 0.f : top;
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < n; ++j) {
+        const float f = att_exp2(part[j][DIM] - base);
+        sum += f * part[j][DIM + 1];
+        x += f * *(const f32x4*)(part[j] + c);
+      }
+      if (!whole) {
+        *(f32x4*)(slot + m * ROW + c) = x;
+        if (c == 0) {
+          slot[m * ROW + DIM] = top;
+          slot[m * ROW + DIM + 1] = sum;
+        }
+        continue;
+      }
+      int from = head.from, to = head.to;
+      if (head.n > 1) att_row_keys(a, head.row + row, from, to);
+      att_write<T>(a, head.row + row, hk * group + hd, c, x, sum, from >= to);
+      if (a.lse && c == 0) att_write_lse(a, head.row + row, hk * group + hd, top, sum, from >= to);
+    }
   }
 }
 
-// Joins the parts of the unit that begins in block blockIdx.x of the split: a wave a column, one after the other in the
-// order of the keys, so that the result does not depend on which block was done first.
+// Joins the parts of the unit that begins in block blockIdx.x and ends in a later one, a block a column (every gridDim.y-th):
+// first the parts' weights, then the weighted sum, dim / 4 threads a part and as many parts at once as that leaves threads
+// for, each its parts in the order of the keys: the result does not depend on which block was done first.
 template <typename T>
-__global__ __launch_bounds__(ATT_THREADS) void paged_join_kernel(PagedAttArgs a, AttPlan p, const float* ws, const AttJoin* joins) {
+__global__ __launch_bounds__(ATT_THREADS) void paged_join_kernel(PagedAttArgs a, AttPlan p, float* ws, const AttJoin* joins) {
+  __shared__ float weight[ATT_PIECES / ATT_WAVES];
+  __shared__ float wave_top[ATT_WAVES], wave_sum[ATT_WAVES];
+  __shared__ f32x4 acc[ATT_THREADS];
   const AttJoin j = joins[blockIdx.x];
   if (j.parts == 0) return;
-  const int lane = threadIdx.x & (WAVE - 1), m = blockIdx.y * ATT_WAVES + threadIdx.x / WAVE;
-  const int group = a.heads / a.kv_heads, hk = j.unit / p.tiles, ROW = a.dim + 4;
-  int row, head;
-  if (!att_column(m, j.n, group, j.unit - hk * p.tiles, row, head)) return;
-  auto part = [&](int i) { return att_slot(const_cast<float*>(ws), blockIdx.x + i, i == 0, a.dim) + m * ROW; };
-  float top = -INFINITY;
-  for (int i = lane; i <= j.parts; i += WAVE) top = fmaxf(top, part(i)[a.dim]);
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+  const int group = a.heads / a.kv_heads, ROW = a.dim + 4, parts = j.parts + 1;
+  const int quads = a.dim / 4, at_once = ATT_THREADS / quads, mine = tid / quads, quad = tid - mine * quads;
+  const int hk = j.unit / p.tiles;
+  for (int m = blockIdx.y; m < ATT_COLS; m += gridDim.y) {
+    int row, head;
+    if (!att_column(m, j.n, group, j.unit - hk * p.tiles, row, head)) break;   // columns that are none come last
+    auto part = [&](int i) { return att_slot(ws, blockIdx.x + i, i == 0, a.dim) + m * ROW; };
+    float top = -INFINITY, sum = 0.f;
+    for (int i = tid; i < parts; i += ATT_THREADS) top = fmaxf(top, weight[i] = part(i)[a.dim]);
 #pragma unroll
-  for (int d = 1; d < WAVE; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, WAVE));
-  const float base = top == -INFINITY ? 0.f : top;
-  float x[PAGED_MAX_DIM / WAVE] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-#pragma unroll 4
-  for (int i = 0; i <= j.parts; ++i) {
-    const float* q = part(i);
-    const float f = att_exp2(q[a.dim] - base);
-    sum += f * q[a.dim + 1];
+    for (int d = 1; d < WAVE; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, WAVE));
+    if (lane == 0) wave_top[wave] = top;
+    __syncthreads();
+    for (int i = 0; i < ATT_WAVES; ++i) top = fmaxf(top, wave_top[i]);
+    const float base = top == -INFINITY ? 0.f : top;
+    for (int i = tid; i < parts; i += ATT_THREADS) {     // the thread's own entries
+      const float f = att_exp2(weight[i] - base);
+      sum += f * part(i)[a.dim + 1];
+      weight[i] = f;
+    }
 #pragma unroll
-    for (int c = 0; c < PAGED_MAX_DIM / WAVE; ++c)
-      if (lane + WAVE * c < a.dim) x[c] += f * q[lane + WAVE * c];
+    for (int d = 1; d < WAVE; d <<= 1) sum += __shfl_xor(sum, d, WAVE);
+    if (lane == 0) wave_sum[wave] = sum;
+    __syncthreads();
+    sum = 0.f;
+    for (int i = 0; i < ATT_WAVES; ++i) sum += wave_sum[i];
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (mine < at_once) {
+#pragma unroll 8
+      for (int i = mine; i < parts; i += at_once) x += weight[i] * *(const f32x4*)(part(i) + 4 * quad);
+    }
+    acc[tid] = x;
+    int from, to;
+    att_row_keys(a, j.row + row, from, to);
+    __syncthreads();
+    if (mine == 0) {
+      for (int i = 1; i < at_once; ++i) x += acc[i * quads + quad];
+      att_write<T>(a, j.row + row, hk * group + head, 4 * quad, x, sum, from >= to);
+    }
+    if (a.lse && tid == 0) att_write_lse(a, j.row + row, hk * group + head, top, sum, from >= to);
+    __syncthreads();                                     // before the LDS is written again
   }
-  int from, to;
-  att_row_keys(a, j.row + row, from, to);
-  const int h = hk * group + head;
-#pragma unroll
-  for (int c = 0; c < PAGED_MAX_DIM / WAVE; ++c)
-    if (lane + WAVE * c < a.dim)
-      ((T*)a.out)[(long long)(j.row + row) * a.out_row + (long long)h * a.out_head + lane + WAVE * c] = Conv<T>::from(from < to ? x[c] / sum : 0.f);
-  if (a.lse && lane == 0) a.lse[(long long)(j.row + row) * a.heads + h] = from < to ? (base + log2f(sum)) * 0.6931471805599453f : -INFINITY;
 }
-
-constexpr int ATT_BLOCKS = 512;              // two blocks a CU
 
 AttPlan att_plan(int rows, int heads, int kv_heads, long long max_keys, bool& split) {
   const int group = heads / kv_heads;
@@ -962,23 +1046,29 @@ AttPlan att_plan(int rows, int heads, int kv_heads, long long max_keys, bool& sp
   p.rows_per_run = group <= ATT_COLS ? ATT_COLS / group : 1;
   p.tiles = (group + ATT_COLS - 1) / ATT_COLS;
   p.units = kv_heads * p.tiles;
-  p.blocks = ATT_BLOCKS;
-  p.wide_q = 0;
-  split = max_keys <= 0 || max_keys > 512 || (long long)rows * p.units > 65536;
+  p.pieces = ATT_PIECES;
+  p.wide_q = p.wide_out = 0;
+  const long long units = (long long)rows * p.units;
+  if (max_keys > 0 && max_keys < (1 << 30)) {            // no more pieces than their least size fills, in steps of 16 keys
+    const long long most = units * ((max_keys + 15) / 16 + 1) / ATT_MIN_STEPS + 1;
+    if (most < p.pieces) p.pieces = (int)(most + ATT_WAVES - 1) / ATT_WAVES * ATT_WAVES;
+  }
+  split = max_keys <= 0 || max_keys > 64 || units > 1 << 22;
   return p;
 }
 
 template <typename T, int DIM>
 hipError_t start_attention(const PagedAttArgs& a, const AttPlan& p, bool split, void* ws, hipStream_t s) {
   if (!split) {
-    hipLaunchKernelGGL((paged_attention_kernel<T, DIM>), dim3((unsigned)a.rows * p.units), dim3(ATT_THREADS), 0, s, a, p);
+    const long long units = (long long)a.rows * p.units;
+    hipLaunchKernelGGL((paged_attention_kernel<T, DIM>), dim3((unsigned)((units + ATT_WAVES - 1) / ATT_WAVES)), dim3(ATT_THREADS), 0, s, a, p);
     return hipGetLastError();
   }
-  float* parts = (float*)ws;
-  AttJoin* joins = (AttJoin*)att_slot(parts, p.blocks, 0, DIM);
-  hipLaunchKernelGGL((paged_attention_split_kernel<T, DIM>), dim3(p.blocks), dim3(ATT_THREADS), 0, s, a, p, parts, joins);
-  const int cols = min(ATT_COLS, a.heads / a.kv_heads * p.rows_per_run);
-  hipLaunchKernelGGL((paged_join_kernel<T>), dim3(p.blocks, (cols + ATT_WAVES - 1) / ATT_WAVES), dim3(ATT_THREADS), 0, s, a, p, parts, joins);
+  const int blocks = p.pieces / ATT_WAVES;
+  AttJoin* joins = (AttJoin*)att_slot((float*)ws, blocks, 0, DIM);
+  hipLaunchKernelGGL((paged_attention_split_kernel<T, DIM>), dim3(blocks), dim3(ATT_THREADS), 0, s, a, p, (float*)ws, joins);
+  const int cols = min(4, a.heads / a.kv_heads * p.rows_per_run);
+  hipLaunchKernelGGL((paged_join_kernel<T>), dim3(blocks, cols), dim3(ATT_THREADS), 0, s, a, p, (float*)ws, joins);
   return hipGetLastError();
 }
 
@@ -1013,7 +1103,7 @@ hipError_t launch_rotary_store(const RotaryArgs& a, hipStream_t s) {
 int64_t paged_attention_workspace(int rows, int heads, int kv_heads, int dim, long long max_keys) {
   bool split;
   const AttPlan p = att_plan(rows, heads, kv_heads, max_keys, split);
-  return split ? (int64_t)p.blocks * (2 * ATT_COLS * (dim + 4) * sizeof(float) + sizeof(AttJoin)) : 0;
+  return split ? (int64_t)(p.pieces / ATT_WAVES) * (2 * ATT_COLS * (dim + 4) * sizeof(float) + sizeof(AttJoin)) : 0;
 }
 
 hipError_t launch_paged_attention(const PagedAttArgs& a, long long max_keys, void* ws, hipStream_t s) {
@@ -1021,6 +1111,7 @@ hipError_t launch_paged_attention(const PagedAttArgs& a, long long max_keys, voi
   AttPlan p = att_plan(a.rows, a.heads, a.kv_heads, max_keys, split);
   const int size = a.dtype == VITS_TYPE_F32 ? 4 : 2;
   p.wide_q = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_row * size % 16 == 0 && a.q_head * size % 16 == 0;
+  p.wide_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_row * size % 16 == 0 && a.out_head * size % 16 == 0;
   if (a.dtype == VITS_TYPE_F32) return start_attention_t<float>(a, p, split, ws, s);
   return a.dtype == VITS_TYPE_F16 ? start_attention_t<_Float16>(a, p, split, ws, s) : start_attention_t<__bf16>(a, p, split, ws, s);
 }
