@@ -63,7 +63,7 @@ ATTEND = dict(q=P, q_row=512, q_head=128, k_cache=P, v_cache=P, page_stride=2 * 
     (dict(dim=288), "required"), (dict(page_size=8), "page_size"), (dict(pages=0), "required"), (dict(width=0), "required"),
     (dict(table_stride=7), "required"), (dict(requests=0), "required"), (dict(window=-1), "required"), (dict(page_stride=100), "overlap"),
     (dict(k_cache=P + 8), "16-byte"), (dict(v_cache=P + 2), "16-byte"), (dict(page_stride=2 * 16 * 128 + 4), "16-byte"),
-    (dict(out=P), "in place"),
+    (dict(out=P), "in place"), (dict(q=P + 8), "16-byte"), (dict(q_row=516), "16-byte"), (dict(q_head=132), "16-byte"),
 ])
 def test_paged_attention_refuses(change, word):
     refused(N.lib.vits_op_paged_attention(*{**ATTEND, **change}.values()), word)

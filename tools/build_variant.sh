@@ -7,6 +7,7 @@ NAME="$1"; SRC="$2"; EXTRA="$3"
 R="$(cd "$(dirname "$0")/.." && pwd)"
 L="$R/vits_amd/lib"; V="$L/variants"; mkdir -p "$V"
 BASE="$(basename "$SRC" .hip)"
+if [ "$BASE" == kernels_paged ]; then EXTRA="-mllvm -amdgpu-mfma-vgpr-form $EXTRA"; fi
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-gpu-rdc -Wall -Wno-unused-function \
   -Xclang -target-feature -Xclang -packed-fp32-ops $EXTRA \
   -c "$R/vits_amd/csrc/$BASE.hip" -o "$V/${BASE}_$NAME.o"

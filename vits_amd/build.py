@@ -18,6 +18,10 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "-Wall", "-Wno-unused-function",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
+# The paged attention keeps its accumulators in the registers that the vector unit reads too.  Left to choose, the compiler gives
+# builds with much LDS the other kind, moves values there, and has been seen to move only those of the lanes that were on.
+SOURCE_FLAGS = {"kernels_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+
 
 def _stale(target: str, deps) -> bool:
     if not os.path.exists(target):
@@ -37,7 +41,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
         o = os.path.join(LIBDIR, src.replace(".hip", ".o"))
         objs.append(o)
         if force or _stale(o, [s] + deps.get(src, headers[:1])):
-            jobs.append([HIPCC, *FLAGS, "-c", s, "-o", o])
+            jobs.append([HIPCC, *FLAGS, *SOURCE_FLAGS.get(src, []), "-c", s, "-o", o])
 
     def run(cmd):
         if verbose:

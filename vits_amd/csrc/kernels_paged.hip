@@ -377,7 +377,10 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int ATT_WAVES = 4;
 constexpr int ATT_THREADS = ATT_WAVES * WAVE;
@@ -408,7 +411,7 @@ struct AttPlan {
   int tiles;               // 16-column tiles of a group
   int units;               // kv_heads * tiles
   int pieces;              // waves that the line is cut for (split form), a multiple of ATT_WAVES
-  int wide_q, wide_out;    // queries, outputs lie on 16-byte addresses
+  int wide_out;            // outputs lie on 16-byte addresses
 };
 
 struct Run {
@@ -416,8 +419,6 @@ struct Run {
   int begin, end;          // keys that any of its rows sees: begin a multiple of 16
   int from;                // where its first row's keys begin
 };
-
-template <typename T> constexpr int att_step() { return sizeof(T) == 2 ? 32 : 16; }
 
 // a row's keys [begin, end); true if its position lies outside the table
 __device__ __forceinline__ bool att_row_keys(const PagedAttArgs& a, int row, int& begin, int& end) {
@@ -481,127 +482,154 @@ __device__ __forceinline__ bool att_column(int m, int n, int group, int tile, in
 
 __device__ __forceinline__ float att_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// A result of a matrix instruction is bound to a wait here, in the block that computes it: read in another block, behind a
+// taken branch, the compiler (ROCm 7.2) has been seen to leave it too short (needed: up to 11 issue slots).
+#define ATT_SETTLE(x) asm volatile("s_nop 15" : "+v"(x))
+
 template <typename T, int DIM>
 struct AttTile {
   static constexpr bool HALF = sizeof(T) == 2;
-  static constexpr int SUB = HALF ? 2 : 1;              // 16-key parts of a step
+  // Registers: Q, K, V and O of a step have to fit 256 (two waves a SIMD) with room for the rest.  So wide heads take 16
+  // keys a step, and fp32 ones load K and V in two passes, the second when the first has been used.
+  static constexpr int SUB = HALF && DIM <= 192 ? 2 : 1;  // 16-key parts of a step
+  static constexpr int PASSES = !HALF && DIM > 160 ? 2 : 1;
   static constexpr int STEP = 16 * SUB;
   static constexpr int KL = DIM * (int)sizeof(T) / 64;   // 16-byte loads of a lane for 16 keys
+  static constexpr int KP = KL / PASSES;
   static constexpr int CH = DIM / 16;                   // channels of a lane in V and in the output
   static constexpr int VW = CH * (int)sizeof(T) / 4;     // dwords of a lane for one row of V
+  static constexpr int VP = VW / PASSES;
   static constexpr int ROW = DIM + 4;                   // floats of a column in LDS and in the workspace, padded
+  static_assert(KL % PASSES == 0 && VW % PASSES == 0);
 
-  u32x4 q[KL], k[SUB][KL];
-  unsigned v[SUB][4][VW];
+  u32x4 q[KL], k[SUB][KP];
+  unsigned v[SUB][4][VP];
   f32x4 o[CH];
   float top, sum;                                       // of this lane's column: running maximum (base 2), and this lane's part of the sum
 
-  __device__ __forceinline__ void load_k(int s, const T* page, int lane) {
-    const char* p = (const char*)page + (lane & 15) * (DIM * sizeof(T)) + (lane >> 4) * 16;
+  __device__ __forceinline__ void load_k(int s, const T* page, int lane, int pass) {
+    const char* p = (const char*)page + (lane & 15) * (DIM * sizeof(T)) + (lane >> 4) * 16 + pass * (KP * 64);
 #pragma unroll
-    for (int i = 0; i < KL; ++i) k[s][i] = *(const u32x4*)(p + 64 * i);
+    for (int i = 0; i < KP; ++i) k[s][i] = *(const u32x4*)(p + 64 * i);
   }
-  __device__ __forceinline__ void load_v(int s, const T* page, int lane) {
-    const char* p = (const char*)page + (lane >> 4) * (4 * DIM * sizeof(T)) + (lane & 15) * (VW * 4);
+  __device__ __forceinline__ void load_v(int s, const T* page, int lane, int pass) {
+    const char* p = (const char*)page + (lane >> 4) * (4 * DIM * sizeof(T)) + (lane & 15) * (VW * 4) + pass * (VP * 4);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const char* r = p + j * (DIM * sizeof(T));
       int w = 0;
 #pragma unroll
-      for (; w + 4 <= VW; w += 4) {
+      for (; w + 4 <= VP; w += 4) {
         const u32x4a x = *(const u32x4a*)(r + 4 * w);
         v[s][j][w] = x[0]; v[s][j][w + 1] = x[1]; v[s][j][w + 2] = x[2]; v[s][j][w + 3] = x[3];
       }
-      if constexpr (VW % 4 == 3) {
+      if constexpr (VP % 4 == 3) {
         const u32x3a x = *(const u32x3a*)(r + 4 * w);
         v[s][j][w] = x[0]; v[s][j][w + 1] = x[1]; v[s][j][w + 2] = x[2];
-      } else if constexpr (VW % 4 == 2) {
+      } else if constexpr (VP % 4 == 2) {
         const u32x2a x = *(const u32x2a*)(r + 4 * w);
         v[s][j][w] = x[0]; v[s][j][w + 1] = x[1];
-      } else if constexpr (VW % 4 == 1) {
+      } else if constexpr (VP % 4 == 1) {
         v[s][j][w] = *(const unsigned*)(r + 4 * w);
       }
     }
   }
 
-  __device__ __forceinline__ void scores(f32x4 (&s)[SUB]) const {
+  // s += K^T Q over the channels of a pass
+  __device__ __forceinline__ void scores(f32x4 (&s)[SUB], int pass) const {
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
-      f32x4 c = {0.f, 0.f, 0.f, 0.f};
+      f32x4 c = s[u];
 #pragma unroll
-      for (int i = 0; i < KL; ++i) {
+      for (int i = 0; i < KP; ++i) {
+        const u32x4 y = q[pass * KP + i];
         if constexpr (!HALF) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[u][i][e]), __uint_as_float(q[i][e]), c, 0, 0, 0);
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[u][i][e]), __uint_as_float(y[e]), c, 0, 0, 0);
         } else if constexpr (__is_same(T, __bf16)) {
-          c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[u][i]), __builtin_bit_cast(bf16x8, q[i]), c, 0, 0, 0);
+          c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[u][i]), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
         } else {
-          c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[u][i]), __builtin_bit_cast(f16x8, q[i]), c, 0, 0, 0);
+          c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[u][i]), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
         }
       }
       s[u] = c;
     }
-    // The scores are read in another block of the program than this one, which the compiler (ROCm 7.2) reaches over a taken branch
-    // without the wait that a matrix instruction's result needs (up to 11 issue slots): the fp32 form at 64 channels read
-    // scores of the step before.  So they are waited for here.
 #pragma unroll
-    for (int u = 0; u < SUB; ++u) asm volatile("s_nop 15" : "+v"(s[u]));
+    for (int u = 0; u < SUB; ++u) ATT_SETTLE(s[u]);
   }
 
-  // acc += V^T P^T, with the rows of V that `see` (one bit a key of this lane: 4 * part + row) leaves out taken as zero
-  template <bool MASKED>
-  __device__ __forceinline__ void weigh(f32x4 (&acc)[CH], const f32x4 (&p)[SUB], unsigned see) const {
-    if constexpr (!HALF) {
+  // the weights of a step as operands
+  struct Weights {
+    f32x4 f;                                            // fp32
+    unsigned hi[2 * SUB], lo[2 * SUB];                  // 16 bits: two keys each; lo is what bf16 leaves of a weight
+  };
+  static __device__ __forceinline__ Weights weights(const f32x4 (&p)[SUB]) {
+    Weights w;
+    w.f = p[0];
+    if constexpr (HALF) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          const unsigned x = MASKED && !(see >> j & 1) ? 0u : v[0][j][c];
-          acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x), p[0][j], acc[c], 0, 0, 0);
-        }
-    } else {
-      u32x4 hi, lo;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const f32x2 w = {p[u][2 * e], p[u][2 * e + 1]};
-          if constexpr (__is_same(T, __bf16)) {
-            const bf16x2 h = __builtin_convertvector(w, bf16x2);
-            hi[2 * u + e] = __builtin_bit_cast(unsigned, h);
-            lo[2 * u + e] = __builtin_bit_cast(unsigned, __builtin_convertvector(w - __builtin_convertvector(h, f32x2), bf16x2));
-          } else {
-            hi[2 * u + e] = __builtin_bit_cast(unsigned, __builtin_convertvector(w, f16x2));
-          }
-        }
-#pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        u32x4 even, odd;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            unsigned x = v[u][2 * e][w], y = v[u][2 * e + 1][w];
-            if (MASKED) {
-              x = see >> (4 * u + 2 * e) & 1 ? x : 0u;
-              y = see >> (4 * u + 2 * e + 1) & 1 ? y : 0u;
-            }
-            even[2 * u + e] = __builtin_amdgcn_perm(y, x, 0x05040100);
-            odd[2 * u + e] = __builtin_amdgcn_perm(y, x, 0x07060302);
-          }
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const u32x4 x = z ? odd : even;
-          f32x4& c = acc[2 * w + z];
-          if constexpr (__is_same(T, __bf16)) {
-            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, lo), c, 0, 0, 0);
-            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, hi), c, 0, 0, 0);
-          } else {
-            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, hi), c, 0, 0, 0);
-          }
+      for (int i = 0; i < 2 * SUB; ++i) {
+        const f32x2 x = {p[i / 2][i % 2 * 2], p[i / 2][i % 2 * 2 + 1]};
+        if constexpr (__is_same(T, __bf16)) {
+          const bf16x2 h = __builtin_convertvector(x, bf16x2);
+          w.hi[i] = __builtin_bit_cast(unsigned, h);
+          w.lo[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(x - __builtin_convertvector(h, f32x2), bf16x2));
+        } else {
+          w.hi[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(x, f16x2));
         }
       }
+    }
+    return w;
+  }
+  static __device__ __forceinline__ f32x4 product(const unsigned (&x)[2 * SUB], const unsigned (&y)[2 * SUB], f32x4 c) {
+    if constexpr (SUB == 2) {
+      const u32x4 a = {x[0], x[1], x[2], x[3]}, b = {y[0], y[1], y[2], y[3]};
+      if constexpr (__is_same(T, __bf16))
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+      else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    } else {
+      const u32x2 a = {x[0], x[1]}, b = {y[0], y[1]};
+      if constexpr (__is_same(T, __bf16))
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+      else
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+    }
+  }
+
+  // leaves the keys out of V that `see` has no bit for (one a key of this lane: 4 * part + row)
+  __device__ __forceinline__ void mask_v(unsigned see) {
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool seen = see >> (4 * u + j) & 1;
+#pragma unroll
+        for (int w = 0; w < VP; ++w) v[u][j][w] = seen ? v[u][j][w] : 0u;
+      }
+  }
+
+  // c[0 .. PER) += V^T P^T for the channels of dword w of a pass: one channel in fp32, two in 16 bits
+  static constexpr int PER = HALF ? 2 : 1;
+  __device__ __forceinline__ void weigh(f32x4* c, int w, const Weights& p) const {
+    if constexpr (!HALF) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[0][j][w]), p.f[j], c[0], 0, 0, 0);
+    } else {
+      unsigned even[2 * SUB], odd[2 * SUB];
+#pragma unroll
+      for (int i = 0; i < 2 * SUB; ++i) {
+        const unsigned x = v[i / 2][i % 2 * 2][w], y = v[i / 2][i % 2 * 2 + 1][w];
+        even[i] = __builtin_amdgcn_perm(y, x, 0x05040100);
+        odd[i] = __builtin_amdgcn_perm(y, x, 0x07060302);
+      }
+      if constexpr (__is_same(T, __bf16)) {
+        c[0] = product(even, p.lo, c[0]);
+        c[1] = product(odd, p.lo, c[1]);
+      }
+      c[0] = product(even, p.hi, c[0]);
+      c[1] = product(odd, p.hi, c[1]);
     }
   }
 
@@ -613,9 +641,10 @@ struct AttTile {
 #pragma unroll
       for (int e = 0; e < 4; ++e) t = fmaxf(t, s[u][e]);
     t = col_max(t);
-    if (__ballot(t > top + ATT_SLACK)) {                // seldom after the first steps
-      const float next = fmaxf(top, t);
-      const float keep = next == -INFINITY ? 1.f : att_exp2(top - next);
+    const bool above = t > top + ATT_SLACK;
+    if (__ballot(above)) {                              // seldom after the first steps
+      const float next = above ? t : top;               // a column goes by its own scores alone
+      const float keep = above ? att_exp2(top - next) : 1.f;
       sum *= keep;
 #pragma unroll
       for (int c = 0; c < CH; ++c) o[c] *= keep;
@@ -634,85 +663,96 @@ struct AttTile {
 
 // x / sum as the result of a column's quad of channels
 template <typename T>
-__device__ __forceinline__ void att_write(const PagedAttArgs& a, int row, int head, int c, f32x4 x, float sum, bool none) {
+__device__ __forceinline__ void att_write(const PagedAttArgs& a, bool wide, int row, int head, int c, f32x4 x, float sum, bool none) {
   T* to = (T*)a.out + (long long)row * a.out_row + (long long)head * a.out_head + c;
+  Pack<T, 4> y;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) to[e] = Conv<T>::from(none ? 0.f : x[e] / sum);
+  for (int e = 0; e < 4; ++e) y.v[e] = Conv<T>::from(none ? 0.f : x[e] / sum);
+  if (!wide) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[e] = y.v[e];
+  } else if constexpr (sizeof(T) == 4) {
+    *(u32x4*)to = __builtin_bit_cast(u32x4, y);
+  } else {
+    *(u32x2*)to = __builtin_bit_cast(u32x2, y);
+  }
 }
 __device__ __forceinline__ void att_write_lse(const PagedAttArgs& a, int row, int head, float top, float sum, bool none) {
   const float base = top == -INFINITY ? 0.f : top;
   a.lse[(long long)row * a.heads + head] = none ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
 }
 
-// Steps [t0, t1) of unit `unit` of run r, by one wave.  whole: that is the unit's every step and the result is written, else
-// this part goes to `slot`, in LDS.
+// A wave's result for its column, or its part of it.  The lane's DIM / 4 channels lie beside each other: 4 lg * CH and on.
 template <typename T, int DIM>
-__device__ __forceinline__ void att_part(const PagedAttArgs& a, const AttPlan& p, const Run& r, int unit, int t0, int t1, bool whole, float* slot) {
+__device__ __forceinline__ void att_leave(const PagedAttArgs& a, const AttPlan& p, const AttTile<T, DIM>& w, int col, int lg, int row, int head,
+                                          bool none, bool whole, float* slot) {
+  constexpr int CH = AttTile<T, DIM>::CH;
+  float* to = slot + col * AttTile<T, DIM>::ROW;
+#pragma unroll
+  for (int c = 0; c < 4 * CH; c += 4) {
+    f32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = w.o[(c + e) % CH][(c + e) / CH];
+    if (whole) att_write<T>(a, p.wide_out, row, head, 4 * lg * CH + c, x, w.sum, none);
+    else *(f32x4*)(to + 4 * lg * CH + c) = x;
+  }
+  if (lg != 0) return;
+  if (!whole) {
+    to[DIM] = w.top;
+    to[DIM + 1] = w.sum;
+  } else if (a.lse) {
+    att_write_lse(a, row, head, w.top, w.sum, none);
+  }
+}
+
+// Steps [t0, t1) of unit `unit` of run r, by one wave.  whole: that is the unit's every step and the result is written, else
+// this part goes to `slot`, in LDS.  Returns whether a page was not one of the cache's.
+//
+// A key that one row of the run sees and another does not has a weight of 0 in the other's column, and 0 times an infinity or
+// a NaN in V would reach it.  So where rows differ and a result is not finite, the part is taken again row by row, with what
+// the row does not see left out of V.
+//
+// No lane is ever switched off in here before the last write: what a lane must not load it loads from where another may, and
+// drops.  With lanes off, the compiler (ROCm 7.2) has been seen to move whole-wave values between registers of the two kinds
+// for the lanes that were on alone, for which reason no build may need more than 256 registers either.
+template <typename T, int DIM>
+__device__ __forceinline__ bool att_part(const PagedAttArgs& a, const AttPlan& p, const Run& r, int unit, int t0, int t1, bool whole, float* slot) {
   using Tile = AttTile<T, DIM>;
-  constexpr int SUB = Tile::SUB, STEP = Tile::STEP, KL = Tile::KL, CH = Tile::CH, ROW = Tile::ROW;
+  constexpr int SUB = Tile::SUB, STEP = Tile::STEP, KL = Tile::KL, CH = Tile::CH, PASSES = Tile::PASSES;
   const int lane = threadIdx.x & (WAVE - 1);
   const int col = lane & 15, lg = lane >> 4;
   const int group = a.heads / a.kv_heads, hk = unit / p.tiles, tile = unit - hk * p.tiles;
   Tile w;
-  int my_row, my_head, begin = 0, end = 0;
+  int my_row, my_head;
   const bool real = att_column(col, r.n, group, tile, my_row, my_head);
-  if (real && r.n == 1) {
-    begin = r.from;
-    end = r.end;
-  } else if (real) {
-    att_row_keys(a, r.row + my_row, begin, end);
-  }
-  // keys that every column of the run sees (a column that is none does not count)
-  int all_from = real ? begin : 0, all_to = real ? end : 0x7fffffff;
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) {
-    all_from = max(all_from, __shfl_xor(all_from, d, WAVE));
-    all_to = min(all_to, __shfl_xor(all_to, d, WAVE));
-  }
-  all_from = __builtin_amdgcn_readfirstlane(all_from);
-  all_to = __builtin_amdgcn_readfirstlane(all_to);
+  my_row = real ? my_row : 0;
+  my_head = real ? my_head : 0;
+  int begin = r.from, end = r.end;
+  if (r.n > 1) att_row_keys(a, r.row + my_row, begin, end);
   {
     const T* q = (const T*)a.q + (long long)(r.row + my_row) * a.q_row + (long long)(hk * group + my_head) * a.q_head;
-    constexpr int N = 16 / sizeof(T);
 #pragma unroll
-    for (int i = 0; i < KL; ++i) {
-      Pack<T, N> x;
-      const int c = (64 * i + 16 * lg) / (int)sizeof(T);
-      w.q[i] = u32x4{0, 0, 0, 0};
-      if (real && p.wide_q) {
-        w.q[i] = *(const u32x4*)(q + c);
-      } else if (real) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) x.v[e] = q[c + e];
-        w.q[i] = __builtin_bit_cast(u32x4, x);
-      }
-    }
+    for (int i = 0; i < KL; ++i) w.q[i] = *(const u32x4*)(q + (64 * i + 16 * lg) / (int)sizeof(T));
   }
-#pragma unroll
-  for (int c = 0; c < CH; ++c) w.o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  w.top = -INFINITY;
-  w.sum = 0.f;
   const float scale = a.scale * 1.4426950408889634f;     // scores in powers of two
 
   // Where the 16-key parts of the next 64 / SUB steps lie, one part a lane: elements from the cache's beginning
   // (16 keys never straddle a page), 0 and a bit in `out` for a part that no row sees or whose page is none.
   const int per_page = a.page_size / 16;
+  const int* table = a.table + (long long)r.req * a.table_stride;
   const long long head_off = (long long)hk * a.page_size * DIM;
   long long at = 0;
-  unsigned long long out = 0;
+  unsigned long long out = 0, stray = 0;
   auto locate = [&](int first) {
     const int t = first + lane / SUB;
     const int key = r.begin + t * STEP + 16 * (lane % SUB);
-    at = 0;
-    bool bad = true;
-    if (t < t1 && key < r.end) {
-      const int part = key / 16, page = part / per_page;
-      const int id = a.table[(long long)r.req * a.table_stride + page];
-      bad = id < 0 || id >= a.pages;
-      if (!bad) at = (long long)id * a.page_stride + head_off + (long long)(part - page * per_page) * 16 * DIM;
-      else if (a.err_flag) atomicOr(a.err_flag, 1);
-    }
-    out = __ballot(bad);
+    const bool seen = t < t1 && key < r.end;
+    const int part = (seen ? key : r.begin) / 16, page = part / per_page;
+    const int id = table[page];
+    const bool there = id >= 0 && id < a.pages;
+    stray |= __ballot(seen && !there);
+    out = __ballot(!seen || !there);
+    at = seen && there ? (long long)id * a.page_stride + head_off + (long long)(part - page * per_page) * 16 * DIM : 0;
   };
   auto part_at = [&](int i) -> long long {               // the part that lane i has located, the same for the wave
     const unsigned lo = __builtin_amdgcn_readlane((unsigned)at, i), hi = __builtin_amdgcn_readlane((unsigned)(at >> 32), i);
@@ -720,41 +760,70 @@ __device__ __forceinline__ void att_part(const PagedAttArgs& a, const AttPlan& p
   };
   const T *kc = (const T*)a.k_cache, *vc = (const T*)a.v_cache;
   constexpr int ROUND = WAVE / SUB;                      // steps that one call of locate() serves
-  int t = t0, in = 0;
-  if (t < t1) {
+
+  for (int alone = -1;;) {                               // -1: all rows together, else the row that is taken
+    // keys that any and that every column in question sees
+    const bool mine = real && (alone < 0 || my_row == alone);
+    int all_from = mine ? begin : 0, all_to = mine ? end : 0x7fffffff, any_from = mine ? begin : 0x7fffffff, any_to = mine ? end : 0;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+      all_from = max(all_from, __shfl_xor(all_from, d, WAVE));
+      all_to = min(all_to, __shfl_xor(all_to, d, WAVE));
+      any_from = min(any_from, __shfl_xor(any_from, d, WAVE));
+      any_to = max(any_to, __shfl_xor(any_to, d, WAVE));
+    }
+    all_from = __builtin_amdgcn_readfirstlane(all_from);
+    all_to = __builtin_amdgcn_readfirstlane(all_to);
+    any_from = __builtin_amdgcn_readfirstlane(any_from);
+    any_to = __builtin_amdgcn_readfirstlane(any_to);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) w.o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    w.top = -INFINITY;
+    w.sum = 0.f;
+    int t = t0, in = 0;
+    long long here[SUB];
     locate(t);
 #pragma unroll
-    for (int u = 0; u < SUB; ++u) w.load_k(u, kc + part_at(u), lane);
-#pragma unroll
-    for (int u = 0; u < SUB; ++u) w.load_v(u, vc + part_at(u), lane);
-  }
-  while (t < t1) {
-    const int key0 = r.begin + t * STEP;
-    const unsigned bad = (unsigned)(out >> (in * SUB)) & ((1u << SUB) - 1);
-    f32x4 s[SUB];
-    w.scores(s);
-    ++t;
-    ++in;
-    long long next[SUB];
-    if (t < t1) {
-      if (in == ROUND) {
-        locate(t);
-        in = 0;
-      }
-#pragma unroll
-      for (int u = 0; u < SUB; ++u) {
-        next[u] = part_at(in * SUB + u);
-        w.load_k(u, kc + next[u], lane);
-      }
+    for (int u = 0; u < SUB; ++u) {
+      here[u] = part_at(u);
+      w.load_k(u, kc + here[u], lane, 0);
     }
 #pragma unroll
-    for (int u = 0; u < SUB; ++u) s[u] *= scale;
-    if (bad == 0 && key0 >= all_from && key0 + STEP <= all_to) {
-      w.soften(s);
-      w.template weigh<false>(w.o, s, 0);
-    } else {
-      // this lane's keys, as its own column sees them and, below, as each row of the run does: what a row does not see has
-      // to be left out of V too, or a weight of 0 would meet an infinity or a NaN there
+    for (int u = 0; u < SUB; ++u) w.load_v(u, vc + here[u], lane, 0);
+    while (t < t1) {
+      const int key0 = r.begin + t * STEP;
+      const unsigned bad = (unsigned)(out >> (in * SUB)) & ((1u << SUB) - 1);
+      f32x4 s[SUB];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int pass = 0; pass < PASSES; ++pass) {
+        if (pass > 0) {
+#pragma unroll
+          for (int u = 0; u < SUB; ++u) w.load_k(u, kc + here[u], lane, pass);
+        }
+        w.scores(s, pass);
+      }
+      ++t;
+      ++in;
+      long long next[SUB];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) next[u] = here[u];
+      if (t < t1) {
+        if (in == ROUND) {
+          locate(t);
+          in = 0;
+        }
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+          next[u] = part_at(in * SUB + u);
+          w.load_k(u, kc + next[u], lane, 0);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) s[u] *= scale;
+      const bool all = bad == 0 && key0 >= all_from && key0 + STEP <= all_to;
+      // this lane's keys that lie in [from, to): one bit each, 4 * part + row
       auto sees = [&](int from, int to) {
         unsigned m = 0;
 #pragma unroll
@@ -766,70 +835,49 @@ __device__ __forceinline__ void att_part(const PagedAttArgs& a, const AttPlan& p
           }
         return m;
       };
-      const unsigned mine = sees(begin, end);
+      if (!all) {
+        const unsigned m = sees(begin, end);
 #pragma unroll
-      for (int u = 0; u < SUB; ++u)
+        for (int u = 0; u < SUB; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[u][e] = mine >> (4 * u + e) & 1 ? s[u][e] : -INFINITY;
+          for (int e = 0; e < 4; ++e) s[u][e] = m >> (4 * u + e) & 1 ? s[u][e] : -INFINITY;
+      }
       w.soften(s);
-      if (r.n == 1) {
-        w.template weigh<true>(w.o, s, sees(all_from, all_to));
-      } else {
-        for (int i = 0; i < r.n; ++i) {
-          int from, to;
-          att_row_keys(a, r.row + i, from, to);
-          f32x4 add[CH];
+      const typename Tile::Weights x = Tile::weights(s);
 #pragma unroll
-          for (int c = 0; c < CH; ++c) add[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-          w.template weigh<true>(add, s, sees(from, to));
-          const bool own = real && my_row == i;
+      for (int pass = 0; pass < PASSES; ++pass) {
+        if (pass > 0) {
 #pragma unroll
-          for (int c = 0; c < CH; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w.o[c][e] += own ? add[c][e] : 0.f;
+          for (int u = 0; u < SUB; ++u) w.load_v(u, vc + here[u], lane, pass);
         }
+        if (!all) w.mask_v(sees(any_from, any_to));
+#pragma unroll
+        for (int d = 0; d < Tile::VP; ++d) w.weigh(&w.o[(pass * Tile::VP + d) * Tile::PER], d, x);
+      }
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) here[u] = next[u];
+      if (t < t1) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) w.load_v(u, vc + here[u], lane, 0);
       }
     }
-    if (t < t1) {
 #pragma unroll
-      for (int u = 0; u < SUB; ++u) w.load_v(u, vc + next[u], lane);
+    for (int c = 0; c < CH; ++c) ATT_SETTLE(w.o[c]);
+    w.sum = col_sum(w.sum);
+    if (alone < 0 && r.n > 1) {
+      bool wild = false;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wild |= !(fabsf(w.o[c][e]) < INFINITY);
+      if (__ballot(wild && real)) {
+        alone = 0;
+        continue;
+      }
     }
+    if (mine) att_leave<T, DIM>(a, p, w, col, lg, r.row + my_row, hk * group + my_head, begin >= end, whole, slot);
+    if (alone < 0 || ++alone == r.n) return stray != 0;
   }
-  w.sum = col_sum(w.sum);
-  if (!real) return;
-  // the lane's DIM / 4 channels lie beside each other: 4 lg * CH and on
-  if (!whole) {
-    float* to = slot + col * ROW;
-#pragma unroll
-    for (int c = 0; c < 4 * CH; c += 4) {
-      f32x4 x;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = w.o[(c + e) % CH][(c + e) / CH];
-      *(f32x4*)(to + 4 * lg * CH + c) = x;
-    }
-    if (lg == 0) {
-      to[DIM] = w.top;
-      to[DIM + 1] = w.sum;
-    }
-    return;
-  }
-  const bool none = begin >= end;
-  const int h = hk * group + my_head;
-  T* to = (T*)a.out + (long long)(r.row + my_row) * a.out_row + (long long)h * a.out_head + 4 * lg * CH;
-  constexpr int N = 16 / sizeof(T);
-#pragma unroll
-  for (int c = 0; c < 4 * CH; c += N) {
-    Pack<T, N> x;
-#pragma unroll
-    for (int e = 0; e < N; ++e) x.v[e] = Conv<T>::from(none ? 0.f : w.o[(c + e) % CH][(c + e) / CH] / w.sum);
-    if (p.wide_out) {
-      *(Pack<T, N>*)(to + c) = x;
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) to[c + e] = x.v[e];
-    }
-  }
-  if (a.lse && lg == 0) att_write_lse(a, r.row + my_row, h, w.top, w.sum, none);
 }
 
 // requests and positions outside the table are not followed
@@ -841,13 +889,14 @@ __device__ __forceinline__ void att_flag_row(const PagedAttArgs& a, int row) {
 
 // A wave a unit: for lengths that a wave takes in a short time, and for so many units that their lengths even out.
 template <typename T, int DIM>
-__global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attention_kernel(PagedAttArgs a, AttPlan p) {
+__global__ __launch_bounds__(ATT_THREADS, 2) void paged_attention_kernel(PagedAttArgs a, AttPlan p) {
   const long long n = (long long)blockIdx.x * ATT_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int row = (int)(n / p.units), unit = (int)(n - (long long)row * p.units);
   if (row >= a.rows) return;
   if (unit == 0 && threadIdx.x % WAVE == 0) att_flag_row(a, row);
   Run r;
-  if (att_run(a, p, row, r)) att_part<T, DIM>(a, p, r, unit, 0, att_run_steps<AttTile<T, DIM>::STEP>(r), true, nullptr);
+  if (att_run(a, p, row, r) && att_part<T, DIM>(a, p, r, unit, 0, att_run_steps<AttTile<T, DIM>::STEP>(r), true, nullptr) && a.err_flag)
+    atomicOr(a.err_flag, 1);
 }
 
 // The line of work cut into p.pieces equal pieces, a wave a piece, a block four that follow each other: a long row beside
@@ -861,7 +910,7 @@ __global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attenti
     int live, row, n, unit, from, to;
     int more;               // [0]: it goes on in the next wave; [1]: blocks behind this one that hold some of it
   };
-  __shared__ float lds[ATT_WAVES][2][ATT_COLS * ROW];
+  __shared__ alignas(16) float lds[ATT_WAVES][2][ATT_COLS * ROW];
   __shared__ Part left[ATT_WAVES][2];
   __shared__ long long wave_sum[ATT_WAVES];
   __shared__ long long found_at[ATT_WAVES];
@@ -920,6 +969,7 @@ __global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attenti
     long long run_at = (long long)((unsigned long long)(unsigned)same((int)(at >> 32)) << 32 | (unsigned)same((int)at)) * p.units;
     long long pos = first;
     int row = r.row;
+    bool stray = false;
     for (;;) {
       const int steps = att_run_steps<STEP>(r);
       for (int unit = (int)((pos - run_at) / steps); unit < p.units && pos < last; ++unit) {
@@ -929,13 +979,14 @@ __global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attenti
         if (!whole && lane == 0)
           left[wave][t0 == 0] = Part{1, r.row, r.n, unit, r.from, r.end,
                                      t0 == 0 ? (int)((unit_at + steps - 1) / (size * ATT_WAVES)) - (int)blockIdx.x : t1 < steps};
-        att_part<T, DIM>(a, p, r, unit, t0, t1, whole, lds[wave][t0 == 0]);
+        stray |= att_part<T, DIM>(a, p, r, unit, t0, t1, whole, lds[wave][t0 == 0]);
         pos = unit_at + t1;
       }
       if (pos >= last) break;
       run_at += (long long)steps * p.units;
       do ++row; while (!att_run(a, p, row, r));           // pos < total: there is one
     }
+    if (stray && a.err_flag) atomicOr(a.err_flag, 1);
   }
   __syncthreads();
 
@@ -956,18 +1007,28 @@ __global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attenti
       const int m = i / (DIM / 4), c = i % (DIM / 4) * 4;
       int row, hd;
       if (!att_column(m, head.n, group, tile, row, hd)) continue;
-      const float* part[ATT_WAVES + 1];
-      int n = 0;
-      if (k > 0) part[n++] = lds[k - 1][1] + m * ROW;
-      for (int w = k; w < w1; ++w) part[n++] = lds[w][0] + m * ROW;
-      float top = -INFINITY, sum = 0.f;
-      for (int j = 0; j < n; ++j) top = fmaxf(top, part[j][DIM]);
+      // the chain's parts lie at most ATT_WAVES + 1 in a row: [1] of wave k - 1, [0] of waves k .. w1 - 1
+      float tops[ATT_WAVES + 1], sums[ATT_WAVES + 1];
+      f32x4 xs[ATT_WAVES + 1];
+#pragma unroll
+      for (int j = 0; j <= ATT_WAVES; ++j) {
+        const bool there = j == 0 ? k > 0 : j > k && j <= w1;
+        const float* part = lds[j == 0 ? (there ? k - 1 : 0) : j - 1][j == 0] + m * ROW;
+        tops[j] = there ? part[DIM] : -INFINITY;
+        sums[j] = there ? part[DIM + 1] : 0.f;
+        xs[j] = *(const f32x4*)(part + c);                 // of no weight where there is no part
+        if (!there) xs[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      float top = tops[0], sum = 0.f;
+#pragma unroll
+      for (int j = 1; j <= ATT_WAVES; ++j) top = fmaxf(top, tops[j]);
       const float base = top == -INFINITY ? 0.f : top;
       f32x4 x = {0.f, 0.f, 0.f, 0.f};
-      for (int j = 0; j < n; ++j) {
-        const float f = att_exp2(part[j][DIM] - base);
-        sum += f * part[j][DIM + 1];
-        x += f * *(const f32x4*)(part[j] + c);
+#pragma unroll
+      for (int j = 0; j <= ATT_WAVES; ++j) {
+        const float f = att_exp2(tops[j] - base);
+        sum += f * sums[j];
+        x += f * xs[j];
       }
       if (!whole) {
         *(f32x4*)(slot + m * ROW + c) = x;
@@ -979,65 +1040,67 @@ __global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attenti
       }
       int from = head.from, to = head.to;
       if (head.n > 1) att_row_keys(a, head.row + row, from, to);
-      att_write<T>(a, head.row + row, hk * group + hd, c, x, sum, from >= to);
+      att_write<T>(a, p.wide_out, head.row + row, hk * group + hd, c, x, sum, from >= to);
       if (a.lse && c == 0) att_write_lse(a, head.row + row, hk * group + hd, top, sum, from >= to);
     }
   }
 }
 
-// Joins the parts of the unit that begins in block blockIdx.x and ends in a later one, a block a column (every gridDim.y-th):
-// first the parts' weights, then the weighted sum, dim / 4 threads a part and as many parts at once as that leaves threads
-// for, each its parts in the order of the keys: the result does not depend on which block was done first.
+// Joins the parts of the unit that begins in block blockIdx.x and ends in a later one, a block a column: dim / 4 threads hold a
+// part, the block as many parts as that leaves threads for, each its parts in the order of the keys, so that the result
+// does not depend on which block was done first.
 template <typename T>
 __global__ __launch_bounds__(ATT_THREADS) void paged_join_kernel(PagedAttArgs a, AttPlan p, float* ws, const AttJoin* joins) {
-  __shared__ float weight[ATT_PIECES / ATT_WAVES];
-  __shared__ float wave_top[ATT_WAVES], wave_sum[ATT_WAVES];
   __shared__ f32x4 acc[ATT_THREADS];
+  __shared__ float wave_sum[ATT_WAVES];
   const AttJoin j = joins[blockIdx.x];
-  if (j.parts == 0) return;
-  const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
-  const int group = a.heads / a.kv_heads, ROW = a.dim + 4, parts = j.parts + 1;
+  const int group = a.heads / a.kv_heads, ROW = a.dim + 4, parts = j.parts + 1, m = blockIdx.y, hk = j.unit / p.tiles;
+  int row, head;
+  if (parts == 1 || !att_column(m, j.n, group, j.unit - hk * p.tiles, row, head)) return;
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1);
   const int quads = a.dim / 4, at_once = ATT_THREADS / quads, mine = tid / quads, quad = tid - mine * quads;
-  const int hk = j.unit / p.tiles;
-  for (int m = blockIdx.y; m < ATT_COLS; m += gridDim.y) {
-    int row, head;
-    if (!att_column(m, j.n, group, j.unit - hk * p.tiles, row, head)) break;   // columns that are none come last
-    auto part = [&](int i) { return att_slot(ws, blockIdx.x + i, i == 0, a.dim) + m * ROW; };
-    float top = -INFINITY, sum = 0.f;
-    for (int i = tid; i < parts; i += ATT_THREADS) top = fmaxf(top, weight[i] = part(i)[a.dim]);
+  int from, to;
+  att_row_keys(a, j.row + row, from, to);
+  auto part = [&](int i) { return att_slot(ws, blockIdx.x + i, i == 0, a.dim) + m * ROW; };
+  constexpr int AHEAD = 4;                                 // loads in flight a thread
+  f32x4 v[AHEAD];
+  auto load = [&](int i0) {                                // what there is not is read from the last part, and has no weight
 #pragma unroll
-    for (int d = 1; d < WAVE; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, WAVE));
-    if (lane == 0) wave_top[wave] = top;
-    __syncthreads();
-    for (int i = 0; i < ATT_WAVES; ++i) top = fmaxf(top, wave_top[i]);
-    const float base = top == -INFINITY ? 0.f : top;
-    for (int i = tid; i < parts; i += ATT_THREADS) {     // the thread's own entries
-      const float f = att_exp2(weight[i] - base);
-      sum += f * part(i)[a.dim + 1];
-      weight[i] = f;
-    }
+    for (int u = 0; u < AHEAD; ++u) v[u] = *(const f32x4*)(part(min(i0 + u * at_once + mine, parts - 1)) + 4 * quad);
+  };
+  load(0);
+  float top = -INFINITY, sum = 0.f;
+  for (int i = lane; i < parts; i += WAVE) top = fmaxf(top, part(i)[a.dim]);
 #pragma unroll
-    for (int d = 1; d < WAVE; d <<= 1) sum += __shfl_xor(sum, d, WAVE);
-    if (lane == 0) wave_sum[wave] = sum;
-    __syncthreads();
-    sum = 0.f;
-    for (int i = 0; i < ATT_WAVES; ++i) sum += wave_sum[i];
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    if (mine < at_once) {
-#pragma unroll 8
-      for (int i = mine; i < parts; i += at_once) x += weight[i] * *(const f32x4*)(part(i) + 4 * quad);
+  for (int d = 1; d < WAVE; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, WAVE));
+  const float base = top == -INFINITY ? 0.f : top;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  float f = 0.f;
+  const int batch = AHEAD * at_once;                       // parts that the block has in flight
+  for (int i = 0; i < parts; i += batch) {                 // the same trips for every lane: all of them hold weights
+    if (i > 0) load(i);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int k = i + u * at_once + mine;
+      const bool there = mine < at_once && k < parts;
+      const float g = there ? att_exp2(part(k)[a.dim] - base) : 0.f;
+      if (there && quad == 0) f += g * part(k)[a.dim + 1];
+      if (there) x += g * v[u];
     }
-    acc[tid] = x;
-    int from, to;
-    att_row_keys(a, j.row + row, from, to);
-    __syncthreads();
-    if (mine == 0) {
-      for (int i = 1; i < at_once; ++i) x += acc[i * quads + quad];
-      att_write<T>(a, j.row + row, hk * group + head, 4 * quad, x, sum, from >= to);
-    }
-    if (a.lse && tid == 0) att_write_lse(a, j.row + row, hk * group + head, top, sum, from >= to);
-    __syncthreads();                                     // before the LDS is written again
   }
+  sum = f;
+#pragma unroll
+  for (int d = 1; d < WAVE; d <<= 1) sum += __shfl_xor(sum, d, WAVE);
+  if (lane == 0) wave_sum[tid / WAVE] = sum;
+  acc[tid] = x;
+  __syncthreads();
+  sum = 0.f;
+  for (int i = 0; i < ATT_WAVES; ++i) sum += wave_sum[i];
+  if (mine == 0) {
+    for (int i = 1; i < at_once; ++i) x += acc[i * quads + quad];
+    att_write<T>(a, p.wide_out, j.row + row, hk * group + head, 4 * quad, x, sum, from >= to);
+  }
+  if (a.lse && tid == 0) att_write_lse(a, j.row + row, hk * group + head, top, sum, from >= to);
 }
 
 AttPlan att_plan(int rows, int heads, int kv_heads, long long max_keys, bool& split) {
@@ -1047,7 +1110,7 @@ AttPlan att_plan(int rows, int heads, int kv_heads, long long max_keys, bool& sp
   p.tiles = (group + ATT_COLS - 1) / ATT_COLS;
   p.units = kv_heads * p.tiles;
   p.pieces = ATT_PIECES;
-  p.wide_q = p.wide_out = 0;
+  p.wide_out = 0;
   const long long units = (long long)rows * p.units;
   if (max_keys > 0 && max_keys < (1 << 30)) {            // no more pieces than their least size fills, in steps of 16 keys
     const long long most = units * ((max_keys + 15) / 16 + 1) / ATT_MIN_STEPS + 1;
@@ -1067,7 +1130,7 @@ hipError_t start_attention(const PagedAttArgs& a, const AttPlan& p, bool split, 
   const int blocks = p.pieces / ATT_WAVES;
   AttJoin* joins = (AttJoin*)att_slot((float*)ws, blocks, 0, DIM);
   hipLaunchKernelGGL((paged_attention_split_kernel<T, DIM>), dim3(blocks), dim3(ATT_THREADS), 0, s, a, p, (float*)ws, joins);
-  const int cols = min(4, a.heads / a.kv_heads * p.rows_per_run);
+  const int cols = min(ATT_COLS, a.heads / a.kv_heads * p.rows_per_run);
   hipLaunchKernelGGL((paged_join_kernel<T>), dim3(blocks, cols), dim3(ATT_THREADS), 0, s, a, p, (float*)ws, joins);
   return hipGetLastError();
 }
@@ -1110,7 +1173,6 @@ hipError_t launch_paged_attention(const PagedAttArgs& a, long long max_keys, voi
   bool split;
   AttPlan p = att_plan(a.rows, a.heads, a.kv_heads, max_keys, split);
   const int size = a.dtype == VITS_TYPE_F32 ? 4 : 2;
-  p.wide_q = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_row * size % 16 == 0 && a.q_head * size % 16 == 0;
   p.wide_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_row * size % 16 == 0 && a.out_head * size % 16 == 0;
   if (a.dtype == VITS_TYPE_F32) return start_attention_t<float>(a, p, split, ws, s);
   return a.dtype == VITS_TYPE_F16 ? start_attention_t<_Float16>(a, p, split, ws, s) : start_attention_t<__bf16>(a, p, split, ws, s);

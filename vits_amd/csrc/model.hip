@@ -1510,8 +1510,8 @@ int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const 
   if (page_stride < (int64_t)kv_heads * page_size * dim) return fail(VITS_ERR_INVALID, "paged attention: pages overlap");
   if (q && q == out) return fail(VITS_ERR_INVALID, "paged attention: cannot run in place");
   const int size = dtype == VITS_TYPE_F32 ? 4 : 2;
-  if ((((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) || (page_stride * size) % 16)
-    return fail(VITS_ERR_INVALID, "paged attention: the caches and their pages must begin on 16-byte addresses");
+  if ((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)q) & 15) || (page_stride * size) % 16 || (q_row * size) % 16 || (q_head * size) % 16)
+    return fail(VITS_ERR_INVALID, "paged attention: the caches, their pages and the heads of q must begin on 16-byte addresses");
   if (ws_bytes < paged_attention_workspace(rows, heads, kv_heads, dim, max_keys) || (ws_bytes > 0 && !ws) || ((uintptr_t)ws & 15))
     return fail(VITS_ERR_WORKSPACE, "paged attention: workspace too small or not on a 16-byte address");
   if (rows == 0) return VITS_OK;

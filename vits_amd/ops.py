@@ -271,6 +271,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         _apart(what, q, out)
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous()):
         raise ValueError(f"paged_attention: lse must be contiguous float32 [{rows}, {heads}], got {lse.dtype} {list(lse.shape)}")
+    if (q.data_ptr() | q.stride(0) * q.element_size() | q.stride(1) * q.element_size()) & 15:
+        q = q.clone(memory_format=torch.contiguous_format)      # the library reads heads on 16-byte addresses
     keys = table.shape[1] * page_size if max_keys is None else max_keys
     nbytes = N.lib.vits_op_paged_attention_workspace_bytes(rows, heads, kv_heads, dim, keys)
     if nbytes < 0:
