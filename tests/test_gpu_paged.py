@@ -201,7 +201,7 @@ def test_plan_python_refusals(ops):
             ops.page_plan(*good, rows=4, out=bad)
     with pytest.raises(ValueError, match="seven"):
         ops.page_plan(*good, rows=4, out=plan[:6])
-    with pytest.raises(ValueError, match="overlaps"):
+    with pytest.raises(RuntimeError, match="overlaps"):
         ops.page_plan(*good, rows=4, out=plan._replace(lengths=pages.lengths))
 
 

@@ -345,6 +345,17 @@ ConvDesc need_conv(vits_model* m, const std::string& name, int cin, int rows, in
 
 namespace {
 // shared checks of the paged-cache operators
+struct Span {
+  const char* p;
+  int64_t n;                 // bytes
+};
+Span span(const void* p, int64_t n) { return Span{(const char*)p, p ? n : 0}; }
+// of rows x heads x dim elements with these strides
+Span span(const void* p, int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t dim, int size) {
+  return span(p, rows > 0 && heads > 0 ? ((rows - 1) * row + (heads - 1) * head + dim) * size : 0);
+}
+bool overlap(const Span& a, const Span& b) { return a.n > 0 && b.n > 0 && a.p < b.p + b.n && b.p < a.p + a.n; }
+
 int check_page_size(int page_size) {
   if (page_size < PAGED_PAGE_UNIT || page_size % PAGED_PAGE_UNIT || page_size > 65536)
     return fail(VITS_ERR_INVALID, "page_size must be a multiple of 16 and at most 65536");
@@ -1443,8 +1454,17 @@ int vits_op_page_plan(const int* lengths, const int* grow, int requests, int* ta
     return fail(VITS_ERR_INVALID, "page plan: 1 to 65535 requests, up to 2^30 rows and pages, a table of at least one page "
                                   "a request and rows that do not overlap required");
   TRY(check_page_size(page_size));
-  if (lengths_out == lengths || lengths_out == grow || cursor_out == cursor)
-    return fail(VITS_ERR_INVALID, "page plan: cannot run in place (every block reads all lengths and the cursor)");
+  // every block reads all lengths and the cursor, so nothing may be written over them, nor one output over another
+  const Span in[3] = {span(lengths, 4ll * requests), span(grow, 4ll * requests), span(cursor, 16)};
+  const Span outs[9] = {span(table, 4ll * ((requests - 1) * table_stride + width)), span(ring, 4ll * pages), span(lengths_out, 4ll * requests),
+                        span(cursor_out, 16), span(row_start, 4ll * (requests + 1)), span(row_request, 4ll * rows),
+                        span(row_position, 4ll * rows), span(row_slot, 8ll * rows), span(status, 4)};
+  for (int i = 0; i < 9; ++i) {
+    for (const Span& x : in)
+      if (overlap(outs[i], x)) return fail(VITS_ERR_INVALID, "page plan: cannot run in place: an output overlaps an input");
+    for (int j = 0; j < i; ++j)
+      if (overlap(outs[i], outs[j])) return fail(VITS_ERR_INVALID, "page plan: cannot run in place: two outputs overlap");
+  }
   PagePlanArgs a{};
   a.lengths = lengths; a.grow = grow; a.requests = requests;
   a.table = table; a.table_stride = table_stride; a.width = width;
@@ -1474,9 +1494,24 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
     TRY(check_page_size(page_size));
     if (page_stride < (int64_t)kv_heads * page_size * dim) return fail(VITS_ERR_INVALID, "rotary store: pages overlap");
   }
-  if (q == out && q && (q_row != out_row || q_head != out_head))
-    return fail(VITS_ERR_INVALID, "rotary store: in place needs the same strides on both sides");
   if (rows == 0) return VITS_OK;
+  const int size = dtype == VITS_TYPE_F32 ? 4 : 2;
+  const Span to = span(out, rows, out_row, q ? heads : 0, out_head, dim, size), from = span(q, rows, q_row, heads, q_head, dim, size);
+  if (q && !(q == out && q_row == out_row && q_head == out_head) && overlap(from, to))
+    return fail(VITS_ERR_INVALID, "rotary store: in place needs the same strides on both sides, and no other overlap");
+  if (k) {
+    const int64_t cache = ((pages - 1) * page_stride + (int64_t)kv_heads * page_size * dim) * size;
+    const Span caches[2] = {span(k_cache, cache), span(v_cache, cache)};
+    const Span ins[3] = {from, span(k, rows, k_row, kv_heads, k_head, dim, size), span(v, rows, v_row, kv_heads, v_head, dim, size)};
+    // (q's own rows may be written in place between k's and v's)
+    for (const Span& c : caches) {
+      if (overlap(c, to)) return fail(VITS_ERR_INVALID, "rotary store: out overlaps a cache");
+      for (const Span& x : ins)
+        if (overlap(c, x)) return fail(VITS_ERR_INVALID, "rotary store: a cache overlaps an input");
+    }
+    if (q && q != out && (overlap(to, ins[1]) || overlap(to, ins[2])))
+      return fail(VITS_ERR_INVALID, "rotary store: out overlaps k or v");
+  }
   RotaryArgs a{};
   a.q = q; a.q_row = q_row; a.q_head = q_head; a.out = out; a.out_row = out_row; a.out_head = out_head; a.heads = heads;
   a.k = k; a.k_row = k_row; a.k_head = k_head; a.v = v; a.v_row = v_row; a.v_head = v_head;
@@ -1508,8 +1543,9 @@ int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const 
     return fail(VITS_ERR_INVALID, "paged attention: at least one page, request and table column, a table of at most 2^30 tokens a "
                                   "request whose rows do not overlap and a window that is not negative required");
   if (page_stride < (int64_t)kv_heads * page_size * dim) return fail(VITS_ERR_INVALID, "paged attention: pages overlap");
-  if (q && q == out) return fail(VITS_ERR_INVALID, "paged attention: cannot run in place");
   const int size = dtype == VITS_TYPE_F32 ? 4 : 2;
+  if (overlap(span(q, rows, q_row, heads, q_head, dim, size), span(out, rows, out_row, heads, out_head, dim, size)))
+    return fail(VITS_ERR_INVALID, "paged attention: cannot run in place");
   if ((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)q) & 15) || (page_stride * size) % 16 || (q_row * size) % 16 || (q_head * size) % 16)
     return fail(VITS_ERR_INVALID, "paged attention: the caches, their pages and the heads of q must begin on 16-byte addresses");
   if (ws_bytes < paged_attention_workspace(rows, heads, kv_heads, dim, max_keys) || (ws_bytes > 0 && !ws) || ((uintptr_t)ws & 15))

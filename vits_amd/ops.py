@@ -18,6 +18,7 @@ raise ValueError, a library error VitsError; ids on the device that are out of r
 whole rows)."""
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple, Optional, Sequence
 
@@ -54,20 +55,6 @@ def new_pages(requests: int, width: int, pages: int, device="cuda") -> Pages:
                  torch.tensor([0, pages], dtype=torch.int64, device=device))
 
 
-def _on_gpu(what: str, first: torch.Tensor, *more) -> torch.device:
-    device = first.device
-    if device.type != "cuda":
-        raise ValueError(f"{what}: tensors must be on a GPU (vits_amd has no CPU path)")
-    for t in more:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: all tensors must be on one GPU, got {t.device} and {device}")
-    return device
-
-
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 def _flat(what: str, name: str, t: torch.Tensor, dtype, n: Optional[int] = None) -> None:
     if t.dtype != dtype or t.dim() != 1 or (n is not None and t.numel() != n) or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be contiguous {dtype} [{'n' if n is None else n}], got {t.dtype} {list(t.shape)}")
@@ -85,34 +72,38 @@ def _table(what: str, table: torch.Tensor) -> None:
         raise ValueError(f"{what}: table must be int32 [requests, width] with contiguous rows, got {table.dtype} {list(table.shape)}")
 
 
-def _caches(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
-    for t in (k_cache, v_cache):
-        if t.dim() != 4 or t.dtype not in _TYPES:
-            raise ValueError(f"{what}: caches must be fp32, fp16 or bf16 [pages, kv_heads, page_size, dim], got {t.dtype} {list(t.shape)}")
-    _, _, page, dim = k_cache.shape
-    if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype or k_cache.stride() != v_cache.stride() \
-            or k_cache.stride()[1:] != (page * dim, dim, 1):
-        raise ValueError(f"{what}: k_cache and v_cache must be alike and contiguous within a page, got {list(k_cache.shape)} and "
-                         f"{list(v_cache.shape)}, strides {list(k_cache.stride())} and {list(v_cache.stride())}")
+def _caches(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor):
+    """Shape and page stride of the two caches."""
+    shape, strides = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or k_cache.dtype not in _TYPES or v_cache.dtype != k_cache.dtype or v_cache.shape != shape or v_cache.stride() != strides \
+            or strides[3] != 1 or strides[2] != shape[3] or strides[1] != shape[2] * shape[3]:
+        raise ValueError(f"{what}: k_cache and v_cache must be alike, fp32, fp16 or bf16 [pages, kv_heads, page_size, dim], and contiguous within a "
+                         f"page, got {k_cache.dtype} {list(shape)} and {v_cache.dtype} {list(v_cache.shape)}, strides {list(strides)} and "
+                         f"{list(v_cache.stride())}")
+    return shape, strides[0]
 
 
-def _err_flag(what: str, flag: Optional[torch.Tensor]) -> int:
-    if flag is None:
-        return 0
-    _flat(what, "err_flag", flag, torch.int32, 1)
-    return flag.data_ptr()
+def _device(what: str, first: torch.Tensor, *more) -> int:
+    """The GPU that every tensor given has to be on."""
+    index = first.get_device()
+    if index < 0:
+        raise ValueError(f"{what}: tensors must be on a GPU (vits_amd has no CPU path)")
+    for t in more:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{what}: all tensors must be on one GPU, got {t.device} and {first.device}")
+    return index
 
 
-def _span(t: torch.Tensor):
-    """First and last byte of a tensor's elements, as a half-open range."""
-    n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
-    return t.data_ptr(), t.data_ptr() + n * t.element_size()
-
-
-def _apart(what: str, a: torch.Tensor, b: torch.Tensor) -> None:
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    if a0 < b1 and b0 < a1:
-        raise ValueError(f"{what}: an output overlaps an input")
+def _call(what: str, index: int, fn, *args) -> None:
+    """fn(*args, stream) on the current stream of GPU `index`.  (The two private functions are what torch.cuda.current_device and
+    current_stream come down to; those take 2 us a call, as much as a third of the rest of a call.)"""
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        N.check(rc, what)
 
 
 def page_plan(lengths: torch.Tensor, grow: torch.Tensor, table: torch.Tensor, ring: torch.Tensor, cursor: torch.Tensor, page_size: int,
@@ -123,39 +114,33 @@ def page_plan(lengths: torch.Tensor, grow: torch.Tensor, table: torch.Tensor, ri
     cursor are returned beside the old ones, so the caller decides when the step counts.  Where the step does not fit,
     `status` says why and nothing is changed."""
     what = "page_plan"
+    i32, i64 = torch.int32, torch.int64
     n = lengths.numel()
     if out is None:
         if rows is None:
             raise ValueError("page_plan: give rows or out")
-        i32 = dict(dtype=torch.int32, device=lengths.device)
-        i64 = dict(dtype=torch.int64, device=lengths.device)
-        out = (torch.empty(n, **i32), torch.empty(2, **i64), torch.empty(n + 1, **i32), torch.empty(rows, **i32),
-               torch.empty(rows, **i32), torch.empty(rows, **i64), torch.empty(1, **i32))
+        d32, d64 = dict(dtype=i32, device=lengths.device), dict(dtype=i64, device=lengths.device)
+        out = (torch.empty(n, **d32), torch.empty(2, **d64), torch.empty(n + 1, **d32), torch.empty(rows, **d32),
+               torch.empty(rows, **d32), torch.empty(rows, **d64), torch.empty(1, **d32))
     elif len(out) != 7:
         raise ValueError("page_plan: out must hold a PagePlan's seven tensors")
-    plan = PagePlan(*out)
+    lengths_out, cursor_out, start, request, position, slot, status = out
     if rows is None:
-        rows = plan.request.numel()
-    i32, i64 = torch.int32, torch.int64
-    device = _on_gpu(what, lengths, grow, table, ring, cursor, *plan)
+        rows = request.numel()
+    index = _device(what, lengths, grow, table, ring, cursor, *out)
     for name, t, dtype, k in (("lengths", lengths, i32, n), ("grow", grow, i32, n), ("ring", ring, i32, None), ("cursor", cursor, i64, 2),
-                              ("out.lengths", plan.lengths, i32, n), ("out.cursor", plan.cursor, i64, 2),
-                              ("out.start", plan.start, i32, n + 1), ("out.request", plan.request, i32, rows),
-                              ("out.position", plan.position, i32, rows), ("out.slot", plan.slot, i64, rows),
-                              ("out.status", plan.status, i32, 1)):
-        _flat(what, name, t, dtype, k)
+                              ("out.lengths", lengths_out, i32, n), ("out.cursor", cursor_out, i64, 2), ("out.start", start, i32, n + 1),
+                              ("out.request", request, i32, rows), ("out.position", position, i32, rows), ("out.slot", slot, i64, rows),
+                              ("out.status", status, i32, 1)):
+        if t.dtype != dtype or not t.is_contiguous() or t.dim() != 1 or t.numel() != k:
+            _flat(what, name, t, dtype, k)
     _table(what, table)
     if table.shape[0] != n:
         raise ValueError(f"page_plan: table has {table.shape[0]} rows for {n} requests")
-    for i in (lengths, grow, cursor):
-        for o in (table, ring, *plan):
-            _apart(what, i, o)
-    with torch.cuda.device(device):
-        N.check(N.lib.vits_op_page_plan(
-            lengths.data_ptr(), grow.data_ptr(), n, table.data_ptr(), table.stride(0), table.shape[1], ring.data_ptr(), ring.numel(),
-            cursor.data_ptr(), page_size, plan.lengths.data_ptr(), plan.cursor.data_ptr(), plan.start.data_ptr(),
-            plan.request.data_ptr(), plan.position.data_ptr(), plan.slot.data_ptr(), rows, plan.status.data_ptr(), _stream(device)), what)
-    return plan
+    _call(what, index, N.lib.vits_op_page_plan, lengths.data_ptr(), grow.data_ptr(), n, table.data_ptr(), table.stride(0), table.shape[1],
+          ring.data_ptr(), ring.numel(), cursor.data_ptr(), page_size, lengths_out.data_ptr(), cursor_out.data_ptr(), start.data_ptr(),
+          request.data_ptr(), position.data_ptr(), slot.data_ptr(), rows, status.data_ptr())
+    return out if type(out) is PagePlan else PagePlan(*out)
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original_length: int = 4096,
@@ -198,50 +183,56 @@ def rotary_store(q: Optional[torch.Tensor], k: Optional[torch.Tensor], v: Option
     if q is None and k is None:
         raise ValueError("rotary_store: neither queries nor keys")
     first = q if q is not None else k
-    if first.dim() != 3 or first.dtype not in _TYPES:
-        raise ValueError(f"rotary_store: rows must be fp32, fp16 or bf16 [rows, heads, dim], got {first.dtype} {list(first.shape)}")
+    dtype = first.dtype
+    if first.dim() != 3 or dtype not in _TYPES:
+        raise ValueError(f"rotary_store: rows must be fp32, fp16 or bf16 [rows, heads, dim], got {dtype} {list(first.shape)}")
     rows, _, dim = first.shape
-    device = _on_gpu(what, first, k, v, k_cache, v_cache, position, slot, freq, out, err_flag)
+    index = _device(what, first, k, v, k_cache, v_cache, position, slot, freq, out, err_flag)
     _flat(what, "position", position, torch.int32, rows)
     _flat(what, "freq", freq, torch.float64)
     if slot is not None:
         _flat(what, "slot", slot, torch.int64, rows)
-    qa = oa = (0, 0, 0)
-    heads = 0
+    q_at = q_row = q_head = out_at = out_row = out_head = heads = 0
     if q is not None:
         heads = q.shape[1]
-        _rows(what, "q", q, rows, heads, dim, first.dtype)
+        _rows(what, "q", q, rows, heads, dim, dtype)
         if out is None:
-            out = torch.empty((rows, heads, dim), dtype=q.dtype, device=device)
-            if slot is not None:
-                out.zero_()                     # rows that are no rows are left as they were: not as the allocator found them
+            # rows that are no rows are left as they were: not as the allocator found them
+            out = (torch.empty if slot is None else torch.zeros)((rows, heads, dim), dtype=dtype, device=q.device)
         else:
-            _rows(what, "out", out, rows, heads, dim, first.dtype)
-            if out.data_ptr() != q.data_ptr() or out.stride() != q.stride():
-                _apart(what, q, out)
-        qa, oa = ((t.data_ptr(), t.stride(0), t.stride(1)) for t in (q, out))
+            _rows(what, "out", out, rows, heads, dim, dtype)
+        q_at, (q_row, q_head, _) = q.data_ptr(), q.stride()
+        out_at, (out_row, out_head, _) = out.data_ptr(), out.stride()
     elif out is not None:
         raise ValueError("rotary_store: out without q")
-    ka = va = (0, 0, 0)
-    kc = vc = page_stride = pages = page_size = kv_heads = 0
+    k_at = k_row = k_head = v_at = v_row = v_head = kc = vc = page_stride = pages = page_size = kv_heads = 0
     if k is not None:
         if v is None or k_cache is None or v_cache is None or slot is None:
             raise ValueError("rotary_store: keys need values, both caches and slots")
-        _caches(what, k_cache, v_cache)
-        pages, kv_heads, page_size, _ = k_cache.shape
-        for name, t in (("k", k), ("v", v)):
-            _rows(what, name, t, rows, kv_heads, dim, first.dtype)
-        if k_cache.dtype != first.dtype or k_cache.shape[3] != dim:
-            raise ValueError(f"rotary_store: caches of {k_cache.dtype} with {k_cache.shape[3]} channels for rows of {first.dtype} with {dim}")
-        ka, va = ((t.data_ptr(), t.stride(0), t.stride(1)) for t in (k, v))
-        kc, vc, page_stride = k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0)
+        (pages, kv_heads, page_size, channels), page_stride = _caches(what, k_cache, v_cache)
+        _rows(what, "k", k, rows, kv_heads, dim, dtype)
+        _rows(what, "v", v, rows, kv_heads, dim, dtype)
+        if k_cache.dtype != dtype or channels != dim:
+            raise ValueError(f"rotary_store: caches of {k_cache.dtype} with {channels} channels for rows of {dtype} with {dim}")
+        k_at, (k_row, k_head, _) = k.data_ptr(), k.stride()
+        v_at, (v_row, v_head, _) = v.data_ptr(), v.stride()
+        kc, vc = k_cache.data_ptr(), v_cache.data_ptr()
     elif v is not None or k_cache is not None or v_cache is not None:
         raise ValueError("rotary_store: values or caches without keys")
-    with torch.cuda.device(device):
-        N.check(N.lib.vits_op_rotary_store(
-            *qa, *oa, heads, *ka, *va, kc, vc, page_stride, pages, page_size, kv_heads, dim, _TYPES[first.dtype], position.data_ptr(),
-            N.ptr(slot), rows, freq.data_ptr(), freq.numel(), scale, int(interleaved), _err_flag(what, err_flag), _stream(device)), what)
+    if err_flag is not None:
+        _flat(what, "err_flag", err_flag, torch.int32, 1)
+    _call(what, index, N.lib.vits_op_rotary_store, q_at, q_row, q_head, out_at, out_row, out_head, heads, k_at, k_row, k_head, v_at, v_row, v_head,
+          kc, vc, page_stride, pages, page_size, kv_heads, dim, _TYPES[dtype], position.data_ptr(), N.ptr(slot), rows, freq.data_ptr(),
+          freq.numel(), scale, interleaved, N.ptr(err_flag))
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(rows: int, heads: int, kv_heads: int, dim: int, max_keys: int) -> int:
+    n = N.lib.vits_op_paged_attention_workspace_bytes(rows, heads, kv_heads, dim, max_keys)
+    if n < 0:
+        N.check(-1, "paged_attention")
+    return n
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, request: torch.Tensor,
@@ -257,32 +248,32 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if q.dim() != 3:
         raise ValueError(f"paged_attention: q must be [rows, heads, dim], got {list(q.shape)}")
     rows, heads, dim = q.shape
-    device = _on_gpu(what, q, k_cache, v_cache, table, request, position, out, lse, err_flag)
-    _caches(what, k_cache, v_cache)
-    pages, kv_heads, page_size, _ = k_cache.shape
-    _rows(what, "q", q, rows, heads, k_cache.shape[3], k_cache.dtype)
+    index = _device(what, q, k_cache, v_cache, table, request, position, out, lse, err_flag)
+    (pages, kv_heads, page_size, channels), page_stride = _caches(what, k_cache, v_cache)
+    _rows(what, "q", q, rows, heads, channels, k_cache.dtype)
     _flat(what, "request", request, torch.int32, rows)
     _flat(what, "position", position, torch.int32, rows)
     _table(what, table)
     if out is None:
-        out = torch.zeros((rows, heads, dim), dtype=q.dtype, device=device)
+        out = torch.zeros((rows, heads, dim), dtype=q.dtype, device=q.device)
     else:
         _rows(what, "out", out, rows, heads, dim, q.dtype)
-        _apart(what, q, out)
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous()):
         raise ValueError(f"paged_attention: lse must be contiguous float32 [{rows}, {heads}], got {lse.dtype} {list(lse.shape)}")
-    if (q.data_ptr() | q.stride(0) * q.element_size() | q.stride(1) * q.element_size()) & 15:
+    if err_flag is not None:
+        _flat(what, "err_flag", err_flag, torch.int32, 1)
+    q_row, q_head, _ = q.stride()
+    if (q.data_ptr() | q_row * q.element_size() | q_head * q.element_size()) & 15:
         q = q.clone(memory_format=torch.contiguous_format)      # the library reads heads on 16-byte addresses
-    keys = table.shape[1] * page_size if max_keys is None else max_keys
-    nbytes = N.lib.vits_op_paged_attention_workspace_bytes(rows, heads, kv_heads, dim, keys)
-    if nbytes < 0:
-        N.check(-1, what)
+        q_row, q_head, _ = q.stride()
+    requests, width = table.shape
+    keys = width * page_size if max_keys is None else max_keys
+    nbytes = _workspace_bytes(rows, heads, kv_heads, dim, keys)
     # a workspace of this call's own: calls on different streams, and graphs that run side by side, share none
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    with torch.cuda.device(device):
-        N.check(N.lib.vits_op_paged_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), pages, page_size,
-            table.data_ptr(), table.stride(0), table.shape[1], table.shape[0], request.data_ptr(), position.data_ptr(), rows, heads,
-            kv_heads, dim, _TYPES[q.dtype], 1.0 / math.sqrt(dim) if scale is None else scale, window, keys, out.data_ptr(),
-            out.stride(0), out.stride(1), N.ptr(lse), _err_flag(what, err_flag), N.ptr(ws), nbytes, _stream(device)), what)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    out_row, out_head, _ = out.stride()
+    _call(what, index, N.lib.vits_op_paged_attention, q.data_ptr(), q_row, q_head, k_cache.data_ptr(), v_cache.data_ptr(), page_stride, pages,
+          page_size, table.data_ptr(), table.stride(0), width, requests, request.data_ptr(), position.data_ptr(), rows, heads, kv_heads, dim,
+          _TYPES[q.dtype], 1.0 / math.sqrt(dim) if scale is None else scale, window, keys, out.data_ptr(), out_row, out_head, N.ptr(lse),
+          N.ptr(err_flag), N.ptr(ws), nbytes)
     return out
