@@ -330,9 +330,9 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
  * of exp(scale * q . k_t), -inf for such a row.  Scores, softmax and sums in fp32.  What lies in the cache behind a row's
  * position, and in pages the table does not name for it, has no influence whatever it holds.
  * dim: 32, 64, ... 256; at most 2^23 rows and, by the table, 2^30 tokens a request; caches, pages and the heads of q begin on 16-byte addresses.  max_keys: how many tokens the host knows a row to see
- * at most (0: as many as the table holds); it only guides how the work is split, a row that sees more is right all
+ * at most (0: unknown; a window bounds it too); it only guides how the work is split, a row that sees more is right all
  * the same.  ws: vits_op_paged_attention_workspace_bytes of the same numbers (-1 for a shape that is refused). */
-int64_t vits_op_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int dim, int64_t max_keys);
+int64_t vits_op_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int dim, int dtype, int64_t max_keys);
 int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, const void* v_cache,
                             int64_t page_stride, int pages, int page_size, const int* table, int64_t table_stride, int width,
                             int requests, const int* row_request, const int* row_position, int rows, int heads, int kv_heads,

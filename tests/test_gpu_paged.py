@@ -447,17 +447,54 @@ def rows_q(cache, rows, heads, dim, dtype, gain=1.5):
     return torch.randn(rows, heads, dim, generator=cache.gen, device="cuda").mul_(gain).to(dtype)
 
 
+@pytest.mark.parametrize("max_keys", [None, 10 ** 9])               # a block a unit, or equal pieces of all the work
 @pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
 @pytest.mark.parametrize("heads,hk,dim,page", [(2, 2, 96, 16), (8, 2, 128, 32), (5, 1, 64, 48), (16, 1, 32, 16), (17, 1, 64, 16), (24, 2, 160, 16),
                                                (40, 1, 192, 64), (4, 4, 224, 16), (6, 3, 256, 128)])
-def test_attention_heads_and_lengths(ops, dtype, heads, hk, dim, page):
+def test_attention_heads_and_lengths(ops, dtype, heads, hk, dim, page, max_keys):
     """Every length around the borders of tiles and pages, a row that sees nothing, and rows that are none."""
     t = TYPES[dtype]
     lengths = [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 100, 127, 128, 129, 255, 257, 300]
     cache = Cache(t, lengths, hk, dim, page, seed=dim + heads)
     request = list(range(len(lengths))) + [-1, 3, -1]
     position = [n - 1 for n in lengths] + [5, -1, -1]
-    check_attention(ops, cache, rows_q(cache, len(request), heads, dim, t), request, position)
+    check_attention(ops, cache, rows_q(cache, len(request), heads, dim, t), request, position, max_keys=max_keys)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 160, 192, 224, 256])
+def test_attention_of_many_short_rows(ops, dtype, dim):
+    """So many units that a wave takes one by itself; every twelfth row against the oracle."""
+    t = TYPES[dtype]
+    rng = random.Random(dim)
+    lengths = [rng.randint(1, 32) for _ in range(540)]
+    cache = Cache(t, lengths, 1, dim, 16, seed=dim)
+    request = [s if s % 12 != 5 else -1 for s in range(540)]
+    position = [n - 1 for n in lengths]
+    q = rows_q(cache, 540, 3, dim, t)
+    out = torch.full((540, 3, dim), 4.0, dtype=t, device="cuda")
+    ops.paged_attention(q, cache.k_cache, cache.v_cache, cache.table, gpu_i32(request), gpu_i32(position), max_keys=32, out=out)
+    assert torch.isfinite(out).all()
+    for r in range(0, 540, 12):
+        ref, _, tol, _ = attend_by_hand(q[r], cache.k[r], cache.v[r], position[r], 1 / math.sqrt(dim), 0)
+        assert bool(((out[r].double().cpu() - ref).abs() <= tol).all()), r
+        assert bool((out[r + 5] == 4.0).all())
+    # the same rows in equal pieces and a block a unit: a wave's sums are in another order
+    for rows, keys in ((540, 10 ** 9), (500, 32)):
+        other = ops.paged_attention(q[:rows], cache.k_cache, cache.v_cache, cache.table, gpu_i32(request[:rows]), gpu_i32(position[:rows]), max_keys=keys)
+        for r in range(0, rows, 12):
+            ref, _, tol, _ = attend_by_hand(q[r], cache.k[r], cache.v[r], position[r], 1 / math.sqrt(dim), 0)
+            assert bool(((other[r].double().cpu() - ref).abs() <= tol).all()), r
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("heads,hk", [(3, 1), (16, 1), (8, 4)])
+def test_attention_of_one_long_row_among_short_ones(ops, dtype, heads, hk):
+    """A unit that reaches over most of the pieces beside units that share one."""
+    t = TYPES[dtype]
+    lengths = [5] * 20 + [30000] + [70] * 19
+    cache = Cache(t, lengths, hk, 64, 16, seed=heads)
+    check_attention(ops, cache, rows_q(cache, 40, heads, 64, t), list(range(40)), [n - 1 for n in lengths])
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
@@ -516,15 +553,16 @@ def test_attention_strides(ops, dtype):
         assert bool((buf[:, 0] == 8).all() and (buf[:, 5:] == 8).all() and (buf[..., :cut] == 8).all() and (buf[..., cut + 64:] == 8).all())
 
 
+@pytest.mark.parametrize("window,max_keys", [(30, None), (0, 10 ** 9)])
 @pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
-def test_attention_ignores_what_is_not_seen(ops, dtype):
+def test_attention_ignores_what_is_not_seen(ops, dtype, window, max_keys):
     """Infinities and NaN behind a row's position, before its window, in its page's unused cells and in other pages change no
     bit of it: also for a row whose neighbour of the same request does see them."""
     t = TYPES[dtype]
     cache = Cache(t, [90, 200], 2, 64, 16, seed=9, junk=0.0)
     q = rows_q(cache, 6, 8, 64, t)
     request, position = gpu_i32([0, 0, 0, 0, 1, 1]), gpu_i32([60, 61, 62, 89, 100, 199])
-    args = dict(table=cache.table, request=request, position=position, window=30)
+    args = dict(table=cache.table, request=request, position=position, window=window, max_keys=max_keys)
     clean = ops.paged_attention(q, cache.k_cache, cache.v_cache, **args)
     for junk in (float("nan"), float("inf"), -float("inf")):
         k, v = cache.k_cache.clone(), cache.v_cache.clone()
@@ -534,16 +572,17 @@ def test_attention_ignores_what_is_not_seen(ops, dtype):
                 k[pid, :, tok % 16] = junk
                 v[pid, :, tok % 16] = junk
         spoil(0, 62, 90)                       # seen by rows 2 and 3 alone
-        spoil(0, 0, 31)
-        spoil(1, 101, 170)
-        spoil(1, 0, 71)
+        if window:
+            spoil(0, 0, 31)
+            spoil(1, 101, 170)
+            spoil(1, 0, 71)
         used = set(cache.table.flatten().tolist())
         for pid in range(cache.pages):
             if pid not in used:
                 k[pid] = junk
                 v[pid] = junk
         got = ops.paged_attention(q, k, v, **args)
-        for r in (0, 1, 4, 5):
+        for r in (0, 1, 4, 5):                 # (row 5 sees 101 .. 170 without a window)
             assert torch.equal(got[r], clean[r]), (junk, r)
         assert bool((~torch.isfinite(got[2])).any())
 

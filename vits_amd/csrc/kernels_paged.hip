@@ -387,6 +387,8 @@ constexpr int ATT_THREADS = ATT_WAVES * WAVE;
 constexpr int ATT_COLS = 16;                 // columns of the products: (row of a run, query head)
 constexpr int ATT_PIECES = 2048;             // the most pieces a call's work is cut into: two waves a SIMD
 constexpr int ATT_MIN_STEPS = 2;             // the least a piece holds
+constexpr int ATT_FEW = 32;                  // units up to which a join takes a block a column
+constexpr int ATT_BLOCK_WAVES = 8;           // waves that take a unit by themselves
 constexpr float ATT_SLACK = 8.f;             // the running maximum follows once it is exceeded by 2^8: weights stay below 256
 
 // max and sum over the four lanes of a column (lane, lane ^ 16, lane ^ 32, lane ^ 48)
@@ -407,7 +409,9 @@ __device__ __forceinline__ float col_sum(float x) {
 // them beside each other), for each run its units (key-value head, 16 query heads of its group) one after the other, for
 // each unit the run's keys.  A run that sees no key has one step, in which everything is masked.
 struct AttPlan {
-  int rows_per_run;        // 16 / group, at least 1
+  int group;               // query heads of a key-value head
+  int per_page;            // 16-key parts of a page
+  int run_shift;           // rows_per_run = 1 << run_shift: a power of two, at most 16 / group (and at least 1)
   int tiles;               // 16-column tiles of a group
   int units;               // kv_heads * tiles
   int pieces;              // waves that the line is cut for (split form), a multiple of ATT_WAVES
@@ -435,13 +439,13 @@ __device__ __forceinline__ bool att_run(const PagedAttArgs& a, const AttPlan& p,
   int end;
   att_row_keys(a, row, r.from, end);                     // loaded beside the requests, not after them
   if (req < 0 || req >= a.requests) return false;
-  const int in = row % p.rows_per_run;
+  const int in = row & ((1 << p.run_shift) - 1);
   if (in > 0 && before == req) return false;
   r.row = row;
   r.req = req;
   r.begin = r.from < end ? r.from : 0x7fffffff;
   r.end = end;
-  const int most = min(p.rows_per_run - in, a.rows - row);
+  const int most = min((1 << p.run_shift) - in, a.rows - row);
   int n = 1;
   for (; n < most && a.row_request[row + n] == req; ++n) {
     int b, e;
@@ -452,6 +456,11 @@ __device__ __forceinline__ bool att_run(const PagedAttArgs& a, const AttPlan& p,
   r.n = n;
   r.begin = r.begin >= r.end ? 0 : r.begin & ~15;
   return true;
+}
+
+// x / y of numbers that are not negative: 64-bit division is a long routine, and these are seldom that large
+__device__ __forceinline__ long long att_div(long long x, long long y) {
+  return (x | y) >> 32 ? x / y : (long long)((unsigned)x / (unsigned)y);
 }
 
 template <int STEP>
@@ -482,6 +491,9 @@ __device__ __forceinline__ bool att_column(int m, int n, int group, int tile, in
 
 __device__ __forceinline__ float att_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// keys of a step
+__host__ __device__ constexpr int att_step(int size, int dim) { return size == 2 && dim <= 192 ? 32 : 16; }
+
 // A result of a matrix instruction is bound to a wait here, in the block that computes it: read in another block, behind a
 // taken branch, the compiler (ROCm 7.2) has been seen to leave it too short (needed: up to 11 issue slots).
 #define ATT_SETTLE(x) asm volatile("s_nop 15" : "+v"(x))
@@ -491,9 +503,9 @@ struct AttTile {
   static constexpr bool HALF = sizeof(T) == 2;
   // Registers: Q, K, V and O of a step have to fit 256 (two waves a SIMD) with room for the rest.  So wide heads take 16
   // keys a step, and fp32 ones load K and V in two passes, the second when the first has been used.
-  static constexpr int SUB = HALF && DIM <= 192 ? 2 : 1;  // 16-key parts of a step
+  static constexpr int STEP = att_step(sizeof(T), DIM);
+  static constexpr int SUB = STEP / 16;                  // 16-key parts of a step
   static constexpr int PASSES = !HALF && DIM > 160 ? 2 : 1;
-  static constexpr int STEP = 16 * SUB;
   static constexpr int KL = DIM * (int)sizeof(T) / 64;   // 16-byte loads of a lane for 16 keys
   static constexpr int KP = KL / PASSES;
   static constexpr int CH = DIM / 16;                   // channels of a lane in V and in the output
@@ -721,7 +733,7 @@ __device__ __forceinline__ bool att_part(const PagedAttArgs& a, const AttPlan& p
   constexpr int SUB = Tile::SUB, STEP = Tile::STEP, KL = Tile::KL, CH = Tile::CH, PASSES = Tile::PASSES;
   const int lane = threadIdx.x & (WAVE - 1);
   const int col = lane & 15, lg = lane >> 4;
-  const int group = a.heads / a.kv_heads, hk = unit / p.tiles, tile = unit - hk * p.tiles;
+  const int group = p.group, hk = p.tiles == 1 ? unit : unit / p.tiles, tile = unit - hk * p.tiles;
   Tile w;
   int my_row, my_head;
   const bool real = att_column(col, r.n, group, tile, my_row, my_head);
@@ -738,7 +750,6 @@ __device__ __forceinline__ bool att_part(const PagedAttArgs& a, const AttPlan& p
 
   // Where the 16-key parts of the next 64 / SUB steps lie, one part a lane: elements from the cache's beginning
   // (16 keys never straddle a page), 0 and a bit in `out` for a part that no row sees or whose page is none.
-  const int per_page = a.page_size / 16;
   const int* table = a.table + (long long)r.req * a.table_stride;
   const long long head_off = (long long)hk * a.page_size * DIM;
   long long at = 0;
@@ -747,12 +758,12 @@ __device__ __forceinline__ bool att_part(const PagedAttArgs& a, const AttPlan& p
     const int t = first + lane / SUB;
     const int key = r.begin + t * STEP + 16 * (lane % SUB);
     const bool seen = t < t1 && key < r.end;
-    const int part = (seen ? key : r.begin) / 16, page = part / per_page;
+    const int part = (seen ? key : r.begin) / 16, page = part / p.per_page;
     const int id = table[page];
     const bool there = id >= 0 && id < a.pages;
     stray |= __ballot(seen && !there);
     out = __ballot(!seen || !there);
-    at = seen && there ? (long long)id * a.page_stride + head_off + (long long)(part - page * per_page) * 16 * DIM : 0;
+    at = seen && there ? (long long)id * a.page_stride + head_off + (long long)(part - page * p.per_page) * 16 * DIM : 0;
   };
   auto part_at = [&](int i) -> long long {               // the part that lane i has located, the same for the wave
     const unsigned lo = __builtin_amdgcn_readlane((unsigned)at, i), hi = __builtin_amdgcn_readlane((unsigned)(at >> 32), i);
@@ -887,16 +898,84 @@ __device__ __forceinline__ void att_flag_row(const PagedAttArgs& a, int row) {
   if (a.err_flag && (req >= a.requests || (req >= 0 && att_row_keys(a, row, b, e)))) atomicOr(a.err_flag, 1);
 }
 
-// A wave a unit: for lengths that a wave takes in a short time, and for so many units that their lengths even out.
+// Joins a block's parts of one unit, N of them in LDS (those that are none have a null pointer), a thread a quad of channels.
+// slot: where the joined part goes; null: it is the whole unit and the result is written.
+template <typename T, int DIM, int N, int THREADS>
+__device__ __forceinline__ void att_join(const PagedAttArgs& a, const AttPlan& p, int row0, int n_rows, int unit, int begin, int end,
+                                         const float* const (&part)[N], const float* any, float* slot) {
+  constexpr int ROW = DIM + 4, QUADS = DIM / 4;
+  const int hk = p.tiles == 1 ? unit : unit / p.tiles, tile = unit - hk * p.tiles;
+#pragma unroll
+  for (int i0 = 0; i0 < ATT_COLS * QUADS; i0 += THREADS) {
+    const int i = i0 + (int)threadIdx.x, m = i / QUADS, c = i % QUADS * 4;
+    int row, head;
+    if (i >= ATT_COLS * QUADS || !att_column(m, n_rows, p.group, tile, row, head)) continue;
+    float tops[N], sums[N];
+    f32x4 xs[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {                        // all loads at once: what is no part is read from one and has no weight
+      const float* from = (part[j] ? part[j] : any) + m * ROW;
+      tops[j] = from[DIM];
+      sums[j] = from[DIM + 1];
+      xs[j] = *(const f32x4*)(from + c);
+    }
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) top = part[j] ? fmaxf(top, tops[j]) : top;
+    const float base = top == -INFINITY ? 0.f : top;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (part[j]) {
+        const float f = att_exp2(tops[j] - base);
+        sum += f * sums[j];
+        x += f * xs[j];
+      }
+    if (slot) {
+      *(f32x4*)(slot + m * ROW + c) = x;
+      if (c == 0) {
+        slot[m * ROW + DIM] = top;
+        slot[m * ROW + DIM + 1] = sum;
+      }
+      continue;
+    }
+    int from = begin, to = end;
+    if (n_rows > 1) att_row_keys(a, row0 + row, from, to);
+    att_write<T>(a, p.wide_out, row0 + row, hk * p.group + head, c, x, sum, from >= to);
+    if (a.lse && c == 0) att_write_lse(a, row0 + row, hk * p.group + head, top, sum, from >= to);
+  }
+}
+
+// A wave a unit: for so many units that they fill the chip, of lengths that a wave takes in a short time.  No workspace, no
+// second launch.
 template <typename T, int DIM>
-__global__ __launch_bounds__(ATT_THREADS, 2) void paged_attention_kernel(PagedAttArgs a, AttPlan p) {
+__global__ __launch_bounds__(ATT_THREADS, 2) void paged_attention_wave_kernel(PagedAttArgs a, AttPlan p) {
   const long long n = (long long)blockIdx.x * ATT_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-  const int row = (int)(n / p.units), unit = (int)(n - (long long)row * p.units);
+  const int row = (int)att_div(n, p.units), unit = (int)(n - (long long)row * p.units);
   if (row >= a.rows) return;
   if (unit == 0 && threadIdx.x % WAVE == 0) att_flag_row(a, row);
   Run r;
   if (att_run(a, p, row, r) && att_part<T, DIM>(a, p, r, unit, 0, att_run_steps<AttTile<T, DIM>::STEP>(r), true, nullptr) && a.err_flag)
     atomicOr(a.err_flag, 1);
+}
+
+// A block a unit, its waves a stretch of the keys each, joined in LDS: for fewer units of such lengths.
+template <typename T, int DIM>
+__global__ __launch_bounds__(ATT_BLOCK_WAVES * WAVE, 1) void paged_attention_block_kernel(PagedAttArgs a, AttPlan p) {
+  __shared__ alignas(16) float lds[ATT_BLOCK_WAVES][ATT_COLS * AttTile<T, DIM>::ROW];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int row = blockIdx.x / p.units, unit = blockIdx.x - row * p.units;
+  if (unit == 0 && threadIdx.x == 0) att_flag_row(a, row);
+  Run r;
+  if (!att_run(a, p, row, r)) return;
+  const int steps = att_run_steps<AttTile<T, DIM>::STEP>(r);
+  const int each = (steps + ATT_BLOCK_WAVES - 1) / ATT_BLOCK_WAVES, t0 = wave * each, t1 = min(t0 + each, steps);
+  if (t0 < t1 && att_part<T, DIM>(a, p, r, unit, t0, t1, false, lds[wave]) && a.err_flag) atomicOr(a.err_flag, 1);
+  __syncthreads();
+  const float* part[ATT_BLOCK_WAVES];
+#pragma unroll
+  for (int w = 0; w < ATT_BLOCK_WAVES; ++w) part[w] = w * each < steps ? lds[w] : nullptr;
+  att_join<T, DIM, ATT_BLOCK_WAVES, ATT_BLOCK_WAVES * WAVE>(a, p, r.row, r.n, unit, r.from, r.end, part, lds[0], nullptr);
 }
 
 // The line of work cut into p.pieces equal pieces, a wave a piece, a block four that follow each other: a long row beside
@@ -939,7 +1018,7 @@ __global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attenti
     total += wave_sum[w];
   }
   total *= p.units;
-  long long size = (total + p.pieces - 1) / p.pieces;
+  long long size = att_div(total + p.pieces - 1, p.pieces);
   if (size < ATT_MIN_STEPS) size = ATT_MIN_STEPS;
   if (tid == 0) joins[blockIdx.x].parts = 0;
   if (blockIdx.x * ATT_WAVES * size >= total) return;      // the whole block
@@ -972,13 +1051,13 @@ __global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attenti
     bool stray = false;
     for (;;) {
       const int steps = att_run_steps<STEP>(r);
-      for (int unit = (int)((pos - run_at) / steps); unit < p.units && pos < last; ++unit) {
+      for (int unit = (int)att_div(pos - run_at, steps); unit < p.units && pos < last; ++unit) {
         const long long unit_at = run_at + (long long)unit * steps;
         const int t0 = (int)(pos - unit_at), t1 = (int)(last - unit_at < steps ? last - unit_at : steps);
         const bool whole = t0 == 0 && t1 == steps;
         if (!whole && lane == 0)
           left[wave][t0 == 0] = Part{1, r.row, r.n, unit, r.from, r.end,
-                                     t0 == 0 ? (int)((unit_at + steps - 1) / (size * ATT_WAVES)) - (int)blockIdx.x : t1 < steps};
+                                     t0 == 0 ? (int)att_div(unit_at + steps - 1, size * ATT_WAVES) - (int)blockIdx.x : t1 < steps};
         stray |= att_part<T, DIM>(a, p, r, unit, t0, t1, whole, lds[wave][t0 == 0]);
         pos = unit_at + t1;
       }
@@ -992,160 +1071,158 @@ __global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attenti
 
   // A chain: what the block holds of one unit, beginning with a wave's [1], or (k == 0) with what an earlier block began,
   // and going on in the [0] of the waves behind
-  const int group = a.heads / a.kv_heads;
+  bool live[ATT_WAVES][2], more[ATT_WAVES];
+#pragma unroll
+  for (int w = 0; w < ATT_WAVES; ++w) {
+    live[w][0] = left[w][0].live;
+    live[w][1] = left[w][1].live;
+    more[w] = left[w][0].more;
+  }
+#pragma unroll
   for (int k = 0; k <= ATT_WAVES; ++k) {
+    if (!(k == 0 ? live[0][0] : live[k - 1][1])) continue;
     const Part head = k == 0 ? left[0][0] : left[k - 1][1];
-    if (!head.live) continue;
-    int w1 = k == 0 ? 1 : k;                              // one past the last wave with a [0] of the chain
-    bool ends = k == 0 ? !left[0][0].more : false;
-    while (!ends && w1 < ATT_WAVES) ends = !left[w1++][0].more;
-    const bool whole = ends && k > 0;
-    if (k > 0 && !ends && tid == 0) joins[blockIdx.x] = AttJoin{head.row, head.n, head.unit, head.more};
-    float* slot = att_slot(ws, blockIdx.x, k > 0, DIM);
-    const int hk = head.unit / p.tiles, tile = head.unit - hk * p.tiles;
-    for (int i = tid; i < ATT_COLS * (DIM / 4); i += ATT_THREADS) {
-      const int m = i / (DIM / 4), c = i % (DIM / 4) * 4;
-      int row, hd;
-      if (!att_column(m, head.n, group, tile, row, hd)) continue;
-      // the chain's parts lie at most ATT_WAVES + 1 in a row: [1] of wave k - 1, [0] of waves k .. w1 - 1
-      float tops[ATT_WAVES + 1], sums[ATT_WAVES + 1];
-      f32x4 xs[ATT_WAVES + 1];
+    const float* part[ATT_WAVES + 1];
+    part[0] = k > 0 ? lds[k - 1][1] : nullptr;
+    bool goes_on = true;
 #pragma unroll
-      for (int j = 0; j <= ATT_WAVES; ++j) {
-        const bool there = j == 0 ? k > 0 : j > k && j <= w1;
-        const float* part = lds[j == 0 ? (there ? k - 1 : 0) : j - 1][j == 0] + m * ROW;
-        tops[j] = there ? part[DIM] : -INFINITY;
-        sums[j] = there ? part[DIM + 1] : 0.f;
-        xs[j] = *(const f32x4*)(part + c);                 // of no weight where there is no part
-        if (!there) xs[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
-      float top = tops[0], sum = 0.f;
-#pragma unroll
-      for (int j = 1; j <= ATT_WAVES; ++j) top = fmaxf(top, tops[j]);
-      const float base = top == -INFINITY ? 0.f : top;
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j <= ATT_WAVES; ++j) {
-        const float f = att_exp2(tops[j] - base);
-        sum += f * sums[j];
-        x += f * xs[j];
-      }
-      if (!whole) {
-        *(f32x4*)(slot + m * ROW + c) = x;
-        if (c == 0) {
-          slot[m * ROW + DIM] = top;
-          slot[m * ROW + DIM + 1] = sum;
-        }
-        continue;
-      }
-      int from = head.from, to = head.to;
-      if (head.n > 1) att_row_keys(a, head.row + row, from, to);
-      att_write<T>(a, p.wide_out, head.row + row, hk * group + hd, c, x, sum, from >= to);
-      if (a.lse && c == 0) att_write_lse(a, head.row + row, hk * group + hd, top, sum, from >= to);
+    for (int w = 0; w < ATT_WAVES; ++w) {
+      part[w + 1] = w >= k && goes_on ? lds[w][0] : nullptr;
+      if (w >= k) goes_on = goes_on && more[w];
     }
+    if (k > 0 && goes_on && tid == 0) joins[blockIdx.x] = AttJoin{head.row, head.n, head.unit, head.more};
+    att_join<T, DIM, ATT_WAVES + 1, ATT_THREADS>(a, p, head.row, head.n, head.unit, head.from, head.to, part, k == 0 ? lds[0][0] : lds[k - 1][1],
+                     k > 0 && !goes_on ? nullptr : att_slot(ws, blockIdx.x, k > 0, DIM));
   }
 }
 
-// Joins the parts of the unit that begins in block blockIdx.x and ends in a later one, a block a column: dim / 4 threads hold a
-// part, the block as many parts as that leaves threads for, each its parts in the order of the keys, so that the result
-// does not depend on which block was done first.
+// Joins the parts of the unit that begins in block blockIdx.x of the split and ends in a later one, `cols` columns a block: four,
+// a wave each, where there are many units and so, as a rule, few parts of each (where one has many after all, the block takes
+// them one after the other); one, where few units have many parts (one row over a long context).  dim / 4 threads hold a part, the team as many parts as that leaves threads for and eight times that in
+// flight, each its parts in the order of the keys, so that the result does not depend on which block was done first.
+constexpr int JOIN_FEW = 16;
 template <typename T>
-__global__ __launch_bounds__(ATT_THREADS) void paged_join_kernel(PagedAttArgs a, AttPlan p, float* ws, const AttJoin* joins) {
+__global__ __launch_bounds__(ATT_THREADS) void paged_join_kernel(PagedAttArgs a, AttPlan p, float* ws, const AttJoin* joins, int cols) {
+  constexpr int AHEAD = 8;
   __shared__ f32x4 acc[ATT_THREADS];
   __shared__ float wave_sum[ATT_WAVES];
   const AttJoin j = joins[blockIdx.x];
-  const int group = a.heads / a.kv_heads, ROW = a.dim + 4, parts = j.parts + 1, m = blockIdx.y, hk = j.unit / p.tiles;
-  int row, head;
-  if (parts == 1 || !att_column(m, j.n, group, j.unit - hk * p.tiles, row, head)) return;
-  const int tid = threadIdx.x, lane = tid & (WAVE - 1);
-  const int quads = a.dim / 4, at_once = ATT_THREADS / quads, mine = tid / quads, quad = tid - mine * quads;
-  int from, to;
-  att_row_keys(a, j.row + row, from, to);
-  auto part = [&](int i) { return att_slot(ws, blockIdx.x + i, i == 0, a.dim) + m * ROW; };
-  constexpr int AHEAD = 4;                                 // loads in flight a thread
-  f32x4 v[AHEAD];
-  auto load = [&](int i0) {                                // what there is not is read from the last part, and has no weight
+  const int parts = j.parts + 1, wave = threadIdx.x / WAVE;
+  if (parts == 1) return;
+  const int ROW = a.dim + 4, quads = a.dim / 4, hk = p.tiles == 1 ? j.unit : j.unit / p.tiles;
+  const bool few = parts <= JOIN_FEW && cols == ATT_WAVES;
+  const int team = few ? WAVE : ATT_THREADS, me = few ? threadIdx.x % WAVE : threadIdx.x;
+  const int at_once = team / quads, mine = me / quads, quad = me - mine * quads;
+  for (int i = 0; i < (few ? 1 : cols); ++i) {
+    const int m = blockIdx.y * cols + (few ? wave : i);
+    int row, head;
+    const bool real = att_column(m, j.n, p.group, j.unit - hk * p.tiles, row, head);
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    float top = -INFINITY, base = 0.f, sum = 0.f;
+    if (real) {
+      auto part = [&](int k) { return att_slot(ws, blockIdx.x + k, k == 0, a.dim) + m * ROW; };
+      f32x4 v[AHEAD];
+      auto load = [&](int k0) {                            // what there is not is read from the last part, and has no weight
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) v[u] = *(const f32x4*)(part(min(i0 + u * at_once + mine, parts - 1)) + 4 * quad);
-  };
-  load(0);
-  float top = -INFINITY, sum = 0.f;
-  for (int i = lane; i < parts; i += WAVE) top = fmaxf(top, part(i)[a.dim]);
+        for (int u = 0; u < AHEAD; ++u) v[u] = *(const f32x4*)(part(min(k0 + u * at_once + mine, parts - 1)) + 4 * quad);
+      };
+      load(0);
+      for (int k = me % WAVE; k < parts; k += WAVE) top = fmaxf(top, part(k)[a.dim]);
 #pragma unroll
-  for (int d = 1; d < WAVE; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, WAVE));
-  const float base = top == -INFINITY ? 0.f : top;
-  f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  float f = 0.f;
-  const int batch = AHEAD * at_once;                       // parts that the block has in flight
-  for (int i = 0; i < parts; i += batch) {                 // the same trips for every lane: all of them hold weights
-    if (i > 0) load(i);
+      for (int d = 1; d < WAVE; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, WAVE));
+      base = top == -INFINITY ? 0.f : top;
+      for (int k0 = 0; k0 < parts; k0 += AHEAD * at_once) {
+        if (k0 > 0) load(k0);
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const int k = i + u * at_once + mine;
-      const bool there = mine < at_once && k < parts;
-      const float g = there ? att_exp2(part(k)[a.dim] - base) : 0.f;
-      if (there && quad == 0) f += g * part(k)[a.dim + 1];
-      if (there) x += g * v[u];
+        for (int u = 0; u < AHEAD; ++u) {
+          const int k = k0 + u * at_once + mine;
+          if (mine < at_once && k < parts) {
+            const float g = att_exp2(part(k)[a.dim] - base);
+            if (quad == 0) sum += g * part(k)[a.dim + 1];
+            x += g * v[u];
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 1; d < WAVE; d <<= 1) sum += __shfl_xor(sum, d, WAVE);
     }
+    if (threadIdx.x % WAVE == 0) wave_sum[wave] = sum;
+    acc[threadIdx.x] = x;
+    __syncthreads();
+    if (real && mine == 0) {
+      const f32x4* other = acc + (few ? wave * WAVE : 0) + quad;
+      for (int k = 1; k < at_once; ++k) x += other[k * quads];
+      if (!few) {
+        sum = 0.f;
+        for (int w = 0; w < ATT_WAVES; ++w) sum += wave_sum[w];
+      }
+      int from, to;
+      att_row_keys(a, j.row + row, from, to);
+      att_write<T>(a, p.wide_out, j.row + row, hk * p.group + head, 4 * quad, x, sum, from >= to);
+      if (a.lse && quad == 0) att_write_lse(a, j.row + row, hk * p.group + head, top, sum, from >= to);
+    }
+    if (!few) __syncthreads();                             // before the LDS is written again
   }
-  sum = f;
-#pragma unroll
-  for (int d = 1; d < WAVE; d <<= 1) sum += __shfl_xor(sum, d, WAVE);
-  if (lane == 0) wave_sum[tid / WAVE] = sum;
-  acc[tid] = x;
-  __syncthreads();
-  sum = 0.f;
-  for (int i = 0; i < ATT_WAVES; ++i) sum += wave_sum[i];
-  if (mine == 0) {
-    for (int i = 1; i < at_once; ++i) x += acc[i * quads + quad];
-    att_write<T>(a, p.wide_out, j.row + row, hk * group + head, 4 * quad, x, sum, from >= to);
-  }
-  if (a.lse && tid == 0) att_write_lse(a, j.row + row, hk * group + head, top, sum, from >= to);
 }
 
-AttPlan att_plan(int rows, int heads, int kv_heads, long long max_keys, bool& split) {
-  const int group = heads / kv_heads;
-  AttPlan p;
-  p.rows_per_run = group <= ATT_COLS ? ATT_COLS / group : 1;
-  p.tiles = (group + ATT_COLS - 1) / ATT_COLS;
+// How a call's work is shared out: a wave a unit, a block a unit, or equal pieces of the line.  By the number of units and
+// the steps of the longest one as far as the host knows; microseconds of the three on requests of 1/16 to all of that length
+// (8 key-value heads of 128 in bf16: 8 units a row, 32 keys a step):
+//   rows x steps     1 x 32         4 x 63         16 x 63        16 x 125         64 x 2          64 x 125        256 x 16       256 x 32
+//   wave/block/split 44 / 14 / 16   86 / 24 / 21   87 / 25 / 31   178 / 51 / 40    8.7 / 11 / 18   192 / 125 / 126  71 / 79 / 83   125 / 117 / 128
+// A block's waves take the longest unit's steps by eights at 1.3 us each, whatever else there is to do; the pieces even that out
+// for about 10 us more (their sums at the start, the join, its launch).
+enum AttForm { ATT_WAVE, ATT_BLOCK, ATT_SPLIT };
+
+AttPlan att_plan(int rows, int heads, int kv_heads, int dim, int dtype, long long max_keys, AttForm& form) {
+  AttPlan p{};
+  p.group = heads / kv_heads;
+  p.run_shift = p.group <= 1 ? 4 : p.group <= 2 ? 3 : p.group <= 4 ? 2 : p.group <= 8 ? 1 : 0;
+  p.tiles = (p.group + ATT_COLS - 1) / ATT_COLS;
   p.units = kv_heads * p.tiles;
   p.pieces = ATT_PIECES;
-  p.wide_out = 0;
-  const long long units = (long long)rows * p.units;
-  if (max_keys > 0 && max_keys < (1 << 30)) {            // no more pieces than their least size fills, in steps of 16 keys
-    const long long most = units * ((max_keys + 15) / 16 + 1) / ATT_MIN_STEPS + 1;
+  if (max_keys <= 0 || max_keys > (1 << 30)) max_keys = 1 << 30;
+  const int step = att_step(dtype == VITS_TYPE_F32 ? 4 : 2, dim);
+  const long long units = (long long)rows * p.units, steps = (max_keys + step - 1) / step;
+  if (units >= 2048 ? steps <= 16 : units >= 512 && steps <= 2) form = ATT_WAVE;
+  else if (steps <= (units >= 512 ? 128 : units >= 128 ? 64 : 32)) form = ATT_BLOCK;
+  else form = ATT_SPLIT;
+  if (units > 1 << 21) form = ATT_SPLIT;                   // more blocks than a grid of the other forms should have
+  if (steps < (1 << 20)) {                                 // no more pieces than their least size fills
+    const long long most = units * (steps + 1) / ATT_MIN_STEPS + 1;
     if (most < p.pieces) p.pieces = (int)(most + ATT_WAVES - 1) / ATT_WAVES * ATT_WAVES;
   }
-  split = max_keys <= 0 || max_keys > 64 || units > 1 << 22;
   return p;
 }
 
 template <typename T, int DIM>
-hipError_t start_attention(const PagedAttArgs& a, const AttPlan& p, bool split, void* ws, hipStream_t s) {
-  if (!split) {
-    const long long units = (long long)a.rows * p.units;
-    hipLaunchKernelGGL((paged_attention_kernel<T, DIM>), dim3((unsigned)((units + ATT_WAVES - 1) / ATT_WAVES)), dim3(ATT_THREADS), 0, s, a, p);
-    return hipGetLastError();
+hipError_t start_attention(const PagedAttArgs& a, const AttPlan& p, AttForm form, void* ws, hipStream_t s) {
+  const unsigned units = (unsigned)a.rows * p.units;
+  if (form == ATT_WAVE) {
+    hipLaunchKernelGGL((paged_attention_wave_kernel<T, DIM>), dim3((units + ATT_WAVES - 1) / ATT_WAVES), dim3(ATT_THREADS), 0, s, a, p);
+  } else if (form == ATT_BLOCK) {
+    hipLaunchKernelGGL((paged_attention_block_kernel<T, DIM>), dim3(units), dim3(ATT_BLOCK_WAVES * WAVE), 0, s, a, p);
+  } else {
+    const int blocks = p.pieces / ATT_WAVES;
+    AttJoin* joins = (AttJoin*)att_slot((float*)ws, blocks, 0, DIM);
+    hipLaunchKernelGGL((paged_attention_split_kernel<T, DIM>), dim3(blocks), dim3(ATT_THREADS), 0, s, a, p, (float*)ws, joins);
+    const int cols = min(ATT_COLS, p.group << p.run_shift), each = units > ATT_FEW ? ATT_WAVES : 1;
+    hipLaunchKernelGGL((paged_join_kernel<T>), dim3(blocks, (cols + each - 1) / each), dim3(ATT_THREADS), 0, s, a, p, (float*)ws, joins, each);
   }
-  const int blocks = p.pieces / ATT_WAVES;
-  AttJoin* joins = (AttJoin*)att_slot((float*)ws, blocks, 0, DIM);
-  hipLaunchKernelGGL((paged_attention_split_kernel<T, DIM>), dim3(blocks), dim3(ATT_THREADS), 0, s, a, p, (float*)ws, joins);
-  const int cols = min(ATT_COLS, a.heads / a.kv_heads * p.rows_per_run);
-  hipLaunchKernelGGL((paged_join_kernel<T>), dim3(blocks, cols), dim3(ATT_THREADS), 0, s, a, p, (float*)ws, joins);
   return hipGetLastError();
 }
 
 template <typename T>
-hipError_t start_attention_t(const PagedAttArgs& a, const AttPlan& p, bool split, void* ws, hipStream_t s) {
+hipError_t start_attention_t(const PagedAttArgs& a, const AttPlan& p, AttForm form, void* ws, hipStream_t s) {
   switch (a.dim) {
-    case 32: return start_attention<T, 32>(a, p, split, ws, s);
-    case 64: return start_attention<T, 64>(a, p, split, ws, s);
-    case 96: return start_attention<T, 96>(a, p, split, ws, s);
-    case 128: return start_attention<T, 128>(a, p, split, ws, s);
-    case 160: return start_attention<T, 160>(a, p, split, ws, s);
-    case 192: return start_attention<T, 192>(a, p, split, ws, s);
-    case 224: return start_attention<T, 224>(a, p, split, ws, s);
-    case 256: return start_attention<T, 256>(a, p, split, ws, s);
+    case 32: return start_attention<T, 32>(a, p, form, ws, s);
+    case 64: return start_attention<T, 64>(a, p, form, ws, s);
+    case 96: return start_attention<T, 96>(a, p, form, ws, s);
+    case 128: return start_attention<T, 128>(a, p, form, ws, s);
+    case 160: return start_attention<T, 160>(a, p, form, ws, s);
+    case 192: return start_attention<T, 192>(a, p, form, ws, s);
+    case 224: return start_attention<T, 224>(a, p, form, ws, s);
+    case 256: return start_attention<T, 256>(a, p, form, ws, s);
   }
   return hipErrorInvalidValue;
 }
@@ -1163,19 +1240,20 @@ hipError_t launch_rotary_store(const RotaryArgs& a, hipStream_t s) {
   return a.dtype == VITS_TYPE_F16 ? start_rotary_t<_Float16>(a, s) : start_rotary_t<__bf16>(a, s);
 }
 
-int64_t paged_attention_workspace(int rows, int heads, int kv_heads, int dim, long long max_keys) {
-  bool split;
-  const AttPlan p = att_plan(rows, heads, kv_heads, max_keys, split);
-  return split ? (int64_t)(p.pieces / ATT_WAVES) * (2 * ATT_COLS * (dim + 4) * sizeof(float) + sizeof(AttJoin)) : 0;
+int64_t paged_attention_workspace(int rows, int heads, int kv_heads, int dim, int dtype, long long max_keys) {
+  AttForm form;
+  const AttPlan p = att_plan(rows, heads, kv_heads, dim, dtype, max_keys, form);
+  return form == ATT_SPLIT ? (int64_t)(p.pieces / ATT_WAVES) * (2 * ATT_COLS * (dim + 4) * sizeof(float) + sizeof(AttJoin)) : 0;
 }
 
 hipError_t launch_paged_attention(const PagedAttArgs& a, long long max_keys, void* ws, hipStream_t s) {
-  bool split;
-  AttPlan p = att_plan(a.rows, a.heads, a.kv_heads, max_keys, split);
+  AttForm form;
+  AttPlan p = att_plan(a.rows, a.heads, a.kv_heads, a.dim, a.dtype, max_keys, form);
   const int size = a.dtype == VITS_TYPE_F32 ? 4 : 2;
+  p.per_page = a.page_size / 16;
   p.wide_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_row * size % 16 == 0 && a.out_head * size % 16 == 0;
-  if (a.dtype == VITS_TYPE_F32) return start_attention_t<float>(a, p, split, ws, s);
-  return a.dtype == VITS_TYPE_F16 ? start_attention_t<_Float16>(a, p, split, ws, s) : start_attention_t<__bf16>(a, p, split, ws, s);
+  if (a.dtype == VITS_TYPE_F32) return start_attention_t<float>(a, p, form, ws, s);
+  return a.dtype == VITS_TYPE_F16 ? start_attention_t<_Float16>(a, p, form, ws, s) : start_attention_t<__bf16>(a, p, form, ws, s);
 }
 
 }  // namespace vits

@@ -362,7 +362,9 @@ int check_page_size(int page_size) {
   return VITS_OK;
 }
 
-int check_att_shape(int rows, int heads, int kv_heads, int dim) {
+int check_att_shape(int rows, int heads, int kv_heads, int dim, int dtype) {
+  if (dtype < VITS_TYPE_F32 || dtype > VITS_TYPE_BF16)
+    return fail(VITS_ERR_INVALID, "paged attention: dtype must be fp32 (0), fp16 (1) or bf16 (2)");
   if (rows < 0 || rows > PAGED_MAX_ROWS || kv_heads < 1 || heads < 1 || heads > PAGED_MAX_HEADS || heads % kv_heads || dim < 32 || dim > PAGED_MAX_DIM || dim % 32)
     return fail(VITS_ERR_INVALID, "paged attention: at most 2^23 rows, 1 to 1024 query heads in equal groups over the key-value heads, and heads of "
                                   "32, 64, ... 256 channels required");
@@ -1523,9 +1525,9 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
   return VITS_OK;
 }
 
-int64_t vits_op_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int dim, int64_t max_keys) {
-  if (check_att_shape(rows, heads, kv_heads, dim) != VITS_OK) return -1;
-  return paged_attention_workspace(rows, heads, kv_heads, dim, max_keys);
+int64_t vits_op_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int dim, int dtype, int64_t max_keys) {
+  if (check_att_shape(rows, heads, kv_heads, dim, dtype) != VITS_OK) return -1;
+  return paged_attention_workspace(rows, heads, kv_heads, dim, dtype, max_keys);
 }
 
 int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, const void* v_cache,
@@ -1535,9 +1537,7 @@ int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const 
                             int64_t out_head, float* lse, int* err_flag, void* ws, int64_t ws_bytes, void* stream) {
   if (rows != 0 && (!q || !k_cache || !v_cache || !table || !row_request || !row_position || !out))
     return fail(VITS_ERR_INVALID, "paged attention: null argument");
-  if (dtype < VITS_TYPE_F32 || dtype > VITS_TYPE_BF16)
-    return fail(VITS_ERR_INVALID, "paged attention: dtype must be fp32 (0), fp16 (1) or bf16 (2)");
-  TRY(check_att_shape(rows, heads, kv_heads, dim));
+  TRY(check_att_shape(rows, heads, kv_heads, dim, dtype));
   TRY(check_page_size(page_size));
   if (pages < 1 || width < 1 || table_stride < width || (int64_t)width * page_size > (1 << 30) || requests < 1 || window < 0)
     return fail(VITS_ERR_INVALID, "paged attention: at least one page, request and table column, a table of at most 2^30 tokens a "
@@ -1548,7 +1548,7 @@ int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const 
     return fail(VITS_ERR_INVALID, "paged attention: cannot run in place");
   if ((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)q) & 15) || (page_stride * size) % 16 || (q_row * size) % 16 || (q_head * size) % 16)
     return fail(VITS_ERR_INVALID, "paged attention: the caches, their pages and the heads of q must begin on 16-byte addresses");
-  if (ws_bytes < paged_attention_workspace(rows, heads, kv_heads, dim, max_keys) || (ws_bytes > 0 && !ws) || ((uintptr_t)ws & 15))
+  if (ws_bytes < paged_attention_workspace(rows, heads, kv_heads, dim, dtype, max_keys) || (ws_bytes > 0 && !ws) || ((uintptr_t)ws & 15))
     return fail(VITS_ERR_WORKSPACE, "paged attention: workspace too small or not on a 16-byte address");
   if (rows == 0) return VITS_OK;
   PagedAttArgs a{};

@@ -228,8 +228,8 @@ def rotary_store(q: Optional[torch.Tensor], k: Optional[torch.Tensor], v: Option
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_bytes(rows: int, heads: int, kv_heads: int, dim: int, max_keys: int) -> int:
-    n = N.lib.vits_op_paged_attention_workspace_bytes(rows, heads, kv_heads, dim, max_keys)
+def _workspace_bytes(rows: int, heads: int, kv_heads: int, dim: int, dtype: int, max_keys: int) -> int:
+    n = N.lib.vits_op_paged_attention_workspace_bytes(rows, heads, kv_heads, dim, dtype, max_keys)
     if n < 0:
         N.check(-1, "paged_attention")
     return n
@@ -268,12 +268,15 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         q_row, q_head, _ = q.stride()
     requests, width = table.shape
     keys = width * page_size if max_keys is None else max_keys
-    nbytes = _workspace_bytes(rows, heads, kv_heads, dim, keys)
+    if 0 < window < keys:
+        keys = window
+    dtype = _TYPES[q.dtype]
+    nbytes = _workspace_bytes(rows, heads, kv_heads, dim, dtype, keys)
     # a workspace of this call's own: calls on different streams, and graphs that run side by side, share none
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     out_row, out_head, _ = out.stride()
     _call(what, index, N.lib.vits_op_paged_attention, q.data_ptr(), q_row, q_head, k_cache.data_ptr(), v_cache.data_ptr(), page_stride, pages,
           page_size, table.data_ptr(), table.stride(0), width, requests, request.data_ptr(), position.data_ptr(), rows, heads, kv_heads, dim,
-          _TYPES[q.dtype], 1.0 / math.sqrt(dim) if scale is None else scale, window, keys, out.data_ptr(), out_row, out_head, N.ptr(lse),
+          dtype, 1.0 / math.sqrt(dim) if scale is None else scale, window, keys, out.data_ptr(), out_row, out_head, N.ptr(lse),
           N.ptr(err_flag), N.ptr(ws), nbytes)
     return out
