@@ -104,23 +104,16 @@ def test_python_functions_refuse_host_tensors():
 def test_python_checks():
     """The functions that the operators' argument checks are made of, on host tensors."""
     x = torch.zeros(4, 3, 8)
-    ops._rows("t", "x", x, 4, 3, 8, torch.float32)
+    assert ops._rows("t", "x", x, (4, 3, 8), torch.float32) == (24, 8, 1)
     for bad in (x.half(), x[:3], x[:, :2], x[..., :7], x.transpose(1, 2).contiguous().transpose(1, 2)):
         with pytest.raises(ValueError, match="t: x must be"):
-            ops._rows("t", "x", bad, 4, 3, 8, torch.float32)
-    n = torch.zeros(6, dtype=torch.int32)
-    ops._flat("t", "n", n, torch.int32, 6)
-    for bad in (n.long(), n[:5], n.view(2, 3), torch.zeros(12, dtype=torch.int32)[::2]):
-        with pytest.raises(ValueError, match="t: n must be"):
-            ops._flat("t", "n", bad, torch.int32, 6)
+            ops._rows("t", "x", bad, (4, 3, 8), torch.float32)
     cache = torch.zeros(5, 2, 2, 16, 8)                        # keys and values of a page side by side
-    ops._caches("t", cache[:, 0], cache[:, 1])
+    assert ops._caches("t", cache[:, 0], cache[:, 1]) == (cache[:, 0].shape, 2 * 2 * 16 * 8)
     for k, v in ((cache[:, 0], cache[:4, 1]), (cache[:, 0], cache[:, 1].half()), (cache[:, 0], cache[:, 1].contiguous()),
                  (cache[0], cache[0][:1]), (cache[:, 0].transpose(1, 2), cache[:, 1].transpose(1, 2)), (cache[:, 0].long(), cache[:, 1].long())):
         with pytest.raises(ValueError, match="t: "):
             ops._caches("t", k, v)
-    with pytest.raises(ValueError, match="table"):
-        ops._table("t", torch.zeros(4, 6, dtype=torch.int32)[:, ::2])
 
 
 def test_rotary_frequencies():

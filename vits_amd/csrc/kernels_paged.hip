@@ -21,29 +21,28 @@ constexpr int WAVE = 64;
 // ---------------------------------------------------------------------------------------------------------
 constexpr int PLAN_THREADS = 256;
 constexpr int PLAN_ROWS = 1024;              // rows of a block: four consecutive ones a thread, 16-byte stores
+constexpr int PLAN_SHARE = 32;               // requests whose lengths and returned pages a block writes, at most: its four waves
+                                             // return pages a request at a time
 
 struct PlanSums {
   long long rows, fresh, back;
 };
-
-__device__ __forceinline__ long long shfl_up64(long long v, int d) { return __shfl_up(v, d, WAVE); }
-
-__device__ __forceinline__ PlanSums plan_of(int len, int grow, unsigned page) {
-  PlanSums p;
-  const unsigned l = len < 0 ? 0u : (unsigned)len, a = grow < 0 ? 0u : (unsigned)grow;
-  const long long held = l / page + (l % page != 0);
-  const unsigned after = l + a;              // below 2^32
-  p.rows = a;
-  p.fresh = (long long)(after / page + (after % page != 0)) - held;
-  p.back = grow < 0 ? held : 0;
-  return p;
+// a request's share of them, and the pages it holds before and after
+struct PlanOf {
+  unsigned rows, held, after;
+  __device__ __forceinline__ unsigned fresh() const { return after - held; }
+  __device__ __forceinline__ unsigned back(int grow) const { return grow < 0 ? held : 0u; }
+};
+__device__ __forceinline__ PlanOf plan_of(int len, int grow, unsigned page) {      // len >= 0, len + grow < 2^31
+  const unsigned a = grow < 0 ? 0u : (unsigned)grow, l = (unsigned)len;
+  return PlanOf{a, (l + page - 1) / page, (l + a + page - 1) / page};              // page <= 65536: below 2^32
 }
 
 __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PagePlanArgs a) {
   __shared__ PlanSums wave_sum[PLAN_THREADS / WAVE];
   __shared__ int wave_bad[PLAN_THREADS / WAVE], wave_mark[PLAN_THREADS / WAVE];
   __shared__ int mark[PLAN_ROWS], m_base[PLAN_ROWS], m_held[PLAN_ROWS], m_fresh[PLAN_ROWS];
-  __shared__ int gone[PLAN_THREADS], gone_held[PLAN_THREADS], gone_at[PLAN_THREADS], n_gone;
+  __shared__ int gone[PLAN_SHARE], gone_held[PLAN_SHARE], gone_at[PLAN_SHARE], n_gone;
   const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
   const unsigned page = (unsigned)a.page_size;
   const int each = (a.requests + PLAN_THREADS - 1) / PLAN_THREADS;
@@ -55,14 +54,14 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PagePlanArgs a)
   for (int s = s0; s < s1; ++s) {
     const int len = a.lengths[s], g = a.grow[s];
     if (len < 0 || g < -1 || (g > 0 && len > 0x7fffffff - g)) { bad |= VITS_PLAN_BAD_LENGTH; continue; }
-    const PlanSums p = plan_of(len, g, page);
-    if (((long long)len + (g > 0 ? g : 0) + page - 1) / page > a.width) bad |= VITS_PLAN_TABLE_FULL;
-    mine.rows += p.rows; mine.fresh += p.fresh; mine.back += p.back;
+    const PlanOf p = plan_of(len, g, page);
+    if (p.after > (unsigned)a.width) bad |= VITS_PLAN_TABLE_FULL;
+    mine.rows += p.rows; mine.fresh += p.fresh(); mine.back += p.back(g);
   }
   PlanSums upto = mine;                      // inclusive over the wave
 #pragma unroll
   for (int d = 1; d < WAVE; d <<= 1) {
-    const long long r = shfl_up64(upto.rows, d), f = shfl_up64(upto.fresh, d), b = shfl_up64(upto.back, d);
+    const long long r = __shfl_up(upto.rows, d, WAVE), f = __shfl_up(upto.fresh, d, WAVE), b = __shfl_up(upto.back, d, WAVE);
     if (lane >= d) { upto.rows += r; upto.fresh += f; upto.back += b; }
     bad |= __shfl_xor(bad, d, WAVE);
   }
@@ -82,11 +81,13 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PagePlanArgs a)
   if (head < 0 || free_pages < 0 || free_pages > a.pages || free_pages + total.back > a.pages) bad |= VITS_PLAN_BAD_RING;
   if (total.rows > a.rows) bad |= VITS_PLAN_ROWS_FULL;
   if (total.fresh > free_pages) bad |= VITS_PLAN_NO_PAGES;
-  const int ring0 = bad ? 0 : (int)(head % a.pages), ring1 = bad ? 0 : (int)(tail % a.pages);
+  // (a counter of less than 2^32 pages is divided in 32 bits: 64 take a long routine)
+  auto place_of = [&](long long c) { return bad ? 0 : c >> 32 ? (int)(c % a.pages) : (int)((unsigned)c % (unsigned)a.pages); };
+  const int ring0 = place_of(head), ring1 = place_of(tail);
 
   // pass 2: mark where requests begin in this block's rows; write what belongs to this block's share of the requests
   const int row0 = blockIdx.x * PLAN_ROWS;
-  const int own0 = blockIdx.x * PLAN_THREADS, own1 = own0 + PLAN_THREADS;
+  const int share = (a.requests + gridDim.x - 1) / gridDim.x, own0 = blockIdx.x * share, own1 = own0 + share;   // at most PLAN_SHARE
   for (int s = s0; s < s1; ++s) {
     const int len = a.lengths[s], g = a.grow[s];
     const bool own = s >= own0 && s < own1;
@@ -94,23 +95,23 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PagePlanArgs a)
       if (own) { a.lengths_out[s] = len; a.row_start[s] = 0; }
       continue;
     }
-    const PlanSums p = plan_of(len, g, page);
+    const PlanOf p = plan_of(len, g, page);
     if (own) {
       a.lengths_out[s] = g < 0 ? 0 : len + g;
       a.row_start[s] = (int)before.rows;
-      if (p.back > 0) {
+      if (p.back(g) > 0) {
         const int n = atomicAdd(&n_gone, 1);           // the order in this list does not reach the results
-        gone[n] = s; gone_held[n] = (int)p.back; gone_at[n] = (int)before.back;
+        gone[n] = s; gone_held[n] = (int)p.held; gone_at[n] = (int)before.back;
       }
     }
     if (p.rows > 0 && before.rows < (long long)row0 + PLAN_ROWS && before.rows + p.rows > row0) {
       const int at = before.rows > row0 ? (int)(before.rows - row0) : 0;
       mark[at] = s;
       m_base[at] = len - (int)before.rows;
-      m_held[at] = (int)(len / page + (len % page != 0));
+      m_held[at] = (int)p.held;
       m_fresh[at] = (int)before.fresh;
     }
-    before.rows += p.rows; before.fresh += p.fresh; before.back += p.back;
+    before.rows += p.rows; before.fresh += p.fresh(); before.back += p.back(g);
   }
   if (blockIdx.x == 0 && tid == 0) {
     a.row_start[a.requests] = bad ? 0 : (int)total.rows;
@@ -1230,7 +1231,7 @@ hipError_t start_attention_t(const PagedAttArgs& a, const AttPlan& p, AttForm fo
 }  // namespace
 
 hipError_t launch_page_plan(const PagePlanArgs& a, hipStream_t s) {
-  const int tiles = (a.rows + PLAN_ROWS - 1) / PLAN_ROWS, shares = (a.requests + PLAN_THREADS - 1) / PLAN_THREADS;
+  const int tiles = (a.rows + PLAN_ROWS - 1) / PLAN_ROWS, shares = (a.requests + PLAN_SHARE - 1) / PLAN_SHARE;
   hipLaunchKernelGGL(page_plan_kernel, dim3(tiles > shares ? tiles : shares), dim3(PLAN_THREADS), 0, s, a);
   return hipGetLastError();
 }

@@ -55,21 +55,17 @@ def new_pages(requests: int, width: int, pages: int, device="cuda") -> Pages:
                  torch.tensor([0, pages], dtype=torch.int64, device=device))
 
 
-def _flat(what: str, name: str, t: torch.Tensor, dtype, n: Optional[int] = None) -> None:
-    if t.dtype != dtype or t.dim() != 1 or (n is not None and t.numel() != n) or not t.is_contiguous():
-        raise ValueError(f"{what}: {name} must be contiguous {dtype} [{'n' if n is None else n}], got {t.dtype} {list(t.shape)}")
+def _refuse(what: str, name: str, t: torch.Tensor, dtype, shape) -> None:
+    raise ValueError(f"{what}: {name} must be contiguous {dtype} [{shape}], got {t.dtype} {list(t.shape)}, strides {list(t.stride())}")
 
 
-def _rows(what: str, name: str, t: torch.Tensor, rows: int, heads: Optional[int], dim: int, dtype) -> None:
-    if t.dtype != dtype or t.dim() != 3 or t.shape[0] != rows or (heads is not None and t.shape[1] != heads) or t.shape[2] != dim \
-            or (t.stride(2) != 1 and dim > 1):
-        raise ValueError(f"{what}: {name} must be {dtype} [{rows}, {'heads' if heads is None else heads}, {dim}] with contiguous "
-                         f"channels, got {t.dtype} {list(t.shape)}, strides {list(t.stride())}")
-
-
-def _table(what: str, table: torch.Tensor) -> None:
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.stride(1) != 1 and table.shape[1] > 1):
-        raise ValueError(f"{what}: table must be int32 [requests, width] with contiguous rows, got {table.dtype} {list(table.shape)}")
+def _rows(what: str, name: str, t: torch.Tensor, shape, dtype) -> tuple:
+    """Strides of a tensor of rows [rows, heads, dim] whose channels are contiguous."""
+    strides = t.stride()
+    if t.dtype is not dtype or t.shape != shape or (strides[2] != 1 and shape[2] > 1):
+        raise ValueError(f"{what}: {name} must be {dtype} {list(shape)} with contiguous channels, got {t.dtype} {list(t.shape)}, strides "
+                         f"{list(strides)}")
+    return strides
 
 
 def _caches(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor):
@@ -128,16 +124,20 @@ def page_plan(lengths: torch.Tensor, grow: torch.Tensor, table: torch.Tensor, ri
     if rows is None:
         rows = request.numel()
     index = _device(what, lengths, grow, table, ring, cursor, *out)
-    for name, t, dtype, k in (("lengths", lengths, i32, n), ("grow", grow, i32, n), ("ring", ring, i32, None), ("cursor", cursor, i64, 2),
-                              ("out.lengths", lengths_out, i32, n), ("out.cursor", cursor_out, i64, 2), ("out.start", start, i32, n + 1),
-                              ("out.request", request, i32, rows), ("out.position", position, i32, rows), ("out.slot", slot, i64, rows),
-                              ("out.status", status, i32, 1)):
-        if t.dtype != dtype or not t.is_contiguous() or t.dim() != 1 or t.numel() != k:
-            _flat(what, name, t, dtype, k)
-    _table(what, table)
-    if table.shape[0] != n:
-        raise ValueError(f"page_plan: table has {table.shape[0]} rows for {n} requests")
-    _call(what, index, N.lib.vits_op_page_plan, lengths.data_ptr(), grow.data_ptr(), n, table.data_ptr(), table.stride(0), table.shape[1],
+    requests, width = table.shape if table.dim() == 2 else (-1, 0)
+    if not (lengths.dtype is i32 and lengths.is_contiguous() and grow.dtype is i32 and grow.numel() == n and grow.is_contiguous()
+            and ring.dtype is i32 and ring.is_contiguous() and cursor.dtype is i64 and cursor.numel() == 2 and cursor.is_contiguous()
+            and table.dtype is i32 and requests == n and (table.stride(1) == 1 or width == 1)
+            and lengths_out.dtype is i32 and lengths_out.numel() == n and lengths_out.is_contiguous()
+            and cursor_out.dtype is i64 and cursor_out.numel() == 2 and cursor_out.is_contiguous()
+            and start.dtype is i32 and start.numel() == n + 1 and start.is_contiguous()
+            and request.dtype is i32 and request.numel() == rows and request.is_contiguous()
+            and position.dtype is i32 and position.numel() == rows and position.is_contiguous()
+            and slot.dtype is i64 and slot.numel() == rows and slot.is_contiguous() and status.dtype is i32 and status.numel() == 1):
+        raise ValueError(f"page_plan: needs contiguous int32 lengths [requests], grow [requests], table [requests, width] (rows contiguous), ring "
+                         f"[pages], int64 cursor [2], and as outputs a PagePlan's tensors with {rows} rows, got "
+                         + ", ".join(f"{t.dtype} {list(t.shape)}" for t in (lengths, grow, table, ring, cursor, *out)))
+    _call(what, index, N.lib.vits_op_page_plan, lengths.data_ptr(), grow.data_ptr(), n, table.data_ptr(), table.stride(0), width,
           ring.data_ptr(), ring.numel(), cursor.data_ptr(), page_size, lengths_out.data_ptr(), cursor_out.data_ptr(), start.data_ptr(),
           request.data_ptr(), position.data_ptr(), slot.data_ptr(), rows, status.data_ptr())
     return out if type(out) is PagePlan else PagePlan(*out)
@@ -188,21 +188,21 @@ def rotary_store(q: Optional[torch.Tensor], k: Optional[torch.Tensor], v: Option
         raise ValueError(f"rotary_store: rows must be fp32, fp16 or bf16 [rows, heads, dim], got {dtype} {list(first.shape)}")
     rows, _, dim = first.shape
     index = _device(what, first, k, v, k_cache, v_cache, position, slot, freq, out, err_flag)
-    _flat(what, "position", position, torch.int32, rows)
-    _flat(what, "freq", freq, torch.float64)
-    if slot is not None:
-        _flat(what, "slot", slot, torch.int64, rows)
+    if position.dtype is not torch.int32 or position.numel() != rows or not position.is_contiguous():
+        _refuse(what, "position", position, torch.int32, rows)
+    if freq.dtype is not torch.float64 or not freq.is_contiguous():
+        _refuse(what, "freq", freq, torch.float64, "pairs")
+    if slot is not None and (slot.dtype is not torch.int64 or slot.numel() != rows or not slot.is_contiguous()):
+        _refuse(what, "slot", slot, torch.int64, rows)
     q_at = q_row = q_head = out_at = out_row = out_head = heads = 0
     if q is not None:
-        heads = q.shape[1]
-        _rows(what, "q", q, rows, heads, dim, dtype)
+        shape = q.shape
+        heads = shape[1]
         if out is None:
             # rows that are no rows are left as they were: not as the allocator found them
-            out = (torch.empty if slot is None else torch.zeros)((rows, heads, dim), dtype=dtype, device=q.device)
-        else:
-            _rows(what, "out", out, rows, heads, dim, dtype)
-        q_at, (q_row, q_head, _) = q.data_ptr(), q.stride()
-        out_at, (out_row, out_head, _) = out.data_ptr(), out.stride()
+            out = (torch.empty if slot is None else torch.zeros)(shape, dtype=dtype, device=q.device)
+        q_at, (q_row, q_head, _) = q.data_ptr(), _rows(what, "q", q, shape, dtype)
+        out_at, (out_row, out_head, _) = out.data_ptr(), _rows(what, "out", out, shape, dtype)
     elif out is not None:
         raise ValueError("rotary_store: out without q")
     k_at = k_row = k_head = v_at = v_row = v_head = kc = vc = page_stride = pages = page_size = kv_heads = 0
@@ -210,17 +210,16 @@ def rotary_store(q: Optional[torch.Tensor], k: Optional[torch.Tensor], v: Option
         if v is None or k_cache is None or v_cache is None or slot is None:
             raise ValueError("rotary_store: keys need values, both caches and slots")
         (pages, kv_heads, page_size, channels), page_stride = _caches(what, k_cache, v_cache)
-        _rows(what, "k", k, rows, kv_heads, dim, dtype)
-        _rows(what, "v", v, rows, kv_heads, dim, dtype)
-        if k_cache.dtype != dtype or channels != dim:
+        if k_cache.dtype is not dtype or channels != dim:
             raise ValueError(f"rotary_store: caches of {k_cache.dtype} with {channels} channels for rows of {dtype} with {dim}")
-        k_at, (k_row, k_head, _) = k.data_ptr(), k.stride()
-        v_at, (v_row, v_head, _) = v.data_ptr(), v.stride()
+        shape = (rows, kv_heads, dim)
+        k_at, (k_row, k_head, _) = k.data_ptr(), _rows(what, "k", k, shape, dtype)
+        v_at, (v_row, v_head, _) = v.data_ptr(), _rows(what, "v", v, shape, dtype)
         kc, vc = k_cache.data_ptr(), v_cache.data_ptr()
     elif v is not None or k_cache is not None or v_cache is not None:
         raise ValueError("rotary_store: values or caches without keys")
-    if err_flag is not None:
-        _flat(what, "err_flag", err_flag, torch.int32, 1)
+    if err_flag is not None and (err_flag.dtype is not torch.int32 or err_flag.numel() != 1):
+        _refuse(what, "err_flag", err_flag, torch.int32, 1)
     _call(what, index, N.lib.vits_op_rotary_store, q_at, q_row, q_head, out_at, out_row, out_head, heads, k_at, k_row, k_head, v_at, v_row, v_head,
           kc, vc, page_stride, pages, page_size, kv_heads, dim, _TYPES[dtype], position.data_ptr(), N.ptr(slot), rows, freq.data_ptr(),
           freq.numel(), scale, interleaved, N.ptr(err_flag))
@@ -250,19 +249,21 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     rows, heads, dim = q.shape
     index = _device(what, q, k_cache, v_cache, table, request, position, out, lse, err_flag)
     (pages, kv_heads, page_size, channels), page_stride = _caches(what, k_cache, v_cache)
-    _rows(what, "q", q, rows, heads, channels, k_cache.dtype)
-    _flat(what, "request", request, torch.int32, rows)
-    _flat(what, "position", position, torch.int32, rows)
-    _table(what, table)
+    shape = (rows, heads, channels)
+    q_row, q_head, _ = _rows(what, "q", q, shape, k_cache.dtype)
+    if request.dtype is not torch.int32 or request.numel() != rows or not request.is_contiguous():
+        _refuse(what, "request", request, torch.int32, rows)
+    if position.dtype is not torch.int32 or position.numel() != rows or not position.is_contiguous():
+        _refuse(what, "position", position, torch.int32, rows)
+    if table.dtype is not torch.int32 or table.dim() != 2 or (table.stride(1) != 1 and table.shape[1] > 1):
+        _refuse(what, "table", table, torch.int32, "requests, width")
     if out is None:
-        out = torch.zeros((rows, heads, dim), dtype=q.dtype, device=q.device)
-    else:
-        _rows(what, "out", out, rows, heads, dim, q.dtype)
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous()):
-        raise ValueError(f"paged_attention: lse must be contiguous float32 [{rows}, {heads}], got {lse.dtype} {list(lse.shape)}")
-    if err_flag is not None:
-        _flat(what, "err_flag", err_flag, torch.int32, 1)
-    q_row, q_head, _ = q.stride()
+        out = torch.zeros(shape, dtype=q.dtype, device=q.device)
+    out_row, out_head, _ = _rows(what, "out", out, shape, q.dtype)
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous()):
+        _refuse(what, "lse", lse, torch.float32, f"{rows}, {heads}")
+    if err_flag is not None and (err_flag.dtype is not torch.int32 or err_flag.numel() != 1):
+        _refuse(what, "err_flag", err_flag, torch.int32, 1)
     if (q.data_ptr() | q_row * q.element_size() | q_head * q.element_size()) & 15:
         q = q.clone(memory_format=torch.contiguous_format)      # the library reads heads on 16-byte addresses
         q_row, q_head, _ = q.stride()
@@ -274,7 +275,6 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     nbytes = _workspace_bytes(rows, heads, kv_heads, dim, dtype, keys)
     # a workspace of this call's own: calls on different streams, and graphs that run side by side, share none
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    out_row, out_head, _ = out.stride()
     _call(what, index, N.lib.vits_op_paged_attention, q.data_ptr(), q_row, q_head, k_cache.data_ptr(), v_cache.data_ptr(), page_stride, pages,
           page_size, table.data_ptr(), table.stride(0), width, requests, request.data_ptr(), position.data_ptr(), rows, heads, kv_heads, dim,
           dtype, 1.0 / math.sqrt(dim) if scale is None else scale, window, keys, out.data_ptr(), out_row, out_head, N.ptr(lse),
