@@ -47,17 +47,20 @@ ROTARY = dict(q=P, q_row=512, q_head=128, out=P + 4096, out_row=512, out_head=12
     (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(rows=-1), "required"), (dict(dim=1, pairs=1), "required"),
     (dict(dim=258), "required"), (dict(pairs=0), "required"), (dict(pairs=65), "required"), (dict(heads=0), "required"),
     (dict(heads=1025), "required"), (dict(kv_heads=0), "required"), (dict(pages=0), "required"), (dict(page_size=20), "page_size"),
-    (dict(page_stride=2 * 16 * 128 - 1), "overlap"), (dict(out=P, out_row=640), "in place"), (dict(out=P, out_head=64), "in place"),
-    (dict(out=P + 256), "in place"), (dict(k_cache=P + 512), "overlaps"), (dict(v_cache=P + 4096), "overlaps"), (dict(k=P + 4096), "overlaps k or v"),
+    (dict(page_stride=2 * 16 * 128 - 1), "overlap"), (dict(out=P, out_row=640), "in place"), (dict(out=P, out_row=2048, out_head=512), "in place"),
+    (dict(q_row=-1), "strides"), (dict(v_head=-1), "strides"), (dict(out_row=500), "overlap"), (dict(out_head=100), "overlap"), (dict(out_row=0), "overlap"),
+    (dict(rows=(1 << 23) + 1), "2^23"), (dict(out=P + 256), "in place"), (dict(k_cache=P + 512), "overlaps"), (dict(v_cache=P + 4096), "overlaps"), (dict(k=P + 4096), "overlaps k or v"),
     (dict(v=P + 5000), "overlaps k or v"), (dict(k_cache=P - (1 << 10)), "overlaps"),
 ])
 def test_rotary_store_refuses(change, word):
     refused(N.lib.vits_op_rotary_store(*{**ROTARY, **change}.values()), word)
 
 
-ATTEND = dict(q=P, q_row=512, q_head=128, k_cache=P, v_cache=P, page_stride=2 * 16 * 128, pages=9, page_size=16, table=P, table_stride=8,
-              width=8, requests=3, row_request=P, row_position=P, rows=3, heads=4, kv_heads=2, dim=128, dtype=2, scale=0.1, window=0,
-              max_keys=128, out=P + 65536, out_row=512, out_head=128, lse=0, err_flag=0, ws=P, ws_bytes=1 << 40, stream=0)
+M = 1 << 20
+ATTEND = dict(q=P, q_row=512, q_head=128, k_cache=P + M, v_cache=P + 2 * M, page_stride=2 * 16 * 128, pages=9, page_size=16, table=P + 3 * M,
+              table_stride=8, width=8, requests=3, row_request=P + 4 * M, row_position=P + 5 * M, rows=3, heads=4, kv_heads=2, dim=128, dtype=2,
+              scale=0.1, window=0, max_keys=128, out=P + 6 * M, out_row=512, out_head=128, lse=0, err_flag=0, ws=P + 8 * M, ws_bytes=1 << 40,
+              stream=0)
 
 
 @pytest.mark.parametrize("change,word", [
@@ -66,8 +69,11 @@ ATTEND = dict(q=P, q_row=512, q_head=128, k_cache=P, v_cache=P, page_stride=2 * 
     (dict(kv_heads=0), "required"), (dict(heads=2048, kv_heads=2048), "required"), (dict(dim=0), "required"), (dict(dim=48), "required"),
     (dict(dim=288), "required"), (dict(page_size=8), "page_size"), (dict(pages=0), "required"), (dict(width=0), "required"),
     (dict(table_stride=7), "required"), (dict(requests=0), "required"), (dict(window=-1), "required"), (dict(page_stride=100), "overlap"),
-    (dict(k_cache=P + 8), "16-byte"), (dict(v_cache=P + 2), "16-byte"), (dict(page_stride=2 * 16 * 128 + 4), "16-byte"),
-    (dict(out=P), "in place"), (dict(out=P + 1024), "in place"), (dict(q=P + 8), "16-byte"), (dict(q_row=516), "16-byte"), (dict(q_head=132), "16-byte"),
+    (dict(k_cache=P + M + 8), "16-byte"), (dict(v_cache=P + 2 * M + 2), "16-byte"), (dict(page_stride=2 * 16 * 128 + 4), "16-byte"),
+    (dict(out=P), "in place"), (dict(out=P + 1024), "in place"), (dict(out=P + M + 64), "in place"), (dict(out=P + 3 * M), "in place"),
+    (dict(lse=P + 2 * M + 64), "in place"), (dict(lse=P + 6 * M + 64), "overlap"), (dict(ws=P + 6 * M), "overlap"), (dict(ws=P), "in place"),
+    (dict(q_row=-512), "strides"), (dict(out_head=-128), "strides"), (dict(out_row=0), "strides"), (dict(out_head=64), "strides"),
+    (dict(out_row=384), "strides"), (dict(width=1 << 27, table_stride=1 << 27), "2^30"), (dict(rows=(1 << 23) + 1), "2^23"), (dict(q=P + 8), "16-byte"), (dict(q_row=516), "16-byte"), (dict(q_head=132), "16-byte"),
 ])
 def test_paged_attention_refuses(change, word):
     refused(N.lib.vits_op_paged_attention(*{**ATTEND, **change}.values()), word)
@@ -82,7 +88,7 @@ def test_paged_attention_workspace():
     if need:
         refused(N.lib.vits_op_paged_attention(*{**ATTEND, "max_keys": 1 << 20, "ws_bytes": need - 1}.values()), "workspace", WORKSPACE)
         refused(N.lib.vits_op_paged_attention(*{**ATTEND, "max_keys": 1 << 20, "ws": 0}.values()), "workspace", WORKSPACE)
-        refused(N.lib.vits_op_paged_attention(*{**ATTEND, "max_keys": 1 << 20, "ws": P + 8}.values()), "workspace", WORKSPACE)
+        refused(N.lib.vits_op_paged_attention(*{**ATTEND, "max_keys": 1 << 20, "ws": P + 8 * M + 8}.values()), "workspace", WORKSPACE)
 
 
 def test_python_functions_refuse_host_tensors():

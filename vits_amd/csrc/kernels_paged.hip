@@ -459,6 +459,32 @@ __device__ __forceinline__ bool att_run(const PagedAttArgs& a, const AttPlan& p,
   return true;
 }
 
+// the same for a wave whose lanes all ask about the same row: the run's rows are looked at side by side
+__device__ __forceinline__ bool att_run_wave(const PagedAttArgs& a, const AttPlan& p, int row, Run& r) {
+  const int lane = threadIdx.x & (WAVE - 1), here = min(row + min(lane, ATT_COLS - 1), a.rows - 1);
+  const int req = a.row_request[here], before = a.row_request[row > 0 ? row - 1 : 0];
+  int from, to;
+  att_row_keys(a, here, from, to);
+  auto same = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  const int mine = same(req), in = row & ((1 << p.run_shift) - 1);
+  if (mine < 0 || mine >= a.requests || (in > 0 && same(before) == mine)) return false;
+  const int most = min((1 << p.run_shift) - in, a.rows - row);
+  const unsigned long long other = __ballot(lane >= most || req != mine);          // lane 0 is not among them
+  r.n = __builtin_ctzll(other);
+  r.row = row;
+  r.req = mine;
+  r.from = same(from);
+  int low = lane < r.n && from < to ? from : 0x7fffffff, high = lane < r.n ? to : 0;
+#pragma unroll
+  for (int d = 1; d < ATT_COLS; d <<= 1) {
+    low = min(low, __shfl_xor(low, d, WAVE));
+    high = max(high, __shfl_xor(high, d, WAVE));
+  }
+  r.end = same(high);
+  r.begin = same(low) >= r.end ? 0 : same(low) & ~15;
+  return true;
+}
+
 // x / y of numbers that are not negative: 64-bit division is a long routine, and these are seldom that large
 __device__ __forceinline__ long long att_div(long long x, long long y) {
   return (x | y) >> 32 ? x / y : (long long)((unsigned)x / (unsigned)y);
@@ -503,10 +529,10 @@ template <typename T, int DIM>
 struct AttTile {
   static constexpr bool HALF = sizeof(T) == 2;
   // Registers: Q, K, V and O of a step have to fit 256 (two waves a SIMD) with room for the rest.  So wide heads take 16
-  // keys a step, and fp32 ones load K and V in two passes, the second when the first has been used.
+  // keys a step, and fp32 ones load K and V in two or four passes, each when the one before has been used.
   static constexpr int STEP = att_step(sizeof(T), DIM);
   static constexpr int SUB = STEP / 16;                  // 16-key parts of a step
-  static constexpr int PASSES = !HALF && DIM > 160 ? 2 : 1;
+  static constexpr int PASSES = HALF || DIM <= 160 ? 1 : DIM < 256 ? 2 : 4;
   static constexpr int KL = DIM * (int)sizeof(T) / 64;   // 16-byte loads of a lane for 16 keys
   static constexpr int KP = KL / PASSES;
   static constexpr int CH = DIM / 16;                   // channels of a lane in V and in the output
@@ -956,7 +982,7 @@ __global__ __launch_bounds__(ATT_THREADS, 2) void paged_attention_wave_kernel(Pa
   if (row >= a.rows) return;
   if (unit == 0 && threadIdx.x % WAVE == 0) att_flag_row(a, row);
   Run r;
-  if (att_run(a, p, row, r) && att_part<T, DIM>(a, p, r, unit, 0, att_run_steps<AttTile<T, DIM>::STEP>(r), true, nullptr) && a.err_flag)
+  if (att_run_wave(a, p, row, r) && att_part<T, DIM>(a, p, r, unit, 0, att_run_steps<AttTile<T, DIM>::STEP>(r), true, nullptr) && a.err_flag)
     atomicOr(a.err_flag, 1);
 }
 
@@ -968,7 +994,7 @@ __global__ __launch_bounds__(ATT_BLOCK_WAVES * WAVE, 1) void paged_attention_blo
   const int row = blockIdx.x / p.units, unit = blockIdx.x - row * p.units;
   if (unit == 0 && threadIdx.x == 0) att_flag_row(a, row);
   Run r;
-  if (!att_run(a, p, row, r)) return;
+  if (!att_run_wave(a, p, row, r)) return;
   const int steps = att_run_steps<AttTile<T, DIM>::STEP>(r);
   const int each = (steps + ATT_BLOCK_WAVES - 1) / ATT_BLOCK_WAVES, t0 = wave * each, t1 = min(t0 + each, steps);
   if (t0 < t1 && att_part<T, DIM>(a, p, r, unit, t0, t1, false, lds[wave]) && a.err_flag) atomicOr(a.err_flag, 1);
@@ -1064,7 +1090,7 @@ __global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attenti
       }
       if (pos >= last) break;
       run_at += (long long)steps * p.units;
-      do ++row; while (!att_run(a, p, row, r));           // pos < total: there is one
+      do ++row; while (!att_run_wave(a, p, row, r));         // pos < total: there is one
     }
     if (stray && a.err_flag) atomicOr(a.err_flag, 1);
   }

@@ -354,6 +354,13 @@ Span span(const void* p, int64_t n) { return Span{(const char*)p, p ? n : 0}; }
 Span span(const void* p, int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t dim, int size) {
   return span(p, rows > 0 && heads > 0 ? ((rows - 1) * row + (heads - 1) * head + dim) * size : 0);
 }
+// rows and heads of an output do not lie over each other, whichever of the two runs faster
+bool apart(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t dim) {
+  if (rows <= 1) row = 1ll << 40;
+  if (heads <= 1) head = 0;
+  return row >= 0 && head >= 0 && (rows <= 1 || heads <= 1 ? (rows <= 1 || row >= dim) && (heads <= 1 || head >= dim)
+                                   : (head >= dim && row >= (heads - 1) * head + dim) || (row >= dim && head >= (rows - 1) * row + dim));
+}
 bool overlap(const Span& a, const Span& b) { return a.n > 0 && b.n > 0 && a.p < b.p + b.n && b.p < a.p + a.n; }
 
 int check_page_size(int page_size) {
@@ -1498,6 +1505,8 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
   }
   if (rows == 0) return VITS_OK;
   const int size = dtype == VITS_TYPE_F32 ? 4 : 2;
+  if (q_row < 0 || q_head < 0 || k_row < 0 || k_head < 0 || v_row < 0 || v_head < 0 || (q && !apart(rows, out_row, heads, out_head, dim)))
+    return fail(VITS_ERR_INVALID, "rotary store: strides must not be negative, nor rows or heads of out overlap");
   const Span to = span(out, rows, out_row, q ? heads : 0, out_head, dim, size), from = span(q, rows, q_row, heads, q_head, dim, size);
   if (q && !(q == out && q_row == out_row && q_head == out_head) && overlap(from, to))
     return fail(VITS_ERR_INVALID, "rotary store: in place needs the same strides on both sides, and no other overlap");
@@ -1544,8 +1553,18 @@ int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const 
                                   "request whose rows do not overlap and a window that is not negative required");
   if (page_stride < (int64_t)kv_heads * page_size * dim) return fail(VITS_ERR_INVALID, "paged attention: pages overlap");
   const int size = dtype == VITS_TYPE_F32 ? 4 : 2;
-  if (overlap(span(q, rows, q_row, heads, q_head, dim, size), span(out, rows, out_row, heads, out_head, dim, size)))
-    return fail(VITS_ERR_INVALID, "paged attention: cannot run in place");
+  if (q_row < 0 || q_head < 0 || !apart(rows, out_row, heads, out_head, dim))
+    return fail(VITS_ERR_INVALID, "paged attention: strides must not be negative, nor rows or heads of out overlap");
+  const int64_t cache = ((pages - 1) * page_stride + (int64_t)kv_heads * page_size * dim) * size;
+  const Span outs[3] = {span(out, rows, out_row, heads, out_head, dim, size), span(lse, 4ll * rows * heads), span(ws, ws_bytes)};
+  const Span ins[6] = {span(q, rows, q_row, heads, q_head, dim, size), span(k_cache, cache), span(v_cache, cache),
+                       span(table, 4ll * ((requests - 1) * table_stride + width)), span(row_request, 4ll * rows), span(row_position, 4ll * rows)};
+  for (int i = 0; i < 3; ++i) {
+    for (const Span& x : ins)
+      if (overlap(outs[i], x)) return fail(VITS_ERR_INVALID, "paged attention: cannot run in place: an output or the workspace overlaps an input");
+    for (int j = 0; j < i; ++j)
+      if (overlap(outs[i], outs[j])) return fail(VITS_ERR_INVALID, "paged attention: out, lse and the workspace overlap");
+  }
   if ((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)q) & 15) || (page_stride * size) % 16 || (q_row * size) % 16 || (q_head * size) % 16)
     return fail(VITS_ERR_INVALID, "paged attention: the caches, their pages and the heads of q must begin on 16-byte addresses");
   if (ws_bytes < paged_attention_workspace(rows, heads, kv_heads, dim, dtype, max_keys) || (ws_bytes > 0 && !ws) || ((uintptr_t)ws & 15))
