@@ -4,6 +4,8 @@
 #include "paged.h"
 #include "../../include/vits_amd.h"
 
+#include <type_traits>
+
 namespace vits {
 namespace {
 
@@ -366,8 +368,8 @@ hipError_t start_rotary_t(RotaryArgs a, hipStream_t s) {
 // same rows, lane n of it the channels n * DIM / 16 and on, whole rows in one instruction.  Nothing of the cache passes
 // through LDS, and no wave waits for another inside the loop over the keys.
 // 16-bit types: v_mfma_f32_16x16x32, 32 keys a step; v_perm pairs the rows' channels to operands.  fp32: v_mfma_f32_16x16x4,
-// 16 keys a step.  bf16 weights go in as two terms (w = h + l, 2^-17 relative): the product's matrix time is a small part of the
-// load time; fp16 weights as one (2^-12 relative).
+// 16 keys a step.  16-bit weights go in as two terms (w = h + l: 2^-17 relative in bf16, 2^-22 in fp16), so that the result carries
+// one rounding only, its own: the products' matrix time is a small part of the load time.
 // ---------------------------------------------------------------------------------------------------------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -601,7 +603,7 @@ struct AttTile {
   // the weights of a step as operands
   struct Weights {
     f32x4 f;                                            // fp32
-    unsigned hi[2 * SUB], lo[2 * SUB];                  // 16 bits: two keys each; lo is what bf16 leaves of a weight
+    unsigned hi[2 * SUB], lo[2 * SUB];                  // 16 bits: two keys each; lo is what 16 bits leave of a weight
   };
   static __device__ __forceinline__ Weights weights(const f32x4 (&p)[SUB]) {
     Weights w;
@@ -610,13 +612,10 @@ struct AttTile {
 #pragma unroll
       for (int i = 0; i < 2 * SUB; ++i) {
         const f32x2 x = {p[i / 2][i % 2 * 2], p[i / 2][i % 2 * 2 + 1]};
-        if constexpr (__is_same(T, __bf16)) {
-          const bf16x2 h = __builtin_convertvector(x, bf16x2);
-          w.hi[i] = __builtin_bit_cast(unsigned, h);
-          w.lo[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(x - __builtin_convertvector(h, f32x2), bf16x2));
-        } else {
-          w.hi[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(x, f16x2));
-        }
+        using Two = std::conditional_t<__is_same(T, __bf16), bf16x2, f16x2>;
+        const Two h = __builtin_convertvector(x, Two);
+        w.hi[i] = __builtin_bit_cast(unsigned, h);
+        w.lo[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(x - __builtin_convertvector(h, f32x2), Two));
       }
     }
     return w;
@@ -663,10 +662,8 @@ struct AttTile {
         even[i] = __builtin_amdgcn_perm(y, x, 0x05040100);
         odd[i] = __builtin_amdgcn_perm(y, x, 0x07060302);
       }
-      if constexpr (__is_same(T, __bf16)) {
-        c[0] = product(even, p.lo, c[0]);
-        c[1] = product(odd, p.lo, c[1]);
-      }
+      c[0] = product(even, p.lo, c[0]);
+      c[1] = product(odd, p.lo, c[1]);
       c[0] = product(even, p.hi, c[0]);
       c[1] = product(odd, p.hi, c[1]);
     }
