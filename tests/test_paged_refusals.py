@@ -91,35 +91,71 @@ def test_paged_attention_workspace():
         refused(N.lib.vits_op_paged_attention(*{**ATTEND, "max_keys": 1 << 20, "ws": P + 8 * M + 8}.values()), "workspace", WORKSPACE)
 
 
-def test_python_functions_refuse_host_tensors():
+def i32(*values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+def test_page_plan_checks_its_tensors():
+    """Shapes and types first, so that they can be told here; then that the tensors are on a GPU."""
     pages = ops.new_pages(3, 4, 20, device="cpu")
+    good = dict(lengths=pages.lengths, grow=i32(1, 1, 1), table=pages.table, ring=pages.ring, cursor=pages.cursor, page_size=16)
+    out = [torch.empty(n, dtype=torch.int64 if i in (1, 5) else torch.int32) for i, n in enumerate((3, 2, 4, 5, 5, 5, 1))]
     with pytest.raises(ValueError, match="GPU"):
-        ops.page_plan(pages.lengths, torch.zeros(3, dtype=torch.int32), pages.table, pages.ring, pages.cursor, 16, rows=4)
+        ops.page_plan(**good, rows=4)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.page_plan(**good, out=out)
     with pytest.raises(ValueError, match="rows or out"):
-        ops.page_plan(pages.lengths, torch.zeros(3, dtype=torch.int32), pages.table, pages.ring, pages.cursor, 16)
-    q, cache = torch.zeros(2, 4, 64), torch.zeros(20, 2, 16, 64)
-    i32 = torch.zeros(2, dtype=torch.int32)
-    with pytest.raises(ValueError, match="GPU"):
-        ops.rotary_store(q, None, None, None, None, i32, None, ops.rotary_frequencies(64, device="cpu"))
-    with pytest.raises(ValueError, match="neither"):
-        ops.rotary_store(None, None, None, None, None, i32, None, ops.rotary_frequencies(64, device="cpu"))
-    with pytest.raises(ValueError, match="GPU"):
-        ops.paged_attention(q, cache, cache, pages.table, i32, i32)
+        ops.page_plan(**good)
+    with pytest.raises(ValueError, match="seven"):
+        ops.page_plan(**good, out=out[:6])
+    for name, bad in (("lengths", pages.lengths.long()), ("grow", i32(1, 1)), ("table", pages.table[:2]), ("table", pages.table.t()),
+                      ("table", pages.table.long()), ("table", torch.zeros(3, 8, dtype=torch.int32)[:, ::2]), ("ring", pages.ring.long()),
+                      ("ring", pages.ring[::2]), ("cursor", pages.cursor.int()), ("cursor", torch.zeros(3, dtype=torch.int64)), ("grow", None)):
+        with pytest.raises(ValueError, match=name):
+            ops.page_plan(**{**good, name: bad}, rows=4)
+    for i, name in enumerate(("lengths", "cursor", "start", "request", "position", "slot", "status")):
+        for bad in (out[i].float(), torch.empty(9, dtype=out[i].dtype)):
+            with pytest.raises(ValueError, match="out." + name):
+                ops.page_plan(**good, rows=5, out=[*out[:i], bad, *out[i + 1:]])
+    with pytest.raises(ValueError, match="out.request"):
+        ops.page_plan(**good, rows=6, out=out)
 
 
-def test_python_checks():
-    """The functions that the operators' argument checks are made of, on host tensors."""
-    x = torch.zeros(4, 3, 8)
-    assert ops._rows("t", "x", x, (4, 3, 8), torch.float32) == (24, 8, 1)
-    for bad in (x.half(), x[:3], x[:, :2], x[..., :7], x.transpose(1, 2).contiguous().transpose(1, 2)):
-        with pytest.raises(ValueError, match="t: x must be"):
-            ops._rows("t", "x", bad, (4, 3, 8), torch.float32)
-    cache = torch.zeros(5, 2, 2, 16, 8)                        # keys and values of a page side by side
-    assert ops._caches("t", cache[:, 0], cache[:, 1]) == (cache[:, 0].shape, 2 * 2 * 16 * 8)
-    for k, v in ((cache[:, 0], cache[:4, 1]), (cache[:, 0], cache[:, 1].half()), (cache[:, 0], cache[:, 1].contiguous()),
-                 (cache[0], cache[0][:1]), (cache[:, 0].transpose(1, 2), cache[:, 1].transpose(1, 2)), (cache[:, 0].long(), cache[:, 1].long())):
-        with pytest.raises(ValueError, match="t: "):
-            ops._caches("t", k, v)
+def test_rotary_store_checks_its_tensors():
+    q, k, v = torch.zeros(4, 4, 64), torch.zeros(4, 2, 64), torch.zeros(4, 2, 64)
+    cache = torch.zeros(5, 2, 2, 16, 64)                       # keys and values of a page side by side
+    freq = ops.rotary_frequencies(64, device="cpu")
+    good = dict(q=q, k=k, v=v, k_cache=cache[:, 0], v_cache=cache[:, 1], position=i32(0, 1, 2, 3), slot=torch.arange(4), freq=freq)
+    alone = dict(k=None, v=None, k_cache=None, v_cache=None)
+    for change in ({}, alone, {**alone, "slot": None}, dict(q=None), dict(out=torch.zeros(4, 4, 64)), dict(err_flag=i32(0))):
+        with pytest.raises(ValueError, match="GPU"):
+            ops.rotary_store(**{**good, **change})
+    for change, word in ((dict(q=None, **alone), "neither"), (dict(q=None, out=q), "without q"), (dict(v=None), "together"), (dict(k=None), "together"),
+                         (dict(slot=None), "together"), (dict(k_cache=None), "together"), (dict(q=q.double()), "fp32"), (dict(q=q[0]), "rows"),
+                         (dict(q=q[:3]), "position"), (dict(k=k[:, :1]), "k must"), (dict(v=v.half()), "v must"), (dict(k=k[..., :32]), "k must"),
+                         (dict(q=q.transpose(1, 2).contiguous().transpose(1, 2)), "q must"), (dict(out=q[:, :2]), "out must"),
+                         (dict(out=q.half()), "out must"), (dict(k_cache=cache[:4, 0]), "alike"), (dict(v_cache=cache[:, 1].contiguous()), "alike"),
+                         (dict(k_cache=cache[:, 0].half(), v_cache=cache[:, 1].half()), "caches"),
+                         (dict(k_cache=cache[:, 0].transpose(1, 2), v_cache=cache[:, 1].transpose(1, 2)), "alike"),
+                         (dict(position=torch.arange(4)), "position"), (dict(slot=i32(0, 1, 2, 3)), "slot"), (dict(freq=freq.float()), "freq"),
+                         (dict(err_flag=i32(0, 0)), "err_flag")):
+        with pytest.raises(ValueError, match=word):
+            ops.rotary_store(**{**good, **change})
+
+
+def test_paged_attention_checks_its_tensors():
+    q, cache = torch.zeros(2, 4, 64), torch.zeros(5, 2, 2, 16, 64)
+    good = dict(q=q, k_cache=cache[:, 0], v_cache=cache[:, 1], table=torch.zeros(3, 4, dtype=torch.int32), request=i32(0, 1), position=i32(3, 4))
+    for change in ({}, dict(out=torch.zeros(2, 4, 64)), dict(lse=torch.zeros(2, 4)), dict(err_flag=i32(0))):
+        with pytest.raises(ValueError, match="GPU"):
+            ops.paged_attention(**{**good, **change})
+    for change, word in ((dict(q=q.half()), "q must"), (dict(q=q[0]), "rows"), (dict(q=q[..., :32]), "q must"), (dict(table=good["table"].long()), "table"),
+                         (dict(table=good["table"][0]), "table"), (dict(request=i32(0)), "request"), (dict(position=torch.tensor([3, 4])), "position"),
+                         (dict(out=q.double()), "out must"), (dict(out=torch.zeros(2, 4, 32)), "out must"), (dict(lse=torch.zeros(2, 3)), "lse"),
+                         (dict(lse=torch.zeros(2, 4, dtype=torch.float64)), "lse"), (dict(k_cache=cache[:, 0, :, :8]), "alike"),
+                         (dict(k_cache=cache[:, 0].long(), v_cache=cache[:, 1].long()), "fp32"), (dict(err_flag=torch.zeros(1)), "err_flag")):
+        with pytest.raises(ValueError, match=word):
+            ops.paged_attention(**{**good, **change})
 
 
 def test_rotary_frequencies():

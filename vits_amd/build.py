@@ -4,12 +4,15 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libvits_amd.so")
+BINDING = os.path.join(LIBDIR, "_vits_ops.so")      # torch tensors to the library's paged-cache operators (host code only)
+CXX = os.environ.get("CXX", "g++")
 SOURCES = ["kernels_conv.hip", "kernels_gl16.hip", "kernels_chain.hip", "kernels_misc.hip", "kernels_paged.hip",
            "model.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -36,6 +39,13 @@ def build(force: bool = False, verbose: bool = True) -> str:
     paged = [os.path.join(CSRC, "paged.h")] + headers[1:]
     deps = {"kernels_paged.hip": paged, "model.hip": headers + paged}
     objs, jobs = [], []
+    bind = os.path.join(CSRC, "ops_binding.cpp")
+    if force or _stale(BINDING, [bind]):
+        import torch
+        at = os.path.dirname(torch.__file__)
+        jobs.append([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                     "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(at, "include"), bind, "-o", BINDING,
+                     "-L" + os.path.join(at, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"])
     for src in SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(LIBDIR, src.replace(".hip", ".o"))
