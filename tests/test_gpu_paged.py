@@ -171,6 +171,23 @@ def test_plan_refuses_on_the_gpu(ops):
         assert want["status"][0] & bit
 
 
+@pytest.mark.parametrize("lengths,grow,bits", [([0] * 4, [1 << 30] * 4, "ROWS_FULL"), ([0] * 300, [1 << 30] * 4 + [0] * 296, "ROWS_FULL"),
+                                               ([2 ** 31 - 1] * 32, [-1] * 32, "BAD_RING"), ([2 ** 31 - 1] * 512, [-1] * 512, "BAD_RING"),
+                                               ([0] * 32, [2 ** 31 - 1] * 32, "NO_PAGES")])
+def test_plan_of_sums_beyond_32_bits(ops, lengths, grow, bits):
+    """Sums that are a multiple of 2^32: refused, not taken for nothing."""
+    from vits_amd import _native as N
+    width, rows = 4, 40
+    table, ring = [[0] * width for _ in lengths], list(range(6))
+    dev = (gpu_i32(lengths), gpu_i32(grow), gpu_i32(table), gpu_i32(ring), torch.tensor([0, 6], dtype=torch.int64, device="cuda"))
+    want = plan_by_hand(lengths, grow, table, ring, [0, 6], 16, rows)
+    plan = ops.page_plan(*dev, 16, rows=rows)
+    assert plan.status.item() & getattr(N, "PLAN_" + bits)
+    for name, values in want.items():
+        assert getattr(plan, name).tolist() == values, name
+    assert dev[2].tolist() == table and dev[3].tolist() == ring
+
+
 def test_plan_into_unaligned_buffers(ops):
     lengths, grow = [3, 100, 0, 16], [1, 1, 90, 40]
     rows = 137

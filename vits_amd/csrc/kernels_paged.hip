@@ -26,9 +26,12 @@ constexpr int PLAN_ROWS = 1024;              // rows of a block: four consecutiv
 constexpr int PLAN_SHARE = 32;               // requests whose lengths and returned pages a block writes, at most: its four waves
                                              // return pages a request at a time
 
+// Sums that stop at 2^31 - 1: beyond any number of rows or pages that a call may have, so a step that is too large is found
+// out without a second word for each sum.
 struct PlanSums {
-  long long rows, fresh, back;
+  unsigned rows, fresh, back;
 };
+__device__ __forceinline__ unsigned plan_add(unsigned a, unsigned b) { return min(a + b, 0x7fffffffu); }
 // a request's share of them, and the pages it holds before and after
 struct PlanOf {
   unsigned rows, held, after;
@@ -50,6 +53,8 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PagePlanArgs a)
   const int each = (a.requests + PLAN_THREADS - 1) / PLAN_THREADS;
   const int s0 = min(tid * each, a.requests), s1 = min(s0 + each, a.requests);
 
+  const long long head = a.cursor[0], tail = a.cursor[1], free_pages = tail - head;
+
   // pass 1: this thread's requests
   PlanSums mine = {0, 0, 0};
   int bad = 0;
@@ -58,37 +63,37 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PagePlanArgs a)
     if (len < 0 || g < -1 || (g > 0 && len > 0x7fffffff - g)) { bad |= VITS_PLAN_BAD_LENGTH; continue; }
     const PlanOf p = plan_of(len, g, page);
     if (p.after > (unsigned)a.width) bad |= VITS_PLAN_TABLE_FULL;
-    mine.rows += p.rows; mine.fresh += p.fresh(); mine.back += p.back(g);
+    mine = PlanSums{plan_add(mine.rows, p.rows), plan_add(mine.fresh, p.fresh()), plan_add(mine.back, p.back(g))};
   }
   PlanSums upto = mine;                      // inclusive over the wave
 #pragma unroll
   for (int d = 1; d < WAVE; d <<= 1) {
-    const long long r = __shfl_up(upto.rows, d, WAVE), f = __shfl_up(upto.fresh, d, WAVE), b = __shfl_up(upto.back, d, WAVE);
-    if (lane >= d) { upto.rows += r; upto.fresh += f; upto.back += b; }
+    const unsigned r = __shfl_up(upto.rows, d, WAVE), f = __shfl_up(upto.fresh, d, WAVE), b = __shfl_up(upto.back, d, WAVE);
+    if (lane >= d) upto = PlanSums{plan_add(upto.rows, r), plan_add(upto.fresh, f), plan_add(upto.back, b)};
     bad |= __shfl_xor(bad, d, WAVE);
   }
   if (lane == WAVE - 1) { wave_sum[wave] = upto; wave_bad[wave] = bad; }
   for (int i = tid; i < PLAN_ROWS; i += PLAN_THREADS) mark[i] = -1;
   if (tid == 0) n_gone = 0;
   __syncthreads();
-  PlanSums total = {0, 0, 0}, before = {upto.rows - mine.rows, upto.fresh - mine.fresh, upto.back - mine.back};
+  PlanSums total = {0, 0, 0}, before = {upto.rows - mine.rows, upto.fresh - mine.fresh, upto.back - mine.back};   // of use if none stopped
   bad = 0;
 #pragma unroll
   for (int w = 0; w < PLAN_THREADS / WAVE; ++w) {
-    if (w < wave) { before.rows += wave_sum[w].rows; before.fresh += wave_sum[w].fresh; before.back += wave_sum[w].back; }
-    total.rows += wave_sum[w].rows; total.fresh += wave_sum[w].fresh; total.back += wave_sum[w].back;
+    const PlanSums x = wave_sum[w];
+    if (w < wave) before = PlanSums{before.rows + x.rows, before.fresh + x.fresh, before.back + x.back};
+    total = PlanSums{plan_add(total.rows, x.rows), plan_add(total.fresh, x.fresh), plan_add(total.back, x.back)};
     bad |= wave_bad[w];
   }
-  const long long head = a.cursor[0], tail = a.cursor[1], free_pages = tail - head;
   if (head < 0 || free_pages < 0 || free_pages > a.pages || free_pages + total.back > a.pages) bad |= VITS_PLAN_BAD_RING;
-  if (total.rows > a.rows) bad |= VITS_PLAN_ROWS_FULL;
+  if (total.rows > (unsigned)a.rows) bad |= VITS_PLAN_ROWS_FULL;
   if (total.fresh > free_pages) bad |= VITS_PLAN_NO_PAGES;
   // (a counter of less than 2^32 pages is divided in 32 bits: 64 take a long routine)
   auto place_of = [&](long long c) { return bad ? 0 : c >> 32 ? (int)(c % a.pages) : (int)((unsigned)c % (unsigned)a.pages); };
   const int ring0 = place_of(head), ring1 = place_of(tail);
 
   // pass 2: mark where requests begin in this block's rows; write what belongs to this block's share of the requests
-  const int row0 = blockIdx.x * PLAN_ROWS;
+  const unsigned row0 = blockIdx.x * PLAN_ROWS;           // below 2^30 + PLAN_ROWS
   const int share = (a.requests + gridDim.x - 1) / gridDim.x, own0 = blockIdx.x * share, own1 = own0 + share;   // at most PLAN_SHARE
   for (int s = s0; s < s1; ++s) {
     const int len = a.lengths[s], g = a.grow[s];
@@ -106,14 +111,14 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PagePlanArgs a)
         gone[n] = s; gone_held[n] = (int)p.held; gone_at[n] = (int)before.back;
       }
     }
-    if (p.rows > 0 && before.rows < (long long)row0 + PLAN_ROWS && before.rows + p.rows > row0) {
+    if (p.rows > 0 && before.rows < row0 + PLAN_ROWS && before.rows + p.rows > row0) {
       const int at = before.rows > row0 ? (int)(before.rows - row0) : 0;
       mark[at] = s;
       m_base[at] = len - (int)before.rows;
       m_held[at] = (int)p.held;
       m_fresh[at] = (int)before.fresh;
     }
-    before.rows += p.rows; before.fresh += p.fresh(); before.back += p.back(g);
+    before = PlanSums{before.rows + p.rows, before.fresh + p.fresh(), before.back + p.back(g)};
   }
   if (blockIdx.x == 0 && tid == 0) {
     a.row_start[a.requests] = bad ? 0 : (int)total.rows;
@@ -919,7 +924,7 @@ __device__ __forceinline__ bool att_part(const PagedAttArgs& a, const AttPlan& p
 __device__ __forceinline__ void att_flag_row(const PagedAttArgs& a, int row) {
   const int req = a.row_request[row];
   int b, e;
-  if (a.err_flag && (req >= a.requests || (req >= 0 && att_row_keys(a, row, b, e)))) atomicOr(a.err_flag, 1);
+  if (req >= a.requests || (req >= 0 && att_row_keys(a, row, b, e))) atomicOr(a.err_flag, 1);
 }
 
 // Joins a block's parts of one unit, N of them in LDS (those that are none have a null pointer), a thread a quad of channels.
@@ -977,10 +982,10 @@ __global__ __launch_bounds__(ATT_THREADS, 2) void paged_attention_wave_kernel(Pa
   const long long n = (long long)blockIdx.x * ATT_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int row = (int)att_div(n, p.units), unit = (int)(n - (long long)row * p.units);
   if (row >= a.rows) return;
-  if (unit == 0 && threadIdx.x % WAVE == 0) att_flag_row(a, row);
   Run r;
   if (att_run_wave(a, p, row, r) && att_part<T, DIM>(a, p, r, unit, 0, att_run_steps<AttTile<T, DIM>::STEP>(r), true, nullptr) && a.err_flag)
     atomicOr(a.err_flag, 1);
+  if (a.err_flag && unit == 0 && threadIdx.x % WAVE == 0) att_flag_row(a, row);
 }
 
 // A block a unit, its waves a stretch of the keys each, joined in LDS: for fewer units of such lengths.
@@ -988,8 +993,8 @@ template <typename T, int DIM>
 __global__ __launch_bounds__(ATT_BLOCK_WAVES * WAVE, 1) void paged_attention_block_kernel(PagedAttArgs a, AttPlan p) {
   __shared__ alignas(16) float lds[ATT_BLOCK_WAVES][ATT_COLS * AttTile<T, DIM>::ROW];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-  const int row = blockIdx.x / p.units, unit = blockIdx.x - row * p.units;
-  if (unit == 0 && threadIdx.x == 0) att_flag_row(a, row);
+  const int row = blockIdx.x / (unsigned)p.units, unit = blockIdx.x - row * p.units;
+  if (a.err_flag && unit == 0 && threadIdx.x == 0) att_flag_row(a, row);
   Run r;
   if (!att_run_wave(a, p, row, r)) return;
   const int steps = att_run_steps<AttTile<T, DIM>::STEP>(r);
@@ -1025,7 +1030,7 @@ __global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attenti
   Run r;
   for (int row = row0; row < row1; ++row) {
     if (att_run(a, p, row, r)) mine += att_run_steps<STEP>(r);
-    if (blockIdx.x == 0) att_flag_row(a, row);
+    if (a.err_flag && blockIdx.x == 0) att_flag_row(a, row);
   }
   long long upto = mine;
 #pragma unroll
@@ -1143,12 +1148,20 @@ __global__ __launch_bounds__(ATT_THREADS) void paged_join_kernel(PagedAttArgs a,
     const bool real = att_column(m, j.n, p.group, j.unit - hk * p.tiles, row, head);
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     float top = -INFINITY, base = 0.f, sum = 0.f;
+    int from = 0, to = 0;
     if (real) {
+      att_row_keys(a, j.row + row, from, to);
       auto part = [&](int k) { return att_slot(ws, blockIdx.x + k, k == 0, a.dim) + m * ROW; };
       f32x4 v[AHEAD];
+      float v_top[AHEAD], v_sum[AHEAD];
       auto load = [&](int k0) {                            // what there is not is read from the last part, and has no weight
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) v[u] = *(const f32x4*)(part(min(k0 + u * at_once + mine, parts - 1)) + 4 * quad);
+        for (int u = 0; u < AHEAD; ++u) {
+          const float* from = part(min(k0 + u * at_once + mine, parts - 1));
+          v[u] = *(const f32x4*)(from + 4 * quad);
+          v_top[u] = from[a.dim];
+          v_sum[u] = from[a.dim + 1];
+        }
       };
       load(0);
       for (int k = me % WAVE; k < parts; k += WAVE) top = fmaxf(top, part(k)[a.dim]);
@@ -1160,11 +1173,11 @@ __global__ __launch_bounds__(ATT_THREADS) void paged_join_kernel(PagedAttArgs a,
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
           const int k = k0 + u * at_once + mine;
-          if (mine < at_once && k < parts) {
-            const float g = att_exp2(part(k)[a.dim] - base);
-            if (quad == 0) sum += g * part(k)[a.dim + 1];
-            x += g * v[u];
-          }
+          const bool there = mine < at_once && k < parts;
+          const float g = att_exp2(v_top[u] - base);
+          sum += there && quad == 0 ? g * v_sum[u] : 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] += there ? g * v[u][e] : 0.f;
         }
       }
 #pragma unroll
@@ -1180,8 +1193,6 @@ __global__ __launch_bounds__(ATT_THREADS) void paged_join_kernel(PagedAttArgs a,
         sum = 0.f;
         for (int w = 0; w < ATT_WAVES; ++w) sum += wave_sum[w];
       }
-      int from, to;
-      att_row_keys(a, j.row + row, from, to);
       att_write<T>(a, p.wide_out, j.row + row, hk * p.group + head, 4 * quad, x, sum, from >= to);
       if (a.lse && quad == 0) att_write_lse(a, j.row + row, hk * p.group + head, top, sum, from >= to);
     }
@@ -1221,16 +1232,16 @@ AttPlan att_plan(int rows, int heads, int kv_heads, int dim, int dtype, long lon
 
 template <typename T, int DIM>
 hipError_t start_attention(const PagedAttArgs& a, const AttPlan& p, AttForm form, void* ws, hipStream_t s) {
-  const unsigned units = (unsigned)a.rows * p.units;
+  const long long units = (long long)a.rows * p.units;      // below 2^22 where a grid is made of it
   if (form == ATT_WAVE) {
-    hipLaunchKernelGGL((paged_attention_wave_kernel<T, DIM>), dim3((units + ATT_WAVES - 1) / ATT_WAVES), dim3(ATT_THREADS), 0, s, a, p);
+    hipLaunchKernelGGL((paged_attention_wave_kernel<T, DIM>), dim3((unsigned)((units + ATT_WAVES - 1) / ATT_WAVES)), dim3(ATT_THREADS), 0, s, a, p);
   } else if (form == ATT_BLOCK) {
-    hipLaunchKernelGGL((paged_attention_block_kernel<T, DIM>), dim3(units), dim3(ATT_BLOCK_WAVES * WAVE), 0, s, a, p);
+    hipLaunchKernelGGL((paged_attention_block_kernel<T, DIM>), dim3((unsigned)units), dim3(ATT_BLOCK_WAVES * WAVE), 0, s, a, p);
   } else {
     const int blocks = p.pieces / ATT_WAVES;
     AttJoin* joins = (AttJoin*)att_slot((float*)ws, blocks, 0, DIM);
     hipLaunchKernelGGL((paged_attention_split_kernel<T, DIM>), dim3(blocks), dim3(ATT_THREADS), 0, s, a, p, (float*)ws, joins);
-    const int cols = min(ATT_COLS, p.group << p.run_shift), each = units > ATT_FEW ? ATT_WAVES : 1;
+    const int cols = min(ATT_COLS, p.group * min(1 << p.run_shift, a.rows)), each = units > ATT_FEW ? ATT_WAVES : 1;
     hipLaunchKernelGGL((paged_join_kernel<T>), dim3(blocks, (cols + each - 1) / each), dim3(ATT_THREADS), 0, s, a, p, (float*)ws, joins, each);
   }
   return hipGetLastError();
