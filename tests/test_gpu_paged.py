@@ -636,6 +636,30 @@ def test_attention_large_scores(ops, dtype):
     check_attention(ops, cache, q, [0], [299])
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_attention_of_many_small_weights(ops, dtype):
+    """A first key of weight 1 and 10^5 more of e^-17.75 = 2^-25.6 each, less than fp16's least number: together they are 2e-3 of
+    the sum.  n roundings follow each other in a sum (16 adds of a lane, its column, four waves, 391 blocks: below 450), on
+    both sides of the division."""
+    t, n, dim = TYPES[dtype], 100000, 32
+    cache = Cache(t, [0], 1, dim, 16, seed=22, width=n // 16 + 1, spare=n // 16 + 1)
+    cache.table.copy_(torch.randperm(cache.pages, device="cuda").to(torch.int32)[None])
+    k, v = torch.zeros(n, 1, dim, dtype=t, device="cuda"), torch.full((n, 1, dim), -1.0, dtype=t, device="cuda")
+    k[1:, :, 0] = -17.75
+    v[0] = 1.0
+    slot = cache.table[0].long()[torch.arange(n, device="cuda") // 16] * 16 + torch.arange(n, device="cuda") % 16
+    ops.rotary_store(None, k, v, cache.k_cache, cache.v_cache, torch.zeros(n, dtype=torch.int32, device="cuda"), slot, ops.rotary_frequencies(dim))
+    q = torch.zeros(1, 1, dim, dtype=t, device="cuda")
+    q[..., 0] = 1.0
+    lse = torch.empty(1, 1, device="cuda")
+    out = ops.paged_attention(q, cache.k_cache, cache.v_cache, cache.table, gpu_i32([0]), gpu_i32([n - 1]), scale=1.0, lse=lse).double().cpu()
+    rest = (n - 1) * math.exp(-17.75)
+    ref = torch.full((1, 1, dim), (1 - rest) / (1 + rest), dtype=torch.float64)
+    near = 2 * (dim + 4) * 2.0 ** -24 * 17.75 + 2.0 ** -19 + 2 * 450 * 2.0 ** -24 + {"fp32": 0.0, "fp16": 2.0 ** -21, "bf16": 2.0 ** -16}[dtype]
+    assert bool(((out - ref).abs() <= half_step(ref, t) + near).all()), (out[0, 0, 0].item(), ref[0, 0, 0].item())
+    assert abs(lse.item() - math.log1p(rest)) <= near
+
+
 def test_attention_ids_outside(ops):
     """Pages outside the cache are left out, requests and positions outside the table not followed; the flag says so."""
     t = torch.bfloat16

@@ -397,7 +397,6 @@ constexpr int ATT_PIECES = 2048;             // the most pieces a call's work is
 constexpr int ATT_MIN_STEPS = 2;             // the least a piece holds
 constexpr int ATT_FEW = 32;                  // units up to which a join takes a block a column
 constexpr int ATT_BLOCK_WAVES = 8;           // waves that take a unit by themselves
-constexpr float ATT_SLACK = 8.f;             // the running maximum follows once it is exceeded by 2^8: weights stay below 256
 
 // max and sum over the four lanes of a column (lane, lane ^ 16, lane ^ 32, lane ^ 48)
 __device__ __forceinline__ float col_max(float x) {
@@ -546,6 +545,11 @@ struct AttTile {
   static constexpr int VW = CH * (int)sizeof(T) / 4;     // dwords of a lane for one row of V
   static constexpr int VP = VW / PASSES;
   static constexpr int ROW = DIM + 4;                   // floats of a column in LDS and in the workspace, padded
+  // The running maximum follows once it is exceeded by 2^SLACK.  fp16 holds nothing below 2^-24, and a long context may have most of its
+  // sum in weights below that: there the maximum stands for a weight of 2^LIFT (the largest, 2^15, is still one), so the smallest
+  // that counts is 2^-35 of it.
+  static constexpr bool F16 = __is_same(T, _Float16);
+  static constexpr float SLACK = F16 ? 4.f : 8.f, LIFT = F16 ? 11.f : 0.f;
   static_assert(KL % PASSES == 0 && VW % PASSES == 0);
 
   u32x4 q[KL], k[SUB][KP];
@@ -682,7 +686,7 @@ struct AttTile {
 #pragma unroll
       for (int e = 0; e < 4; ++e) t = fmaxf(t, s[u][e]);
     t = col_max(t);
-    const bool above = t > top + ATT_SLACK;
+    const bool above = t > top + SLACK;
     if (__ballot(above)) {                              // seldom after the first steps
       const float next = above ? t : top;               // a column goes by its own scores alone
       const float keep = above ? att_exp2(top - next) : 1.f;
@@ -691,7 +695,7 @@ struct AttTile {
       for (int c = 0; c < CH; ++c) o[c] *= keep;
       top = next;
     }
-    const float base = top == -INFINITY ? 0.f : top;
+    const float base = top == -INFINITY ? 0.f : top - LIFT;
 #pragma unroll
     for (int u = 0; u < SUB; ++u)
 #pragma unroll
@@ -904,6 +908,7 @@ __device__ __forceinline__ bool att_part(const PagedAttArgs& a, const AttPlan& p
 #pragma unroll
     for (int c = 0; c < CH; ++c) ATT_SETTLE(w.o[c]);
     w.sum = col_sum(w.sum);
+    w.top -= Tile::LIFT;                                  // from here on what a weight of 1 stands for
     if (alone < 0 && r.n > 1) {
       bool wild = false;
 #pragma unroll
