@@ -710,6 +710,19 @@ def test_attention_far_pages(ops):
     assert bool(((out[0].double().cpu() - ref).abs() <= tol).all())
 
 
+def test_attention_of_single_pages_and_requests(ops):
+    """The strides of dimensions of one element are of no consequence."""
+    t = torch.float16
+    cache = Cache(t, [11], 1, 64, 16, seed=23, spare=0)
+    q = rows_q(cache, 1, 4, 64, t)
+    ref, _, tol, _ = attend_by_hand(q[0], cache.k[0], cache.v[0], 10, 1 / 8, 0)
+    shape = (1, 1, 16, 64)
+    for stride in ((0, 1024, 64, 1), (1024, 5, 64, 1), (7, 0, 64, 1)):
+        k, v = (c.as_strided(shape, stride) for c in (cache.k_cache, cache.v_cache))
+        out = ops.paged_attention(q.as_strided((1, 4, 64), (3, 64, 1)), k, v, cache.table.t(), gpu_i32([0]), gpu_i32([10]))
+        assert bool(((out[0].double().cpu() - ref).abs() <= tol).all()), stride
+
+
 def test_attention_python_refusals(ops):
     cache = Cache(torch.bfloat16, [30], 2, 64, 16, seed=16)
     q = rows_q(cache, 2, 4, 64, torch.bfloat16)
@@ -823,6 +836,38 @@ def test_calls_on_other_streams(ops):
     for i in range(2):
         for o in got[i]:
             assert torch.equal(o, alone[i])
+
+
+def test_captured_calls_have_their_own_workspaces(ops):
+    """Two graphs of calls that cut their work into pieces, replayed one after the other and side by side with eager calls between."""
+    cache = Cache(torch.bfloat16, [9000, 700], 2, 64, 16, seed=24)
+    request, position = gpu_i32([0, 1]), gpu_i32([8999, 699])
+    qs = [rows_q(cache, 2, 8, 64, torch.bfloat16) for _ in range(3)]
+    call = lambda q, out: ops.paged_attention(q, cache.k_cache, cache.v_cache, cache.table, request, position, out=out)      # noqa: E731
+    alone = [call(q, torch.empty_like(q)) for q in qs]
+    outs = [torch.empty_like(q) for q in qs]
+    torch.cuda.synchronize()
+    graphs = []
+    for q, out in zip(qs[:2], outs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call(q, out)
+            call(q, out)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for n in range(8):
+        for out in outs:
+            out.fill_(n)
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            if n % 2:
+                with torch.cuda.stream(s):
+                    g.replay()
+            else:
+                g.replay()
+        call(qs[2], outs[2])
+        torch.cuda.synchronize()
+        for out, want in zip(outs, alone):
+            assert torch.equal(out, want)
 
 
 def test_the_same_call_gives_the_same_bytes(ops):

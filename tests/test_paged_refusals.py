@@ -177,3 +177,31 @@ def test_rotary_frequencies():
                 dict(rotary_dim=8, scaling="other"), dict(rotary_dim=8, scaling="ramp", fast=1.0, slow=1.0), dict(rotary_dim=8, factor=math.nan)):
         with pytest.raises(ValueError):
             ops.rotary_frequencies(**bad, device="cpu")
+
+
+def test_gradients_are_refused_not_dropped():
+    q, cache, v = torch.zeros(2, 4, 64), torch.zeros(5, 2, 2, 16, 64), torch.zeros(2, 2, 64)
+    at = dict(position=i32(3, 4))
+    attention = dict(q=q, k_cache=cache[:, 0], v_cache=cache[:, 1], table=torch.zeros(3, 4, dtype=torch.int32), request=i32(0, 1), **at)
+    rotary = dict(q=q, k=v, v=v, k_cache=cache[:, 0], v_cache=cache[:, 1], slot=torch.arange(2), freq=ops.rotary_frequencies(64, device="cpu"), **at)
+    for call, good, names in ((ops.paged_attention, attention, ("q", "k_cache")), (ops.rotary_store, rotary, ("q", "k", "v"))):
+        for name in names:
+            asks = {**good, name: good[name].detach().clone(memory_format=torch.preserve_format).requires_grad_()}
+            if name == "k_cache":
+                asks = {**good, name: cache.clone().requires_grad_()[:, 0]}
+            with pytest.raises(ValueError, match="gradient"):
+                call(**asks)
+            with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+                call(**asks)
+
+
+def test_strides_of_single_dimensions_say_nothing():
+    """One page, one key-value head, one request: views whose stride there is any number are taken (up to the check for a GPU)."""
+    def single(shape, stride):
+        return torch.zeros(4096 * 4).as_strided(shape, stride)
+    q, at = torch.zeros(2, 4, 64), i32(3, 4)
+    for shape, stride in (((1, 2, 16, 64), (0, 1024, 64, 1)), ((3, 1, 16, 64), (1024, 64, 64, 1)), ((1, 1, 16, 64), (7, 5, 64, 1))):
+        k, v = single(shape, stride), single(shape, stride)
+        for table in (torch.zeros(1, 3, dtype=torch.int32), torch.zeros(3, 1, dtype=torch.int32).t()):
+            with pytest.raises(ValueError, match="GPU"):
+                ops.paged_attention(q, k, v, table, i32(0, 0), at)

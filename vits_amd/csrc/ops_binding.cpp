@@ -4,6 +4,7 @@
 // interface and its documentation; it passes the current stream and makes the tensors' GPU the current one.
 #include <Python.h>
 
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -72,7 +73,7 @@ void rows_of(const Tensor& t, at::ScalarType type, int64_t rows, int64_t heads, 
 
 void caches_of(const Tensor& k, const Tensor& v, const char* what) {
   const bool alike = k.dim() == 4 && v.scalar_type() == k.scalar_type() && v.sizes() == k.sizes() && v.strides() == k.strides();
-  if (!alike || k.stride(3) != 1 || k.stride(2) != k.size(3) || k.stride(1) != k.size(2) * k.size(3))
+  if (!alike || k.stride(3) != 1 || k.stride(2) != k.size(3) || (k.stride(1) != k.size(2) * k.size(3) && k.size(1) > 1))
     throw Refused{std::string(what) + ": k_cache and v_cache must be alike, [pages, kv_heads, page_size, dim], and contiguous within a page, got " +
                   describe(k) + " and " + describe(v)};
 }
@@ -80,6 +81,17 @@ void caches_of(const Tensor& k, const Tensor& v, const char* what) {
 void table_of(const Tensor& t, const char* what) {
   if (t.scalar_type() != at::kInt || t.dim() != 2 || (t.stride(1) != 1 && t.size(1) > 1))
     throw Refused{std::string(what) + ": table must be int32 [requests, width] with contiguous rows, got " + describe(t)};
+}
+
+// (the stride of a dimension of one element says nothing)
+int64_t page_stride(const Tensor& cache) { return cache.size(0) > 1 ? cache.stride(0) : cache.size(1) * cache.size(2) * cache.size(3); }
+int64_t table_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+void no_grad(const char* what, std::initializer_list<const Tensor*> values) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : values)
+    if (t && t->requires_grad())
+      throw Refused{std::string(what) + ": records no gradient: call it under torch.no_grad() (or on detached tensors)"};
 }
 
 void on_gpu(const char* what, const Tensor& first, std::initializer_list<const Tensor*> more) {
@@ -150,7 +162,7 @@ PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
       flat(*out[i], i == 1 || i == 5 ? at::kLong : at::kInt, sizes[i], what, names[i]);
     }
     on_gpu(what, lengths, {&grow, &table, &ring, &cursor, out[0], out[1], out[2], out[3], out[4], out[5], out[6]});
-    return done(plan_fn((int*)lengths.data_ptr(), (int*)grow.data_ptr(), narrow(requests, what), (int*)table.data_ptr(), table.stride(0),
+    return done(plan_fn((int*)lengths.data_ptr(), (int*)grow.data_ptr(), narrow(requests, what), (int*)table.data_ptr(), table_stride(table),
                         narrow(table.size(1), what), (int*)ring.data_ptr(), narrow(ring.numel(), what), (int64_t*)cursor.data_ptr(),
                         integer32(a[5], what), (int*)out[0]->data_ptr(), (int64_t*)out[1]->data_ptr(), (int*)out[2]->data_ptr(),
                         (int*)out[3]->data_ptr(), (int*)out[4]->data_ptr(), (int64_t*)out[5]->data_ptr(), narrow(rows, what),
@@ -189,10 +201,11 @@ PyObject* rotary_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (kc->scalar_type() != first.scalar_type() || kc->size(3) != dim)
         throw Refused{"rotary_store: the caches' type and channels are not the rows': " + describe(*kc) + " and " + describe(first)};
     }
+    no_grad(what, {q, k, v, kc, vc, out});
     on_gpu(what, first, {k, v, kc, vc, slot, out, flag, &position, &freq});
     return done(rotary_fn(at_(q), q ? q->stride(0) : 0, q ? q->stride(1) : 0, at_(out), out ? out->stride(0) : 0, out ? out->stride(1) : 0,
                           narrow(heads, what), at_(k), k ? k->stride(0) : 0, k ? k->stride(1) : 0, at_(v), v ? v->stride(0) : 0,
-                          v ? v->stride(1) : 0, at_(kc), at_(vc), kc ? kc->stride(0) : 0, kc ? narrow(kc->size(0), what) : 0,
+                          v ? v->stride(1) : 0, at_(kc), at_(vc), kc ? page_stride(*kc) : 0, kc ? narrow(kc->size(0), what) : 0,
                           kc ? narrow(kc->size(2), what) : 0, kc ? narrow(kc->size(1), what) : 0, narrow(dim, what), type,
                           (int*)position.data_ptr(), (int64_t*)at_(slot), narrow(rows, what), (double*)freq.data_ptr(),
                           narrow(freq.numel(), what), (float)real(a[9]), PyObject_IsTrue(a[8]) > 0, (int*)at_(flag), address(a[12])),
@@ -219,6 +232,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (lse && (lse->dim() != 2 || lse->size(0) != rows || lse->size(1) != heads || lse->scalar_type() != at::kFloat || !lse->is_contiguous()))
       throw Refused{"paged_attention: lse must be contiguous float32 [rows, heads], got " + describe(*lse)};
     if (flag) flat(*flag, at::kInt, 1, what, "err_flag");
+    no_grad(what, {&q0, &kc, &vc, &out});
     on_gpu(what, q0, {&kc, &vc, &table, &request, &position, &out, lse, flag});
     const int64_t size = q0.element_size();
     const bool aligned = ((uintptr_t)q0.data_ptr() | (uintptr_t)(q0.stride(0) * size) | (uintptr_t)(q0.stride(1) * size)) % 16 == 0;
@@ -233,8 +247,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     // a workspace of this call's own: calls on different streams, and graphs that run side by side, share none
     Tensor ws;
     if (bytes) ws = at::empty({bytes}, q0.options().dtype(at::kByte));
-    return done(attention_fn(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(), kc.stride(0), narrow(kc.size(0), what),
-                             narrow(kc.size(2), what), (int*)table.data_ptr(), table.stride(0), narrow(table.size(1), what),
+    return done(attention_fn(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(), page_stride(kc), narrow(kc.size(0), what),
+                             narrow(kc.size(2), what), (int*)table.data_ptr(), table_stride(table), narrow(table.size(1), what),
                              narrow(table.size(0), what), (int*)request.data_ptr(), (int*)position.data_ptr(), r, h, hk, d, type,
                              (float)real(a[6]), window, keys, out.data_ptr(), out.stride(0), out.stride(1), (float*)at_(lse), (int*)at_(flag),
                              bytes ? ws.data_ptr() : nullptr, bytes, address(a[12])),
