@@ -292,6 +292,54 @@ def test_rotary_store(ops, dtype, interleaved, rows, hq, hk, dim, rot, layout):
     assert torch.equal(cache, before)                                                  # no other cell was written
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("rows,hq,hk,dim,rot,layout", [(1, 96, 8, 96, 96, "own"), (2, 64, 8, 192, 182, "odd"), (3, 40, 8, 256, 2, "fused"),
+                                                       (300, 5, 5, 34, 22, "odd"), (1100, 32, 8, 64, 54, "fused")])
+def test_rotary_store_in_slices(ops, dtype, interleaved, rows, hq, hk, dim, rot, layout):
+    """A row's items over several blocks, several rows a block, heads that end beside 16 bytes; in place, with slots outside the
+    cache: those rows' queries stay too, and the flag says so."""
+    t = TYPES[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(rows + dim)
+    q, k, v = make_rows(t, rows, hq, hk, dim, layout, gen)
+    page, pages = 32, rows // 32 + 2
+    k_cache, v_cache = (torch.randn(pages, hk, page, dim, generator=gen, device="cuda").to(t) for _ in range(2))
+    position = torch.randint(0, 2 ** 20, (rows,), generator=gen, dtype=torch.int32, device="cuda")
+    slot = torch.randperm(pages * page, generator=gen, device="cuda")[:rows]
+    if rows > 1:
+        slot[rows // 2] = pages * page
+    freq, flag, live = ops.rotary_frequencies(rot), gpu_i32([0]), (slot < pages * page).cpu()
+    old, parts = q.clone(), (q, k, v)
+    turned = ops.rotary_store(*parts, k_cache, v_cache, position, slot, freq, interleaved=interleaved, out=q, err_flag=flag)
+    assert turned is q and flag.item() == (rows > 1)
+    ref, size = rotate_by_hand(old, position, freq, interleaved, 1.0)
+    near_rotation(q[live], ref[live], size[live], t)
+    assert torch.equal(q[..., rot:], old[..., rot:]) and torch.equal(q[~live], old[~live])
+    s = slot[live]
+    ref, size = rotate_by_hand(k, position, freq, interleaved, 1.0)
+    near_rotation(k_cache[s // page, :, s % page], ref[live], size[live], t)
+    assert torch.equal(v_cache[s // page, :, s % page], v[live])
+
+
+def test_rotary_store_many_items(ops):
+    """So many that a thread takes several, over ragged heads off the 16-byte addresses: the same bits as for few rows at a time."""
+    gen = torch.Generator(device="cuda").manual_seed(31)
+    rows, hq, hk, dim, rot, page = 4000, 40, 8, 66, 54, 16
+    for t, interleaved in ((torch.float32, False), (torch.bfloat16, True)):
+        q, k, v = make_rows(t, rows, hq, hk, dim, "odd", gen)
+        caches = [torch.zeros(rows // page, hk, page, dim, dtype=t, device="cuda") for _ in range(4)]
+        position = torch.arange(rows, dtype=torch.int32, device="cuda") + 77
+        slot = torch.randperm(rows, generator=gen, device="cuda")
+        slot[5::7] = -1
+        freq = ops.rotary_frequencies(rot)
+        out = ops.rotary_store(q, k, v, caches[0], caches[1], position, slot, freq, interleaved=interleaved)
+        for i in range(0, rows, 500):
+            part = slice(i, i + 500)
+            few = ops.rotary_store(q[part], k[part], v[part], caches[2], caches[3], position[part], slot[part], freq, interleaved=interleaved)
+            assert torch.equal(few, out[part])
+        assert torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_rotary_parts_alone(ops, dtype):
     """Queries without keys (new, in place, strided out), keys without queries."""

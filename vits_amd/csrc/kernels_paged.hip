@@ -11,6 +11,9 @@ namespace {
 
 constexpr int WAVE = 64;
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 // ---------------------------------------------------------------------------------------------------------
 // page plan.  With a = max(grow, 0), held = ceil(length / page), fresh = ceil((length + a) / page) - held and back =
 // held of a request that ends, three prefix sums over the requests say which rows, which free pages and which ring
@@ -223,7 +226,7 @@ template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
 // cos and sin of position * freq, times scale.  A far position leaves fp32 no bits for the angle within its turn
 // (position 10^6: half a radian), so the product and the reduction to an eighth of a turn are in 64 bits; what is left
 // is rounded to fp32 once, where its error is 2^-24 of at most pi / 4.
-__device__ __forceinline__ void rotary_angle(int position, double freq, float scale, float& c, float& s) {
+__device__ __forceinline__ void rotary_angle(int position, double freq, float scale, f32x2& cs) {
   const double turns = (double)position * freq * 0.15915494309189533577;      // 1 / (2 pi)
   const double whole = rint(turns);
   const double part = turns - whole;                     // -1/2 .. 1/2
@@ -231,8 +234,8 @@ __device__ __forceinline__ void rotary_angle(int position, double freq, float sc
   float s0, c0;
   sincospif((float)((part - quarter * 0.25) * 2.0), &s0, &c0);
   const int k = (int)quarter & 3;
-  c = scale * (k == 0 ? c0 : k == 1 ? -s0 : k == 2 ? -c0 : s0);
-  s = scale * (k == 0 ? s0 : k == 1 ? c0 : k == 2 ? -s0 : -c0);
+  cs.x = scale * (k == 0 ? c0 : k == 1 ? -s0 : k == 2 ? -c0 : s0);
+  cs.y = scale * (k == 0 ? s0 : k == 1 ? c0 : k == 2 ? -s0 : -c0);
 }
 
 // written as products and sums of its own choice, so that every variant below gives the same bits
@@ -244,26 +247,50 @@ __device__ __forceinline__ void rotary_turn(float& u, float& w, float c, float s
 
 constexpr int ROT_THREADS = 256;
 
-// N channels an item: 16 bytes where sizes and addresses allow, else one.  An item that turns holds N channels of either
-// half in the half layout, N channels = N / 2 pairs in the interleaved one (and one pair where N is 1).
-template <typename T, int N, bool INTER>
-__global__ __launch_bounds__(ROT_THREADS) void rotary_store_kernel(RotaryArgs a, int rows_per_block) {
-  extern __shared__ float cs[];                          // [rows_per_block][pairs][2]
+// 16 bytes at the alignment of their values: global memory takes them at any address
+template <int ALIGN> struct AnyAt;
+template <> struct AnyAt<2> { typedef unsigned x4 __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct AnyAt<4> { typedef unsigned x4 __attribute__((ext_vector_type(4), aligned(4))); };
+
+// An item is 16 bytes of a head: N channels of both halves (half layout) or N / 2 pairs (interleaved) that turn, N channels
+// that pass through, N channels of a value.  RAGGED: not all of these are whole items; what is left of each goes one by one.
+struct RotaryPart {
+  int wide, all;                                         // whole items, and with the single ones
+  __host__ __device__ RotaryPart(int channels, int n, int unit) : wide(channels / n), all(channels / n + channels % n / unit) {}
+};
+
+// A block takes rows_per_block rows, or a slice of one row's items.
+template <typename T, bool INTER, bool RAGGED>
+__global__ __launch_bounds__(ROT_THREADS) void rotary_store_kernel(RotaryArgs a, int rows_per_block, int slice) {
+  constexpr int N = 16 / sizeof(T), TWO = INTER ? 2 : 1;
+  using At = AnyAt<sizeof(T)>;
+  extern __shared__ f32x2 cs[];                          // [rows_per_block][pairs]: cos and sin, and what a single item reads beyond
   const int tid = threadIdx.x;
   const int row0 = blockIdx.x * rows_per_block, rows = min(rows_per_block, a.rows - row0);
   for (int i = tid; i < rows * a.pairs; i += ROT_THREADS) {
     const int r = i / a.pairs, p = i % a.pairs;
-    rotary_angle(a.position[row0 + r], a.freq[p], a.scale, cs[2 * i], cs[2 * i + 1]);
+    rotary_angle(a.position[row0 + r], a.freq[p], a.scale, cs[i]);
   }
   __syncthreads();
-  const int turn = INTER && N > 1 ? 2 * a.pairs / N : a.pairs / N;   // items of a head that turn
-  const int pass = (a.dim - 2 * a.pairs) / N, whole = a.dim / N;     // ... that pass through; of a value head
-  const int per_head = turn + pass;
-  const int n_q = a.heads * per_head, n_k = a.kv_heads * per_head, n_v = a.kv_heads * whole;
-  const int per_row = n_q + n_k + n_v;
+  const RotaryPart turn(TWO * a.pairs, N, TWO), pass(a.dim - 2 * a.pairs, N, 1), whole(a.dim, N, 1);
+  const int n_turn = RAGGED ? turn.all : turn.wide, n_whole = RAGGED ? whole.all : whole.wide, per_head = n_turn + (RAGGED ? pass.all : pass.wide);
+  const int n_q = a.heads * per_head, n_k = a.kv_heads * per_head, per_row = n_q + n_k + a.kv_heads * n_whole;
+  const int first = blockIdx.y * slice, last = min(rows * per_row, first + slice);
   const int64_t slots = (int64_t)a.pages * a.page_size;
-  using P = Pack<T, N>;
-  for (int i = tid; i < rows * per_row; i += ROT_THREADS) {
+
+  auto load = [](const T* src, bool one) {
+    u32x4 x = {0, 0, 0, 0};
+    if (!RAGGED || !one) x = *(const typename At::x4*)src;
+    else if constexpr (sizeof(T) == 4) x[0] = *(const unsigned*)src;
+    else x[0] = *(const unsigned short*)src;
+    return x;
+  };
+  auto store = [](T* dst, const u32x4& x, bool one) {
+    if (!RAGGED || !one) *(typename At::x4*)dst = x;
+    else if constexpr (sizeof(T) == 4) *(unsigned*)dst = x[0];
+    else *(unsigned short*)dst = (unsigned short)x[0];
+  };
+  for (int i = first + tid; i < last; i += ROT_THREADS) {
     const int r = i / per_row, row = row0 + r;
     int j = i - r * per_row;
     int64_t slot = a.slot ? a.slot[row] : 0;
@@ -274,11 +301,15 @@ __global__ __launch_bounds__(ROT_THREADS) void rotary_store_kernel(RotaryArgs a,
     }
     const int64_t pg = a.k ? slot / a.page_size : 0;
     const int64_t cell = pg * a.page_stride + (slot - pg * a.page_size) * a.dim;
+    // channel of item j of a part, and whether it is a single one
+    auto channel = [](int j, int wide, int unit) { return RAGGED && j >= wide ? wide * N + (j - wide) * unit : j * N; };
     if (j >= n_q + n_k) {
       j -= n_q + n_k;
-      const int h = j / whole, c = (j - h * whole) * N;
-      const T* src = (const T*)a.v + row * a.v_row + h * a.v_head + c;
-      *(P*)((T*)a.v_cache + cell + (int64_t)h * a.page_size * a.dim + c) = *(const P*)src;
+      const int h = j / n_whole;
+      j -= h * n_whole;
+      const int c = channel(j, whole.wide, 1);
+      const bool one = j >= whole.wide;
+      store((T*)a.v_cache + cell + (int64_t)h * a.page_size * a.dim + c, load((const T*)a.v + row * a.v_row + h * a.v_head + c, one), one);
       continue;
     }
     const T* src;
@@ -295,50 +326,48 @@ __global__ __launch_bounds__(ROT_THREADS) void rotary_store_kernel(RotaryArgs a,
       dst = (T*)a.k_cache + cell + (int64_t)h * a.page_size * a.dim;
     }
     j -= h * per_head;
-    if (j >= turn) {
-      const int c = 2 * a.pairs + (j - turn) * N;
-      *(P*)(dst + c) = *(const P*)(src + c);
+    if (j >= n_turn) {
+      j -= n_turn;
+      const int c = 2 * a.pairs + channel(j, pass.wide, 1);
+      const bool one = j >= pass.wide;
+      store(dst + c, load(src + c, one), one);
       continue;
     }
-    const float* ang = cs + (size_t)r * a.pairs * 2;
-    if constexpr (INTER && N == 1) {
-      float u = Conv<T>::to(src[2 * j]), w = Conv<T>::to(src[2 * j + 1]);
-      rotary_turn(u, w, ang[2 * j], ang[2 * j + 1]);
-      dst[2 * j] = Conv<T>::from(u);
-      dst[2 * j + 1] = Conv<T>::from(w);
-    } else if constexpr (INTER) {
-      P x = *(const P*)(src + j * N);
+    const int c = channel(j, turn.wide, TWO);
+    const bool one = j >= turn.wide;
+    const f32x2* ang = cs + r * a.pairs + c / TWO;
+    struct Values { T v[N]; };
+    Values x = __builtin_bit_cast(Values, load(src + c, one)), y = x;
+    if constexpr (!INTER) y = __builtin_bit_cast(Values, load(src + a.pairs + c, one));
+    else if (RAGGED && one) x.v[1] = src[c + 1];
 #pragma unroll
-      for (int e = 0; e < N / 2; ++e) {
-        float u = Conv<T>::to(x.v[2 * e]), w = Conv<T>::to(x.v[2 * e + 1]);
-        rotary_turn(u, w, ang[j * N + 2 * e], ang[j * N + 2 * e + 1]);
-        x.v[2 * e] = Conv<T>::from(u);
-        x.v[2 * e + 1] = Conv<T>::from(w);
-      }
-      *(P*)(dst + j * N) = x;
-    } else {
-      P x = *(const P*)(src + j * N), y = *(const P*)(src + a.pairs + j * N);
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        float u = Conv<T>::to(x.v[e]), w = Conv<T>::to(y.v[e]);
-        rotary_turn(u, w, ang[2 * (j * N + e)], ang[2 * (j * N + e) + 1]);
-        x.v[e] = Conv<T>::from(u);
-        y.v[e] = Conv<T>::from(w);
-      }
-      *(P*)(dst + j * N) = x;
-      *(P*)(dst + a.pairs + j * N) = y;
+    for (int e = 0; e < N / TWO; ++e) {
+      T &lo = x.v[TWO * e], &hi = INTER ? x.v[TWO * e + 1] : y.v[e];
+      float u = Conv<T>::to(lo), w = Conv<T>::to(hi);
+      rotary_turn(u, w, ang[e].x, ang[e].y);
+      lo = Conv<T>::from(u);
+      hi = Conv<T>::from(w);
     }
+    store(dst + c, __builtin_bit_cast(u32x4, x), one);
+    if constexpr (!INTER) store(dst + a.pairs + c, __builtin_bit_cast(u32x4, y), one);
+    else if (RAGGED && one) dst[c + 1] = x.v[1];
   }
 }
 
-template <typename T, int N, bool INTER>
+template <typename T, bool INTER, bool RAGGED>
 hipError_t start_rotary(const RotaryArgs& a, hipStream_t s) {
-  const int per_row = (a.heads + (a.k ? 2 * a.kv_heads : 0)) * (a.dim / N);
-  int rpb = per_row >= 1024 ? 1 : (1024 + per_row - 1) / per_row;    // about four items a thread
-  rpb = min(rpb, min(16, a.rows));
+  constexpr int N = 16 / sizeof(T);
+  const RotaryPart turn(INTER ? 2 * a.pairs : a.pairs, N, INTER ? 2 : 1), pass(a.dim - 2 * a.pairs, N, 1), whole(a.dim, N, 1);
+  const int per_row = (a.heads + a.kv_heads) * (turn.all + pass.all) + a.kv_heads * whole.all;
+  // Up to 2^21 items one a thread, beyond about four, for which the angles serve then.  (862 rows of 40 ragged heads of 192,
+  // 7e5 items: 8.1 us with one, 11.5 with four; 8192 rows of 40 heads of 128, 3.7e6 items: 50 us with one, 44 with four.)
+  const bool few = (long long)a.rows * per_row <= 1 << 21;
+  int rpb = min(min(16, a.rows), few ? max(1, ROT_THREADS / per_row) : (1024 + per_row - 1) / per_row);
   while (rpb > 1 && (a.rows + rpb - 1) / rpb < 256) rpb = (rpb + 1) / 2;   // few rows: spread them over the CUs
-  const size_t lds = (size_t)rpb * a.pairs * 2 * sizeof(float);      // at most 16 KiB
-  hipLaunchKernelGGL((rotary_store_kernel<T, N, INTER>), dim3((a.rows + rpb - 1) / rpb), dim3(ROT_THREADS), lds, s, a, rpb);
+  const int slices = few && rpb == 1 ? (per_row + ROT_THREADS - 1) / ROT_THREADS : 1;
+  const int slice = rpb == 1 ? (per_row + slices - 1) / slices : rpb * per_row;
+  const size_t lds = ((size_t)rpb * a.pairs * 2 + 2 * N) * sizeof(float);          // at most 16 KiB and a little
+  hipLaunchKernelGGL((rotary_store_kernel<T, INTER, RAGGED>), dim3((a.rows + rpb - 1) / rpb, slices), dim3(ROT_THREADS), lds, s, a, rpb, slice);
   return hipGetLastError();
 }
 
@@ -347,18 +376,9 @@ hipError_t start_rotary_t(RotaryArgs a, hipStream_t s) {
   constexpr int N = 16 / sizeof(T);
   if (!a.k) a.kv_heads = 0;
   if (!a.q) a.heads = 0;
-  // sixteen-byte items need halves (or pairs) and rests in whole items, and every row and head on a 16-byte address
-  bool wide = a.dim % N == 0 && (a.interleaved ? 2 * a.pairs : a.pairs) % N == 0;
-  auto on16 = [&](const void* p, long long row, long long head) {
-    wide = wide && reinterpret_cast<uintptr_t>(p) % 16 == 0 && row % N == 0 && head % N == 0;
-  };
-  if (a.q) { on16(a.q, a.q_row, a.q_head); on16(a.out, a.out_row, a.out_head); }
-  if (a.k) {
-    on16(a.k, a.k_row, a.k_head); on16(a.v, a.v_row, a.v_head);
-    on16(a.k_cache, a.page_stride, 0); on16(a.v_cache, a.page_stride, 0);
-  }
-  if (a.interleaved) return wide ? start_rotary<T, N, true>(a, s) : start_rotary<T, 1, true>(a, s);
-  return wide ? start_rotary<T, N, false>(a, s) : start_rotary<T, 1, false>(a, s);
+  const bool ragged = a.dim % N || (a.interleaved ? 2 * a.pairs : a.pairs) % N || (a.dim - 2 * a.pairs) % N;
+  if (a.interleaved) return ragged ? start_rotary<T, true, true>(a, s) : start_rotary<T, true, false>(a, s);
+  return ragged ? start_rotary<T, false, true>(a, s) : start_rotary<T, false, false>(a, s);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -377,7 +397,6 @@ hipError_t start_rotary_t(RotaryArgs a, hipStream_t s) {
 // one rounding only, its own: the products' matrix time is a small part of the load time.
 // ---------------------------------------------------------------------------------------------------------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x3a __attribute__((ext_vector_type(3), aligned(4)));
 typedef unsigned u32x2a __attribute__((ext_vector_type(2), aligned(4)));
 typedef unsigned u32x4a __attribute__((ext_vector_type(4), aligned(4)));
@@ -387,7 +406,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int ATT_WAVES = 4;
