@@ -329,9 +329,11 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
  * h / (heads / kv_heads).  A row that sees no token (position < 0) gives 0.  lse [rows][heads] fp32 or NULL: log of the sum
  * of exp(scale * q . k_t), -inf for such a row.  Scores, softmax and sums in fp32.  What lies in the cache behind a row's
  * position, and in pages the table does not name for it, has no influence whatever it holds.
- * dim: 32, 64, ... 256; at most 2^23 rows and, by the table, 2^30 tokens a request; caches, pages and the heads of q begin on 16-byte addresses.  max_keys: how many tokens the host knows a row to see
- * at most (0: unknown; a window bounds it too); it only guides how the work is split, a row that sees more is right all
- * the same.  ws: vits_op_paged_attention_workspace_bytes of the same numbers (-1 for a shape that is refused). */
+ * dim: 32, 64, ... 256; at most 2^23 rows and, by the table, 2^30 tokens a request; caches, pages and the heads of q begin
+ * on 16-byte addresses.  max_keys: how many tokens the host knows a row to see at most (0: unknown; a window bounds it too);
+ * it only guides how the work is split, a row that sees more is right all the same.  ws (16-byte address, may be NULL for 0
+ * bytes): vits_op_paged_attention_workspace_bytes of the same numbers (-1 for a shape that is refused); calls that may run at
+ * the same time need one each. */
 int64_t vits_op_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int dim, int dtype, int64_t max_keys);
 int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, const void* v_cache,
                             int64_t page_stride, int pages, int page_size, const int* table, int64_t table_stride, int width,
