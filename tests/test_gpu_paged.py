@@ -147,6 +147,16 @@ def test_plan_of_prompts_across_blocks(ops, total):
     check_plan(ops, [0] * len(grow), grow, 16, -(-max(grow) // 16), sum(-(-g // 16) for g in grow), total + 3)
 
 
+def test_plan_of_the_most_requests(ops):
+    """65535 requests: a thread sums 256 of them, and a block serves 32."""
+    rng = random.Random(65535)
+    lengths = [rng.randint(0, 70) for _ in range(65535)]
+    grow = [rng.choice((-1, 0, 1, 1, 3)) for _ in lengths]
+    fresh = sum(-(-(l + max(g, 0)) // 16) - -(-l // 16) for l, g in zip(lengths, grow))
+    want = check_plan(ops, lengths, grow, 16, 5, fresh, sum(max(g, 0) for g in grow) + 9)
+    assert want["status"] == [0]
+
+
 def test_plan_without_rows(ops):
     check_plan(ops, [40, 17, 0], [-1, 0, -1], 16, 3, 4, 0)
     check_plan(ops, [40, 17, 0], [-1, 0, -1], 16, 3, 4, 5)
@@ -601,6 +611,16 @@ def test_attention_many_rows(ops, rows):
     cache = Cache(torch.bfloat16, lengths, 1, 64, 16, seed=rows)
     request = [s if rng.random() > 0.1 else -1 for s in range(rows)]
     check_attention(ops, cache, rows_q(cache, rows, 2, 64, torch.bfloat16), request, [n - 1 for n in lengths])
+
+
+@pytest.mark.parametrize("max_keys", [None, 700, 16])
+@pytest.mark.parametrize("dtype,heads,hk,window", [("bf16", 8, 2, 0), ("fp16", 3, 3, 50), ("fp32", 16, 1, 0)])
+def test_attention_of_prompts(ops, dtype, heads, hk, window, max_keys):
+    """Whole prompts row by row, beside a row that comes twice and rows of requests in turn, out of order."""
+    cache = Cache(TYPES[dtype], [700, 90], hk, 64, 32, seed=25)
+    request = [0] * 700 + [1] * 90 + [0, 0] + [1, 0] * 20
+    position = list(range(700)) + list(range(90)) + [411, 411] + [x for i in range(20) for x in (89 - i, 17 * i)]
+    check_attention(ops, cache, rows_q(cache, len(request), heads, 64, TYPES[dtype]), request, position, window=window, max_keys=max_keys)
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
