@@ -1248,8 +1248,15 @@ __global__ __launch_bounds__(ATT_THREADS) void paged_join_kernel(PagedAttArgs a,
 // (8 key-value heads of 128 in bf16: 8 units a row, 32 keys a step):
 //   rows x steps     1 x 32         4 x 63         16 x 63        16 x 125         64 x 2          64 x 125        256 x 16       256 x 32
 //   wave/block/split 44 / 14 / 16   86 / 24 / 21   87 / 25 / 31   178 / 51 / 40    8.7 / 11 / 18   192 / 125 / 126  71 / 79 / 83   125 / 117 / 128
-// A block's waves take the longest unit's steps by eights at 1.3 us each, whatever else there is to do; the pieces even that out
-// for about 10 us more (their sums at the start, the join, its launch).
+// A block's waves take the longest unit's steps by eights at 0.14 us a KiB of a step (fp32: 0.19), whatever else there is to do; the
+// pieces even that out for about 9 us more (their sums at the start, the join, its launch), and for more the more units there are.
+// So the border lies at so many KiB of the longest unit as those are worth.  Block / split beside it, at KiB:
+//   units             2 - 8                12 - 24           40 - 80           120 - 240
+//   bf16 of 128       608: 17/16           608: 16/19        1000: 25/21       1000: 25/31
+//   bf16 / fp16 of 64 500: 16/15           500: 16/17        750: 22/22        750: 24/30
+//   fp16 of 256       500: 15/16           800: 21/20        1200: 29/34       3000: 91/92
+//   fp32 of 96, 128   384: 15/15           384: 15/17        600: 21/17        1200: 43/42
+//   fp32 of 32, 64    400: 15/14           600: 19/16        600: 21/20        750: 28/24 (32), 34/38 (64)
 enum AttForm { ATT_WAVE, ATT_BLOCK, ATT_SPLIT };
 
 AttPlan att_plan(int rows, int heads, int kv_heads, int dim, int dtype, long long max_keys, AttForm& form) {
@@ -1260,10 +1267,10 @@ AttPlan att_plan(int rows, int heads, int kv_heads, int dim, int dtype, long lon
   p.units = kv_heads * p.tiles;
   p.pieces = ATT_PIECES;
   if (max_keys <= 0 || max_keys > (1 << 30)) max_keys = 1 << 30;
-  const int step = att_step(dtype == VITS_TYPE_F32 ? 4 : 2, dim);
+  const int size = dtype == VITS_TYPE_F32 ? 4 : 2, step = att_step(size, dim);
   const long long units = (long long)rows * p.units, steps = (max_keys + step - 1) / step;
   if (units >= 2048 ? steps <= 16 : units >= 512 && steps <= 2) form = ATT_WAVE;
-  else if (steps <= (units >= 512 ? 128 : units >= 128 ? 64 : 32)) form = ATT_BLOCK;
+  else if (steps <= 128 && steps * (step * dim * size / 512) <= (size == 4 ? 380 + 4 * units : 450 + 7 * units)) form = ATT_BLOCK;
   else form = ATT_SPLIT;
   if (units > 1 << 21) form = ATT_SPLIT;                   // more blocks than a grid of the other forms should have
   if (steps < (1 << 20)) {                                 // no more pieces than their least size fills
