@@ -334,7 +334,8 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
  * it only guides how the work is split, a row that sees more is right all the same.  ws (16-byte address, may be NULL for 0
  * bytes): vits_op_paged_attention_workspace_bytes of the same numbers (-1 for a shape that is refused); calls that may run at
  * the same time need one each. */
-int64_t vits_op_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int dim, int dtype, int64_t max_keys);
+int64_t vits_op_paged_attention_workspace_bytes(int requests, int rows, int heads, int kv_heads, int dim, int dtype,
+                                                int64_t max_keys);
 int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, const void* v_cache,
                             int64_t page_stride, int pages, int page_size, const int* table, int64_t table_stride, int width,
                             int requests, const int* row_request, const int* row_position, int rows, int heads, int kv_heads,

@@ -82,9 +82,10 @@ def test_paged_attention_refuses(change, word):
 def test_paged_attention_workspace():
     size = N.lib.vits_op_paged_attention_workspace_bytes
     for bad in ((-1, 4, 2, 128, 2, 0), (1, 4, 3, 128, 2, 0), (1, 0, 1, 128, 2, 0), (1, 4, 2, 40, 2, 0), (1, 4, 2, 512, 2, 0), (1, 4, 2, 128, 3, 0)):
-        assert size(*bad) == -1
-    need = size(3, 4, 2, 128, 2, 1 << 20)
-    assert need > 0 and size(0, 4, 2, 128, 2, 0) >= 0 and size(3, 4, 2, 128, 2, 100) == 0
+        assert size(3, *bad) == -1
+    need = size(3, 3, 4, 2, 128, 2, 1 << 20)
+    assert need > 0 and size(3, 0, 4, 2, 128, 2, 0) >= 0 and size(3, 3, 4, 2, 128, 2, 100) == 0
+    assert size(64, 64, 4, 2, 128, 2, 600) == 0 and size(1, 64, 4, 2, 128, 2, 600) > 0               # a row each; a prompt's rows
     if need:
         refused(N.lib.vits_op_paged_attention(*{**ATTEND, "max_keys": 1 << 20, "ws_bytes": need - 1}.values()), "workspace", WORKSPACE)
         refused(N.lib.vits_op_paged_attention(*{**ATTEND, "max_keys": 1 << 20, "ws": 0}.values()), "workspace", WORKSPACE)

@@ -99,7 +99,7 @@ def _load():
         "vits_op_page_plan": (i32, [vp, vp, i32, vp, i64, i32, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, i32, vp, vp]),
         "vits_op_rotary_store": (i32, [vp, i64, i64, vp, i64, i64, i32, vp, i64, i64, vp, i64, i64, vp, vp, i64, i32, i32, i32,
                                        i32, i32, vp, vp, i32, vp, i32, f32, i32, vp, vp]),
-        "vits_op_paged_attention_workspace_bytes": (i64, [i32, i32, i32, i32, i32, i64]),
+        "vits_op_paged_attention_workspace_bytes": (i64, [i32, i32, i32, i32, i32, i32, i64]),
         "vits_op_paged_attention": (i32, [vp, i64, i64, vp, vp, i64, i32, i32, vp, i64, i32, i32, vp, vp, i32, i32, i32, i32,
                                           i32, f32, i32, i64, vp, i64, i64, vp, vp, vp, i64, vp]),
     }

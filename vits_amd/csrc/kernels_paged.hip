@@ -1257,9 +1257,14 @@ __global__ __launch_bounds__(ATT_THREADS) void paged_join_kernel(PagedAttArgs a,
 //   fp16 of 256       500: 15/16           800: 21/20        1200: 29/34       3000: 91/92
 //   fp32 of 96, 128   384: 15/15           384: 15/17        600: 21/17        1200: 43/42
 //   fp32 of 32, 64    400: 15/14           600: 19/16        600: 21/20        750: 28/24 (32), 34/38 (64)
+// More units than the chip has SIMDs need no splitting while they are short (fp16, 8 heads of 64, rows x steps, wave / block / split):
+//   256 x 19 37/38/48   512 x 19 77/79/95   512 x 47 177/149/170   2048 x 8 116/210/176   2048 x 19 257/293/295
+// Rows of prompts (16 and more a request: more cannot be told here) stand in runs, and a block or wave for every row of a run but
+// the first has nothing to do, which costs a block of eight waves its start all the same.  One prompt, bf16, 32 / 8 heads of 128:
+//   256 rows 26/55/30   512 rows 63/119/52   2048 rows 647/909/412   4096 rows 2340/2940/1220
 enum AttForm { ATT_WAVE, ATT_BLOCK, ATT_SPLIT };
 
-AttPlan att_plan(int rows, int heads, int kv_heads, int dim, int dtype, long long max_keys, AttForm& form) {
+AttPlan att_plan(int requests, int rows, int heads, int kv_heads, int dim, int dtype, long long max_keys, AttForm& form) {
   AttPlan p{};
   p.group = heads / kv_heads;
   p.run_shift = p.group <= 1 ? 4 : p.group <= 2 ? 3 : p.group <= 4 ? 2 : p.group <= 8 ? 1 : 0;
@@ -1269,8 +1274,9 @@ AttPlan att_plan(int rows, int heads, int kv_heads, int dim, int dtype, long lon
   if (max_keys <= 0 || max_keys > (1 << 30)) max_keys = 1 << 30;
   const int size = dtype == VITS_TYPE_F32 ? 4 : 2, step = att_step(size, dim);
   const long long units = (long long)rows * p.units, steps = (max_keys + step - 1) / step;
-  if (units >= 2048 ? steps <= 16 : units >= 512 && steps <= 2) form = ATT_WAVE;
-  else if (steps <= 128 && steps * (step * dim * size / 512) <= (size == 4 ? 380 + 4 * units : 450 + 7 * units)) form = ATT_BLOCK;
+  const bool prompts = rows >= 16ll * requests;
+  if (prompts ? steps <= 8 : steps <= (units >= 8192 ? 32 : units >= 2048 ? 20 : units >= 512 ? 2 : 0)) form = ATT_WAVE;
+  else if (!prompts && steps <= 128 && steps * (step * dim * size / 512) <= (size == 4 ? 380 + 4 * units : 450 + 7 * units)) form = ATT_BLOCK;
   else form = ATT_SPLIT;
   if (units > 1 << 21) form = ATT_SPLIT;                   // more blocks than a grid of the other forms should have
   if (steps < (1 << 20)) {                                 // no more pieces than their least size fills
@@ -1325,15 +1331,15 @@ hipError_t launch_rotary_store(const RotaryArgs& a, hipStream_t s) {
   return a.dtype == VITS_TYPE_F16 ? start_rotary_t<_Float16>(a, s) : start_rotary_t<__bf16>(a, s);
 }
 
-int64_t paged_attention_workspace(int rows, int heads, int kv_heads, int dim, int dtype, long long max_keys) {
+int64_t paged_attention_workspace(int requests, int rows, int heads, int kv_heads, int dim, int dtype, long long max_keys) {
   AttForm form;
-  const AttPlan p = att_plan(rows, heads, kv_heads, dim, dtype, max_keys, form);
+  const AttPlan p = att_plan(requests, rows, heads, kv_heads, dim, dtype, max_keys, form);
   return form == ATT_SPLIT ? (int64_t)(p.pieces / ATT_WAVES) * (2 * ATT_COLS * (dim + 4) * sizeof(float) + sizeof(AttJoin)) : 0;
 }
 
 hipError_t launch_paged_attention(const PagedAttArgs& a, long long max_keys, void* ws, hipStream_t s) {
   AttForm form;
-  AttPlan p = att_plan(a.rows, a.heads, a.kv_heads, a.dim, a.dtype, max_keys, form);
+  AttPlan p = att_plan(a.requests, a.rows, a.heads, a.kv_heads, a.dim, a.dtype, max_keys, form);
   const int size = a.dtype == VITS_TYPE_F32 ? 4 : 2;
   p.per_page = a.page_size / 16;
   p.wide_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_row * size % 16 == 0 && a.out_head * size % 16 == 0;

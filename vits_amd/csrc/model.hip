@@ -1534,9 +1534,9 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
   return VITS_OK;
 }
 
-int64_t vits_op_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int dim, int dtype, int64_t max_keys) {
+int64_t vits_op_paged_attention_workspace_bytes(int requests, int rows, int heads, int kv_heads, int dim, int dtype, int64_t max_keys) {
   if (check_att_shape(rows, heads, kv_heads, dim, dtype) != VITS_OK) return -1;
-  return paged_attention_workspace(rows, heads, kv_heads, dim, dtype, max_keys);
+  return paged_attention_workspace(requests, rows, heads, kv_heads, dim, dtype, max_keys);
 }
 
 int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, const void* v_cache,
@@ -1567,7 +1567,7 @@ int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const 
   }
   if ((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)q) & 15) || (page_stride * size) % 16 || (q_row * size) % 16 || (q_head * size) % 16)
     return fail(VITS_ERR_INVALID, "paged attention: the caches, their pages and the heads of q must begin on 16-byte addresses");
-  if (ws_bytes < paged_attention_workspace(rows, heads, kv_heads, dim, dtype, max_keys) || (ws_bytes > 0 && !ws) || ((uintptr_t)ws & 15))
+  if (ws_bytes < paged_attention_workspace(requests, rows, heads, kv_heads, dim, dtype, max_keys) || (ws_bytes > 0 && !ws) || ((uintptr_t)ws & 15))
     return fail(VITS_ERR_WORKSPACE, "paged attention: workspace too small or not on a 16-byte address");
   if (rows == 0) return VITS_OK;
   PagedAttArgs a{};

@@ -23,7 +23,7 @@ int (*plan_fn)(const int*, const int*, int, int*, int64_t, int, int*, int, const
                int*, void*);
 int (*rotary_fn)(const void*, int64_t, int64_t, void*, int64_t, int64_t, int, const void*, int64_t, int64_t, const void*, int64_t, int64_t, void*,
                  void*, int64_t, int, int, int, int, int, const int*, const int64_t*, int, const double*, int, float, int, int*, void*);
-int64_t (*workspace_fn)(int, int, int, int, int, int64_t);
+int64_t (*workspace_fn)(int, int, int, int, int, int, int64_t);
 int (*attention_fn)(const void*, int64_t, int64_t, const void*, const void*, int64_t, int, int, const int*, int64_t, int, int, const int*,
                     const int*, int, int, int, int, int, float, int, int64_t, void*, int64_t, int64_t, float*, int*, void*, int64_t, void*);
 const char* (*last_error_fn)();
@@ -242,7 +242,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (keys <= 0) keys = table.size(1) * kc.size(2);
     if (window > 0 && window < keys) keys = window;
     const int r = narrow(rows, what), h = narrow(heads, what), hk = narrow(kc.size(1), what), d = narrow(dim, what);
-    const int64_t bytes = workspace_fn(r, h, hk, d, type, keys);
+    const int64_t bytes = workspace_fn(narrow(table.size(0), what), r, h, hk, d, type, keys);
     if (bytes < 0) return done(-1, what);
     // a workspace of this call's own: calls on different streams, and graphs that run side by side, share none
     Tensor ws;

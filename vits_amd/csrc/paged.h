@@ -53,7 +53,7 @@ struct PagedAttArgs {
   float* lse;
   int* err_flag;
 };
-int64_t paged_attention_workspace(int rows, int heads, int kv_heads, int dim, int dtype, long long max_keys);
+int64_t paged_attention_workspace(int requests, int rows, int heads, int kv_heads, int dim, int dtype, long long max_keys);
 hipError_t launch_paged_attention(const PagedAttArgs& a, long long max_keys, void* ws, hipStream_t s);
 
 }  // namespace vits
