@@ -326,9 +326,11 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
 
 /* Attention of single rows: out[r][h] = sum_t w_t v_t with w = softmax_t(scale * q[r][h] . k_t) over the tokens t of row
  * r's request with position - window < t <= position (window 0: from the first token on), keys and values of head
- * h / (heads / kv_heads).  A row that sees no token (position < 0) gives 0.  lse [rows][heads] fp32 or NULL: log of the sum
- * of exp(scale * q . k_t), -inf for such a row.  Scores, softmax and sums in fp32.  What lies in the cache behind a row's
- * position, and in pages the table does not name for it, has no influence whatever it holds.
+ * h / (heads / kv_heads).  A row that sees no token (position < 0, or none of its pages is one of the cache's) gives 0.  A row
+ * whose scores are all -inf has no value and gives NaN.  lse [rows][heads] fp32 or NULL: log of the sum of
+ * exp(scale * q . k_t), -inf for both.  Scores, softmax and sums in fp32.  What lies in the cache behind a row's position,
+ * and in pages the table does not name for it, has no influence whatever it holds.  A position beyond the table's last token: the
+ * tokens of its window that the table holds count, the others are left out.
  * dim: 32, 64, ... 256; at most 2^23 rows and, by the table, 2^30 tokens a request; caches, pages and the heads of q begin
  * on 16-byte addresses.  max_keys: how many tokens the host knows a row to see at most (0: unknown; a window bounds it too);
  * it only guides how the work is split, a row that sees more is right all the same.  ws (16-byte address, may be NULL for 0

@@ -1,0 +1,96 @@
+"""The paged-cache operators on the GPU where a call is legal and its data is not what one expects.  Values against 64 bits, with the
+bounds that test_gpu_paged.py derives."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_paged import TYPES, Cache, attend_by_hand, gpu_i32, rows_q
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available(), "GPU tests need an MI355X"
+    from vits_amd import ops
+    return ops
+
+
+@pytest.mark.parametrize("copies,max_keys", [(80, 32), (1, 32), (1, 10 ** 9)])       # a wave a unit, a block a unit, equal pieces
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_attention_of_pages_that_are_none(ops, dtype, copies, max_keys):
+    """A row whose every page lies outside the cache sees nothing and gives 0, beside rows of the same request that see a page; a row
+    whose pages are there and whose scores are all -inf has no value, whatever other pages are missing."""
+    t, page, window, bad = TYPES[dtype], 16, 16, (-1, 10 ** 6, -2 ** 31, 2 ** 31 - 1)
+    cache = Cache(t, [32] * (6 * copies), 2, 64, page, seed=31)
+    heads, table = 6, cache.table.clone()
+    request, position, want = [], [], []                  # want: the first key that counts, None for nothing, "nan" for no value
+    for c in range(copies):
+        s = 6 * c
+        for at, p, w in ((s, 15, None), (s + 1, 31, None), (s + 2, 15, None), (s + 2, 31, 16), (s + 2, 20, 16), (s + 3, 31, "nan"), (s + 4, 20, "nan"),
+                         (s + 5, 31, 16)):
+            request.append(at)
+            position.append(p)
+            want.append(w)
+        table[s, 0], table[s + 1, 1], table[s + 2, 0], table[s + 4, 0] = bad[c % 4], bad[(c + 1) % 4], bad[(c + 2) % 4], bad[(c + 3) % 4]
+        for at in (s + 3, s + 4):
+            cache.k_cache[cache.table[at, 1]] = -math.inf
+    q = rows_q(cache, len(request), heads, 64, t)
+    for r, w in enumerate(want):
+        if w == "nan":
+            q[r] = 1.0
+    flag, lse, out = gpu_i32([0]), torch.full((len(request), heads), 4.0, device="cuda"), torch.full_like(q, 4.0)
+    ops.paged_attention(q, cache.k_cache, cache.v_cache, table, gpu_i32(request), gpu_i32(position), window=window, max_keys=max_keys, out=out, lse=lse,
+                        err_flag=flag)
+    assert flag.item() == 1
+    out, lse = out.double().cpu(), lse.double().cpu()
+    for r, (s, p, w) in enumerate(zip(request, position, want)):
+        if w == "nan":
+            assert bool(torch.isnan(out[r]).all()) and bool((lse[r] == -math.inf).all()), r
+        elif w is None:
+            assert bool((out[r] == 0).all()) and bool((lse[r] == -math.inf).all()), (r, out[r])
+        else:
+            ref, ref_lse, tol, tol_lse = attend_by_hand(q[r], cache.k[s][w:], cache.v[s][w:], p - w, 1 / 8, window)
+            assert bool(((out[r] - ref).abs() <= tol).all()) and bool(((lse[r] - ref_lse).abs() <= tol_lse).all()), r
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_attention_of_missing_pages_over_many_blocks(ops, dtype):
+    """The same where a row's keys are cut into pieces that several blocks hold."""
+    t, n, far = TYPES[dtype], 20000, 10 ** 6
+    cache = Cache(t, [n, n, n], 1, 64, 16, seed=32)
+    table = cache.table.clone()
+    table[0] = -1
+    table[1, :-1] = cache.pages
+    cache.k_cache[cache.table[2].long()] = -math.inf
+    q = rows_q(cache, 4, 4, 64, t)
+    q[2] = 1.0
+    for request, position in (([0, 1, 2, -1], [n - 1] * 4), ([0, 1, 2, 0], [n - 1] * 3 + [far])):
+        lse, out, flag = torch.full((4, 4), 4.0, device="cuda"), torch.full_like(q, 4.0), gpu_i32([0])
+        ops.paged_attention(q, cache.k_cache, cache.v_cache, table, gpu_i32(request), gpu_i32(position), out=out, lse=lse, err_flag=flag)
+        assert flag.item() == 1
+        out, lse = out.double().cpu(), lse.double().cpu()
+        assert bool((out[0] == 0).all() and (lse[0] == -math.inf).all())
+        ref, ref_lse, tol, tol_lse = attend_by_hand(q[1], cache.k[1][n - 16:], cache.v[1][n - 16:], 15, 1 / 8, 0)
+        assert bool(((out[1] - ref).abs() <= tol).all()) and bool(((lse[1] - ref_lse).abs() <= tol_lse).all())
+        assert bool(torch.isnan(out[2]).all() and (lse[2] == -math.inf).all())
+        assert bool((out[3] == (4.0 if request[3] < 0 else 0.0)).all())
+
+
+@pytest.mark.parametrize("max_keys", [32, 10 ** 9])
+def test_attention_of_a_position_beyond_the_table(ops, max_keys):
+    """What the table holds of its window counts, and the flag says that there was more."""
+    t = torch.bfloat16
+    cache = Cache(t, [64, 64, 64], 2, 64, 16, seed=33)
+    q = rows_q(cache, 3, 4, 64, t)
+    position, window = [70, 64 + 19, 2 ** 31 - 1], 20
+    for w, low in ((0, [0, 0, 0]), (window, [51, 64, 64])):
+        flag, lse = gpu_i32([0]), torch.empty(3, 4, device="cuda")
+        out = ops.paged_attention(q, cache.k_cache, cache.v_cache, cache.table, gpu_i32([0, 1, 2]), gpu_i32(position), window=w, max_keys=max_keys, lse=lse,
+                                  err_flag=flag).double().cpu()
+        assert flag.item() == 1
+        for r in range(3):
+            ref, ref_lse, tol, tol_lse = attend_by_hand(q[r], cache.k[r][low[r]:], cache.v[r][low[r]:], 63 - low[r], 1 / 8, 0)
+            assert bool(((out[r] - ref).abs() <= tol).all()), (w, r)
+            assert bool(torch.equal(lse[r].double().cpu(), ref_lse)) if low[r] == 64 else bool(((lse[r].double().cpu() - ref_lse).abs() <= tol_lse).all())

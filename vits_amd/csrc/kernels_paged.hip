@@ -475,6 +475,15 @@ __device__ __forceinline__ bool att_row_keys(const PagedAttArgs& a, int row, int
   return stop > cap;
 }
 
+// Whether one of the pages of a request's keys [from, to) is one of the cache's.  Asked where a row's weights sum up to 0: if there is
+// one, all its scores are -inf and softmax has no value (0 / 0); if there is none, the row sees nothing.
+__device__ __forceinline__ bool att_any_page(const PagedAttArgs& a, int req, int from, int to) {
+  const int* table = a.table + (long long)req * a.table_stride;
+  bool any = false;
+  for (int p = from / a.page_size, last = (to - 1) / a.page_size; p <= last && !any; ++p) any = table[p] >= 0 && table[p] < a.pages;
+  return any;
+}
+
 // whether a run begins at `row`, and what it is
 __device__ __forceinline__ bool att_run(const PagedAttArgs& a, const AttPlan& p, int row, Run& r) {
   const int req = a.row_request[row], before = a.row_request[row > 0 ? row - 1 : 0];
@@ -955,7 +964,17 @@ __device__ __forceinline__ bool att_part(const PagedAttArgs& a, const AttPlan& p
         continue;
       }
     }
-    if (mine) att_leave<T, DIM>(a, p, w, col, lg, r.row + my_row, hk * group + my_head, begin >= end, whole, slot);
+    bool none = begin >= end;
+    const bool zero = whole && mine && !none && w.sum == 0.f;
+    if (__ballot(zero)) {                                 // as att_any_page does, all lanes side by side over the run's pages
+      bool any = !zero;
+      for (int page = r.begin / a.page_size; page * a.page_size < r.end && __ballot(!any); ++page) {
+        const int id = table[page], key = page * a.page_size;
+        any = any || (id >= 0 && id < a.pages && key < end && key + a.page_size > begin);
+      }
+      none = none || !any;
+    }
+    if (mine) att_leave<T, DIM>(a, p, w, col, lg, r.row + my_row, hk * group + my_head, none, whole, slot);
     if (alone < 0 || ++alone == r.n) return stray != 0;
   }
 }
@@ -1010,8 +1029,9 @@ __device__ __forceinline__ void att_join(const PagedAttArgs& a, const AttPlan& p
     }
     int from = begin, to = end;
     if (n_rows > 1) att_row_keys(a, row0 + row, from, to);
-    att_write<T>(a, p.wide_out, row0 + row, hk * p.group + head, c, x, sum, from >= to);
-    if (a.lse && c == 0) att_write_lse(a, row0 + row, hk * p.group + head, top, sum, from >= to);
+    const bool none = from >= to || (sum == 0.f && !att_any_page(a, a.row_request[row0], from, to));
+    att_write<T>(a, p.wide_out, row0 + row, hk * p.group + head, c, x, sum, none);
+    if (a.lse && c == 0) att_write_lse(a, row0 + row, hk * p.group + head, top, sum, none);
   }
 }
 
@@ -1236,8 +1256,9 @@ __global__ __launch_bounds__(ATT_THREADS) void paged_join_kernel(PagedAttArgs a,
         sum = 0.f;
         for (int w = 0; w < ATT_WAVES; ++w) sum += wave_sum[w];
       }
-      att_write<T>(a, p.wide_out, j.row + row, hk * p.group + head, 4 * quad, x, sum, from >= to);
-      if (a.lse && quad == 0) att_write_lse(a, j.row + row, hk * p.group + head, top, sum, from >= to);
+      const bool none = from >= to || (sum == 0.f && !att_any_page(a, a.row_request[j.row], from, to));
+      att_write<T>(a, p.wide_out, j.row + row, hk * p.group + head, 4 * quad, x, sum, none);
+      if (a.lse && quad == 0) att_write_lse(a, j.row + row, hk * p.group + head, top, sum, none);
     }
     if (!few) __syncthreads();                             // before the LDS is written again
   }
