@@ -94,3 +94,26 @@ def test_attention_of_a_position_beyond_the_table(ops, max_keys):
             ref, ref_lse, tol, tol_lse = attend_by_hand(q[r], cache.k[r][low[r]:], cache.v[r][low[r]:], 63 - low[r], 1 / 8, 0)
             assert bool(((out[r] - ref).abs() <= tol).all()), (w, r)
             assert bool(torch.equal(lse[r].double().cpu(), ref_lse)) if low[r] == 64 else bool(((lse[r].double().cpu() - ref_lse).abs() <= tol_lse).all())
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("layout", ["heads of a row", "each head", "one row for all"])
+def test_rotary_in_place_beside_keys(ops, dtype, layout):
+    """q turned in place with k and v in the same memory, between its rows or its heads: as from tensors of their own."""
+    t, rows, heads, dim = TYPES[dtype], 50, 4, 64
+    gen = torch.Generator(device="cuda").manual_seed(41)
+    if layout == "each head":
+        x = torch.randn(rows, heads, 3, dim, generator=gen, device="cuda").to(t)
+        q, k, v = x.unbind(2)
+    else:
+        x = torch.randn(rows, heads + 4, dim, generator=gen, device="cuda").to(t)
+        q, k, v = x[:, :heads], x[:, heads:heads + 2], x[:, heads + 2:]
+        if layout == "one row for all":
+            k, v = k[7:8].expand(rows, -1, -1), v[49:].expand(rows, -1, -1)
+    own = [y.contiguous() for y in (q, k, v)]
+    caches = [torch.zeros(4, k.shape[1], 16, dim, dtype=t, device="cuda") for _ in range(4)]
+    position, slot, freq = torch.arange(rows, dtype=torch.int32, device="cuda") * 3, torch.randperm(64, generator=gen, device="cuda")[:rows], ops.rotary_frequencies(dim)
+    want = ops.rotary_store(*own, caches[0], caches[1], position, slot, freq)
+    got = ops.rotary_store(q, k, v, caches[2], caches[3], position, slot, freq, out=q)
+    assert got is q and torch.equal(q, want) and torch.equal(k, own[1]) and torch.equal(v, own[2])
+    assert torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])

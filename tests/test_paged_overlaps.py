@@ -1,0 +1,36 @@
+"""Memory that the paged-cache operators would read and write, or write twice, in one launch: refused, on the host, before anything runs.
+No GPU: a refused call touches none of its pointers."""
+import pytest
+
+from vits_amd import _native as N
+
+P, M = 1 << 24, 1 << 20          # P stands for a device address on a 16-byte boundary; never followed
+INVALID = -1
+SIZE, DIM = 2, 128               # bf16
+HEAD = DIM * SIZE
+
+
+def refused(rc, word):
+    assert rc == INVALID
+    assert word in N.lib.vits_last_error().decode()
+
+
+# q, k and v of a row beside each other (4 + 2 + 2 heads), q turned in place
+FUSED = dict(q=P, q_row=8 * DIM, q_head=DIM, out=P, out_row=8 * DIM, out_head=DIM, heads=4, k=P + 4 * HEAD, k_row=8 * DIM, k_head=DIM, v=P + 6 * HEAD,
+             v_row=8 * DIM, v_head=DIM, k_cache=P + M, v_cache=P + 2 * M, page_stride=2 * 16 * DIM, pages=9, page_size=16, kv_heads=2, dim=DIM, dtype=2,
+             position=P + 3 * M, slot=P + 4 * M, rows=3, freq=P + 5 * M, pairs=64, scale=1.0, interleaved=0, err_flag=P + 6 * M, stream=0)
+ROW = 8 * HEAD
+# each head's query, key and value beside each other
+PER_HEAD = {**FUSED, "kv_heads": 4, "page_stride": 4 * 16 * DIM, "k": P + HEAD, "v": P + 2 * HEAD,
+            **{n: 3 * DIM for n in ("q_head", "out_head", "k_head", "v_head")}, **{n: 12 * DIM for n in ("q_row", "out_row", "k_row", "v_row")}}
+
+
+@pytest.mark.parametrize("base,change", [
+    (FUSED, dict(k=P)), (FUSED, dict(v=P)), (FUSED, dict(k=P + 2 * HEAD)), (FUSED, dict(v=P + 3 * HEAD)), (FUSED, dict(v=P + 4 * HEAD - 2)),
+    (FUSED, dict(k=P + ROW)), (FUSED, dict(k=P + 2 * ROW + HEAD)), (FUSED, dict(k=P + 7 * HEAD)),             # another row's queries
+    (FUSED, dict(k=P - ROW + 3 * HEAD)), (FUSED, dict(k_row=4 * DIM)), (FUSED, dict(v_row=0, v=P + 2 * ROW)), (FUSED, dict(k_head=3 * DIM, v_head=3 * DIM, v=P + 3 * HEAD)),
+    (PER_HEAD, dict(k=P)), (PER_HEAD, dict(k=P + HEAD - 2)), (PER_HEAD, dict(v=P + 3 * HEAD)), (PER_HEAD, dict(v=P + 2 * HEAD + 2)),
+    (PER_HEAD, dict(k_head=2 * DIM)), ({**FUSED, "rows": 1}, dict(k=P + 3 * HEAD)), ({**FUSED, "rows": 1}, dict(k=P - HEAD)),
+])
+def test_in_place_rotation_of_shared_rows(base, change):
+    refused(N.lib.vits_op_rotary_store(*{**base, **change}.values()), "k or v")

@@ -363,6 +363,36 @@ bool apart(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t dim) 
 }
 bool overlap(const Span& a, const Span& b) { return a.n > 0 && b.n > 0 && a.p < b.p + b.n && b.p < a.p + a.n; }
 
+// Rows of heads of `dim` bytes, strides in bytes, a's rows at least `dim` apart: do a cell of `a` and one of `b` share a byte?
+// Exact where b's rows lie as far apart as a's or there is one of either; rows at two different distances are taken to meet.
+struct Rows {
+  const char* p;
+  int64_t rows, row, heads, head;
+};
+bool meet(Rows a, Rows b, int64_t dim) {
+  if (b.row == 0) b.rows = 1;
+  const int64_t row = a.rows > 1 ? a.row : b.row, by = (int64_t)((uintptr_t)b.p - (uintptr_t)a.p);
+  if (a.rows > 1 && b.rows > 1 && a.row != b.row) return true;
+  // row i of b is n = i - j rows behind row j of a: -a.rows < n < b.rows
+  auto near = [&](int64_t x) {                           // some |x + n * row| < dim
+    if (a.rows <= 1 && b.rows <= 1) return x > -dim && x < dim;
+    const int64_t rest = (x % row + row) % row, n = (rest - x) / row;
+    return (rest < dim && n > -a.rows && n < b.rows) || (row - rest < dim && n - 1 > -a.rows && n - 1 < b.rows);
+  };
+  const int64_t a_len = (a.heads - 1) * a.head + dim, b_len = (b.heads - 1) * b.head + dim;
+  if (row > 0 && (by % row + row) % row >= a_len && (by % row + row) % row + b_len <= row) return false;   // beside each other in every row
+  if (a.heads > 1 && b.heads > 1 && a.head != b.head) {
+    for (int64_t i = 0; i < a.heads; ++i)
+      for (int64_t j = 0; j < b.heads; ++j)
+        if (near(by + j * b.head - i * a.head)) return true;
+    return false;
+  }
+  const int64_t head = a.heads > 1 ? a.head : b.head;
+  for (int64_t i = 1 - a.heads; i < b.heads; ++i)
+    if (near(by + i * head)) return true;
+  return false;
+}
+
 int check_page_size(int page_size) {
   if (page_size < PAGED_PAGE_UNIT || page_size % PAGED_PAGE_UNIT || page_size > 65536)
     return fail(VITS_ERR_INVALID, "page_size must be a multiple of 16 and at most 65536");
@@ -1514,7 +1544,6 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
     const int64_t cache = ((pages - 1) * page_stride + (int64_t)kv_heads * page_size * dim) * size;
     const Span caches[2] = {span(k_cache, cache), span(v_cache, cache)};
     const Span ins[3] = {from, span(k, rows, k_row, kv_heads, k_head, dim, size), span(v, rows, v_row, kv_heads, v_head, dim, size)};
-    // (q's own rows may be written in place between k's and v's)
     for (const Span& c : caches) {
       if (overlap(c, to)) return fail(VITS_ERR_INVALID, "rotary store: out overlaps a cache");
       for (const Span& x : ins)
@@ -1522,6 +1551,14 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
     }
     if (q && q != out && (overlap(to, ins[1]) || overlap(to, ins[2])))
       return fail(VITS_ERR_INVALID, "rotary store: out overlaps k or v");
+    // in place k and v may lie between q's rows or heads, but not on them: they are read while q is written
+    if (q && q == out) {
+      const Rows on{(const char*)q, rows, q_row * size, heads, q_head * size};
+      const Rows with[2] = {{(const char*)k, rows, k_row * size, kv_heads, k_head * size}, {(const char*)v, rows, v_row * size, kv_heads, v_head * size}};
+      for (int i = 0; i < 2; ++i)
+        if (overlap(to, ins[1 + i]) && meet(on, with[i], (int64_t)dim * size))
+          return fail(VITS_ERR_INVALID, "rotary store: q is turned in place and shares cells with k or v");
+    }
   }
   RotaryArgs a{};
   a.q = q; a.q_row = q_row; a.q_head = q_head; a.out = out; a.out_row = out_row; a.out_head = out_head; a.heads = heads;
