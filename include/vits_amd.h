@@ -314,7 +314,7 @@ int vits_op_page_plan(const int* lengths, const int* grow, int requests, int* ta
  * position * freq[i] (radians; freq in 64 bits, [pairs], the product too): channels i and i + pairs (interleaved == 0) or
  * 2i and 2i + 1 are (a, b) -> scale * (a cos - b sin, b cos + a sin); the other channels pass through.  q's rows go to
  * out (may be q itself, with the same strides, where k and v lie beside q's heads, not on them), k's and v's to slot [rows] of
- * the caches.  q may be NULL (no queries), or
+ * the caches (which must not share cells).  q may be NULL (no queries), or
  * k, v and the caches (then slot may be NULL too: every row is one).  Computed in fp32, rounded once.  The slots of one
  * call have to differ: where two rows share one, each stored value is either row's.  Scaled positions are scaled
  * frequencies (vits_amd/ops.py: rotary_frequencies); the gradient with respect to q is the same call on the gradient of

@@ -34,3 +34,13 @@ PER_HEAD = {**FUSED, "kv_heads": 4, "page_stride": 4 * 16 * DIM, "k": P + HEAD, 
 ])
 def test_in_place_rotation_of_shared_rows(base, change):
     refused(N.lib.vits_op_rotary_store(*{**base, **change}.values()), "k or v")
+
+
+BODY = 2 * 16 * DIM * SIZE       # bytes of a page
+PAIRED = {**FUSED, "page_stride": 2 * 2 * 16 * DIM, "v_cache": P + M + BODY}                            # [pages][2][...]
+
+
+@pytest.mark.parametrize("base,at", [(FUSED, 0), (FUSED, BODY - 2), (FUSED, 2 - BODY), (FUSED, 8 * BODY), (FUSED, 9 * BODY - 2), (PAIRED, 0), (PAIRED, BODY - 2),
+                                     (PAIRED, BODY + 2), (PAIRED, 2 * BODY), (PAIRED, -16 * BODY), (PAIRED, 8 * BODY + 16), (PAIRED, 17 * BODY - 2)])
+def test_a_cache_over_the_other(base, at):
+    refused(N.lib.vits_op_rotary_store(*{**base, "v_cache": P + M + at}.values()), "caches overlap")

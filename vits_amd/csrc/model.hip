@@ -1541,7 +1541,9 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
   if (q && !(q == out && q_row == out_row && q_head == out_head) && overlap(from, to))
     return fail(VITS_ERR_INVALID, "rotary store: in place needs the same strides on both sides, and no other overlap");
   if (k) {
-    const int64_t cache = ((pages - 1) * page_stride + (int64_t)kv_heads * page_size * dim) * size;
+    const int64_t body = (int64_t)kv_heads * page_size * dim * size, cache = (pages - 1) * page_stride * size + body;
+    if (meet(Rows{(const char*)k_cache, pages, page_stride * size, 1, 0}, Rows{(const char*)v_cache, pages, page_stride * size, 1, 0}, body))
+      return fail(VITS_ERR_INVALID, "rotary store: the two caches overlap");
     const Span caches[2] = {span(k_cache, cache), span(v_cache, cache)};
     const Span ins[3] = {from, span(k, rows, k_row, kv_heads, k_head, dim, size), span(v, rows, v_row, kv_heads, v_head, dim, size)};
     for (const Span& c : caches) {
