@@ -44,3 +44,27 @@ PAIRED = {**FUSED, "page_stride": 2 * 2 * 16 * DIM, "v_cache": P + M + BODY}    
                                      (PAIRED, BODY + 2), (PAIRED, 2 * BODY), (PAIRED, -16 * BODY), (PAIRED, 8 * BODY + 16), (PAIRED, 17 * BODY - 2)])
 def test_a_cache_over_the_other(base, at):
     refused(N.lib.vits_op_rotary_store(*{**base, "v_cache": P + M + at}.values()), "caches overlap")
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(position=P + 2 * HEAD), "out"), (dict(slot=P + ROW), "out"), (dict(freq=P + 64), "out"), (dict(err_flag=P + 3 * HEAD), "err_flag"),
+    (dict(position=P + M + 64), "cache"), (dict(slot=P + 2 * M - 8), "cache"), (dict(freq=P + 2 * M + 128), "cache"), (dict(err_flag=P + M + 4), "err_flag"),
+    (dict(err_flag=P + 3 * M + 8), "err_flag"), (dict(err_flag=P + 4 * M + 20), "err_flag"), (dict(err_flag=P + 5 * M + 508), "err_flag"),
+    (dict(err_flag=P + 4 * HEAD), "err_flag"), (dict(err_flag=P + 7 * HEAD), "err_flag"),
+    (dict(q=0, out=0, position=P + M), "cache"), (dict(k=0, v=0, k_cache=0, v_cache=0, slot=0, position=P), "out"),
+    (dict(k=0, v=0, k_cache=0, v_cache=0, freq=P + 8), "out"), (dict(k=0, v=0, k_cache=0, v_cache=0, err_flag=P + 8), "err_flag"),
+    (dict(slot=P + 2 * M + 9 * BODY - 8), "cache"),
+])
+def test_rotary_store_over_its_rows_numbers(change, word):
+    refused(N.lib.vits_op_rotary_store(*{**FUSED, **change}.values()), word)
+
+
+ATTEND = dict(q=P, q_row=512, q_head=128, k_cache=P + M, v_cache=P + 2 * M, page_stride=2 * 16 * 128, pages=9, page_size=16, table=P + 3 * M,
+              table_stride=8, width=8, requests=3, row_request=P + 4 * M, row_position=P + 5 * M, rows=3, heads=4, kv_heads=2, dim=128, dtype=2,
+              scale=0.1, window=0, max_keys=128, out=P + 6 * M, out_row=512, out_head=128, lse=P + 7 * M, err_flag=P + 8 * M, ws=P + 9 * M, ws_bytes=1 << 20,
+              stream=0)
+
+
+@pytest.mark.parametrize("at", [P + 8, P + M, P + 2 * M + 400, P + 3 * M + 4, P + 4 * M + 8, P + 5 * M, P + 6 * M + 12, P + 7 * M + 44, P + 9 * M + 16])
+def test_paged_attention_err_flag_over_another_tensor(at):
+    refused(N.lib.vits_op_paged_attention(*{**ATTEND, "err_flag": at}.values()), "err_flag")

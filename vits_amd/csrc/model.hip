@@ -1540,6 +1540,12 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
   const Span to = span(out, rows, out_row, q ? heads : 0, out_head, dim, size), from = span(q, rows, q_row, heads, q_head, dim, size);
   if (q && !(q == out && q_row == out_row && q_head == out_head) && overlap(from, to))
     return fail(VITS_ERR_INVALID, "rotary store: in place needs the same strides on both sides, and no other overlap");
+  const Span numbers[3] = {span(position, 4ll * rows), span(slot, 8ll * rows), span(freq, 8ll * pairs)}, flag = span(err_flag, 4);
+  for (const Span& x : numbers) {
+    if (overlap(to, x)) return fail(VITS_ERR_INVALID, "rotary store: out overlaps position, slot or freq");
+    if (overlap(flag, x)) return fail(VITS_ERR_INVALID, "rotary store: err_flag overlaps another tensor");
+  }
+  if (overlap(flag, to) || overlap(flag, from)) return fail(VITS_ERR_INVALID, "rotary store: err_flag overlaps another tensor");
   if (k) {
     const int64_t body = (int64_t)kv_heads * page_size * dim * size, cache = (pages - 1) * page_stride * size + body;
     if (meet(Rows{(const char*)k_cache, pages, page_stride * size, 1, 0}, Rows{(const char*)v_cache, pages, page_stride * size, 1, 0}, body))
@@ -1550,7 +1556,11 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
       if (overlap(c, to)) return fail(VITS_ERR_INVALID, "rotary store: out overlaps a cache");
       for (const Span& x : ins)
         if (overlap(c, x)) return fail(VITS_ERR_INVALID, "rotary store: a cache overlaps an input");
+      for (const Span& x : numbers)
+        if (overlap(c, x)) return fail(VITS_ERR_INVALID, "rotary store: a cache overlaps an input");
+      if (overlap(flag, c)) return fail(VITS_ERR_INVALID, "rotary store: err_flag overlaps another tensor");
     }
+    if (overlap(flag, ins[1]) || overlap(flag, ins[2])) return fail(VITS_ERR_INVALID, "rotary store: err_flag overlaps another tensor");
     if (q && q != out && (overlap(to, ins[1]) || overlap(to, ins[2])))
       return fail(VITS_ERR_INVALID, "rotary store: out overlaps k or v");
     // in place k and v may lie between q's rows or heads, but not on them: they are read while q is written
@@ -1595,7 +1605,7 @@ int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const 
   if (q_row < 0 || q_head < 0 || !apart(rows, out_row, heads, out_head, dim))
     return fail(VITS_ERR_INVALID, "paged attention: strides must not be negative, nor rows or heads of out overlap");
   const int64_t cache = ((pages - 1) * page_stride + (int64_t)kv_heads * page_size * dim) * size;
-  const Span outs[3] = {span(out, rows, out_row, heads, out_head, dim, size), span(lse, 4ll * rows * heads), span(ws, ws_bytes)};
+  const Span outs[3] = {span(out, rows, out_row, heads, out_head, dim, size), span(lse, 4ll * rows * heads), span(ws, ws_bytes)}, flag = span(err_flag, 4);
   const Span ins[6] = {span(q, rows, q_row, heads, q_head, dim, size), span(k_cache, cache), span(v_cache, cache),
                        span(table, 4ll * ((requests - 1) * table_stride + width)), span(row_request, 4ll * rows), span(row_position, 4ll * rows)};
   for (int i = 0; i < 3; ++i) {
@@ -1603,7 +1613,10 @@ int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const 
       if (overlap(outs[i], x)) return fail(VITS_ERR_INVALID, "paged attention: cannot run in place: an output or the workspace overlaps an input");
     for (int j = 0; j < i; ++j)
       if (overlap(outs[i], outs[j])) return fail(VITS_ERR_INVALID, "paged attention: out, lse and the workspace overlap");
+    if (overlap(outs[i], flag)) return fail(VITS_ERR_INVALID, "paged attention: err_flag overlaps another tensor");
   }
+  for (const Span& x : ins)
+    if (overlap(x, flag)) return fail(VITS_ERR_INVALID, "paged attention: err_flag overlaps another tensor");
   if ((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)q) & 15) || (page_stride * size) % 16 || (q_row * size) % 16 || (q_head * size) % 16)
     return fail(VITS_ERR_INVALID, "paged attention: the caches, their pages and the heads of q must begin on 16-byte addresses");
   if (ws_bytes < paged_attention_workspace(requests, rows, heads, kv_heads, dim, dtype, max_keys) || (ws_bytes > 0 && !ws) || ((uintptr_t)ws & 15))
