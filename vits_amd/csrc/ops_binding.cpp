@@ -201,7 +201,7 @@ PyObject* rotary_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (kc->scalar_type() != first.scalar_type() || kc->size(3) != dim)
         throw Refused{"rotary_store: the caches' type and channels are not the rows': " + describe(*kc) + " and " + describe(first)};
     }
-    no_grad(what, {q, k, v, kc, vc, out});
+    no_grad(what, {q, k, v, kc, vc, &freq, out});
     on_gpu(what, first, {k, v, kc, vc, slot, out, flag, &position, &freq});
     return done(rotary_fn(at_(q), q ? q->stride(0) : 0, q ? q->stride(1) : 0, at_(out), out ? out->stride(0) : 0, out ? out->stride(1) : 0,
                           narrow(heads, what), at_(k), k ? k->stride(0) : 0, k ? k->stride(1) : 0, at_(v), v ? v->stride(0) : 0,
@@ -232,7 +232,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (lse && (lse->dim() != 2 || lse->size(0) != rows || lse->size(1) != heads || lse->scalar_type() != at::kFloat || !lse->is_contiguous()))
       throw Refused{"paged_attention: lse must be contiguous float32 [rows, heads], got " + describe(*lse)};
     if (flag) flat(*flag, at::kInt, 1, what, "err_flag");
-    no_grad(what, {&q0, &kc, &vc, &out});
+    no_grad(what, {&q0, &kc, &vc, &out, lse});
     on_gpu(what, q0, {&kc, &vc, &table, &request, &position, &out, lse, flag});
     const int64_t size = q0.element_size();
     const bool aligned = ((uintptr_t)q0.data_ptr() | (uintptr_t)(q0.stride(0) * size) | (uintptr_t)(q0.stride(1) * size)) % 16 == 0;
