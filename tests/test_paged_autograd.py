@@ -2,6 +2,7 @@
 is known to have been written.  On the CPU a call that is not refused for that is refused for its device."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from vits_amd import ops
 
@@ -28,3 +29,17 @@ def test_gradients_are_refused(call, args, name):
         call(**asks)
     with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
         call(**asks)
+
+
+@pytest.mark.parametrize("call,args,name", calls(), ids=lambda x: getattr(x, "__name__", x if isinstance(x, str) else ""))
+def test_tangents_are_refused(call, args, name):
+    with forward_ad.dual_level():
+        dual = {**args, name: forward_ad.make_dual(args[name], torch.ones_like(args[name]))}
+        with pytest.raises(ValueError, match="tangent"):
+            call(**dual)
+        with torch.no_grad(), pytest.raises(ValueError, match="tangent"):       # which switches off gradients alone
+            call(**dual)
+        with pytest.raises(ValueError, match="GPU"):
+            call(**args)
+    with pytest.raises(ValueError, match="GPU"):
+        call(**args)

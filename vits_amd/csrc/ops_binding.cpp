@@ -6,6 +6,7 @@
 
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <string>
@@ -88,6 +89,10 @@ int64_t page_stride(const Tensor& cache) { return cache.size(0) > 1 ? cache.stri
 int64_t table_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
 void no_grad(const char* what, std::initializer_list<const Tensor*> values) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode())      // (which torch.no_grad leaves on)
+    for (const Tensor* t : values)
+      if (t && t->_fw_grad(0).defined())
+        throw Refused{std::string(what) + ": carries no tangent along: call it on the primal tensors (torch.autograd.forward_ad.unpack_dual)"};
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor* t : values)
     if (t && t->requires_grad())

@@ -14,8 +14,9 @@ The kernels are in libvits_amd.so (vits_op_page_plan, vits_op_rotary_store, vits
 the formulas and the layouts); there is no fallback.  Everything runs on the current stream of the tensors' device, nothing
 waits for the GPU, and with the outputs given (`out=`, `lse=`) a call can be captured into a graph.  Wrong shapes and types
 raise ValueError, a library error VitsError; ids on the device that are out of range are left out and OR 1 into `err_flag`
-(an int32 tensor of one element), where one is given.  No call records a gradient: tensors that ask for one are refused unless
-under torch.no_grad().  The reference has no counterpart (its attention, attentions.py:179-332, takes whole rows).
+(an int32 tensor of one element), where one is given.  No call records a gradient or carries a tangent along: tensors that ask
+for a gradient are refused unless under torch.no_grad(), and dual tensors of forward-mode differentiation always.  The
+reference has no counterpart (its attention, attentions.py:179-332, takes whole rows).
 
 Between these functions and the C ABI stands a binding of host code (csrc/ops_binding.cpp, lib/_vits_ops.so): a step makes two
 of these calls a layer, and a call of thirty arguments through ctypes costs as much as the kernel behind it."""
