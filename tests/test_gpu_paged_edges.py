@@ -117,3 +117,41 @@ def test_rotary_in_place_beside_keys(ops, dtype, layout):
     got = ops.rotary_store(q, k, v, caches[2], caches[3], position, slot, freq, out=q)
     assert got is q and torch.equal(q, want) and torch.equal(k, own[1]) and torch.equal(v, own[2])
     assert torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+
+
+def test_what_is_written_counts_as_written(ops):
+    """Autograd learns of in-place writes by a tensor's version: a cache or an output that a recorded product has saved and a call then
+    overwrites makes its backward an error, not a wrong gradient."""
+    t = torch.float32
+    gen = torch.Generator(device="cuda").manual_seed(42)
+    pages = ops.new_pages(2, 4, 8)
+    grow = gpu_i32([3, 2])
+    plan = ops.page_plan(pages.lengths, grow, pages.table, pages.ring, pages.cursor, 16, rows=6)
+    written = [pages.table, pages.ring, *plan]
+    before = [x._version for x in written]
+    read = [pages.lengths, grow, pages.cursor]
+    kept = [x._version for x in read]
+    assert ops.page_plan(pages.lengths, grow, pages.table, pages.ring, pages.cursor, 16, out=plan) is plan
+    assert all(x._version > n for x, n in zip(written, before)) and [x._version for x in read] == kept
+
+    q, k, v = (torch.randn(6, h, 32, generator=gen, device="cuda") for h in (4, 2, 2))
+    both = torch.zeros(8, 2, 2, 16, 32, device="cuda")
+    out, lse, flag = torch.zeros_like(q), torch.zeros(6, 4, device="cuda"), gpu_i32([0])
+    freq = ops.rotary_frequencies(32)
+    store = lambda: ops.rotary_store(q, k, v, both[:, 0], both[:, 1], plan.position, plan.slot, freq, out=out, err_flag=flag)      # noqa: E731
+    attend = lambda: ops.paged_attention(q, both[:, 0], both[:, 1], pages.table, plan.request, plan.position, out=out, lse=lse, err_flag=flag)  # noqa: E731
+    for call, written, read in ((store, (both, out, flag), (q, k, v, plan.slot, freq)), (attend, (out, lse, flag), (q, both, pages.table))):
+        before, kept = [x._version for x in written], [x._version for x in read]
+        call()
+        assert all(x._version > n for x, n in zip(written, before)) and [x._version for x in read] == kept
+    weight = torch.ones_like(both, requires_grad=True)
+    loss = (weight * both).sum()
+    with torch.no_grad():
+        store()
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    with torch.inference_mode():                          # tensors without a version
+        caches = [torch.zeros(8, 2, 16, 32, dtype=t, device="cuda") for _ in range(2)]
+        ops.rotary_store(q, k, v, *caches, plan.position, plan.slot, freq)
+    got = ops.rotary_store(q, k, v, *caches, plan.position, plan.slot, freq)      # an inference tensor outside that mode, as before
+    assert torch.equal(caches[0], both[:, 0]) and got.shape == q.shape

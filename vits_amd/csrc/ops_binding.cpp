@@ -125,8 +125,13 @@ void* address(PyObject* o) {
   return p;
 }
 
-PyObject* done(int rc, const char* what) {
-  if (rc == 0) Py_RETURN_NONE;
+// written: what the call has overwritten.  Autograd learns of that by a tensor's version (inference tensors have none).
+PyObject* done(int rc, const char* what, std::initializer_list<const Tensor*> written = {}) {
+  if (rc == 0) {
+    for (const Tensor* t : written)
+      if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    Py_RETURN_NONE;
+  }
   PyErr_Format(vits_error, "%s failed (%d): %s", what, rc, last_error_fn());
   return nullptr;
 }
@@ -172,7 +177,7 @@ PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
                         integer32(a[5], what), (int*)out[0]->data_ptr(), (int64_t*)out[1]->data_ptr(), (int*)out[2]->data_ptr(),
                         (int*)out[3]->data_ptr(), (int*)out[4]->data_ptr(), (int64_t*)out[5]->data_ptr(), narrow(rows, what),
                         (int*)out[6]->data_ptr(), address(a[8])),
-                what);
+                what, {&table, &ring, out[0], out[1], out[2], out[3], out[4], out[5], out[6]});
   });
 }
 
@@ -214,7 +219,7 @@ PyObject* rotary_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
                           kc ? narrow(kc->size(2), what) : 0, kc ? narrow(kc->size(1), what) : 0, narrow(dim, what), type,
                           (int*)position.data_ptr(), (int64_t*)at_(slot), narrow(rows, what), (double*)freq.data_ptr(),
                           narrow(freq.numel(), what), (float)real(a[9]), PyObject_IsTrue(a[8]) > 0, (int*)at_(flag), address(a[12])),
-                what);
+                what, {kc, vc, out, flag});
   });
 }
 
@@ -257,7 +262,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                              narrow(table.size(0), what), (int*)request.data_ptr(), (int*)position.data_ptr(), r, h, hk, d, type,
                              (float)real(a[6]), window, keys, out.data_ptr(), out.stride(0), out.stride(1), (float*)at_(lse), (int*)at_(flag),
                              bytes ? ws.data_ptr() : nullptr, bytes, address(a[12])),
-                what);
+                what, {&out, lse, flag});
   });
 }
 
