@@ -1,0 +1,57 @@
+"""The in-tree build: when a target is built again.  No compiler runs here."""
+import os
+import subprocess
+
+import pytest
+
+from vits_amd import build as b
+
+
+@pytest.fixture
+def tree(tmp_path, monkeypatch):
+    """The build in an empty library folder, with compilers that only write down what they were asked for."""
+    ran = []
+
+    def compiler(cmd, check=True, **kw):
+        ran.append(cmd)
+        with open(cmd[cmd.index("-o") + 1], "w") as f:
+            f.write("built")
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+    for name in ("LIBDIR", "LIB", "BINDING"):
+        monkeypatch.setattr(b, name, str(tmp_path / os.path.basename(getattr(b, name))) if name != "LIBDIR" else str(tmp_path))
+    monkeypatch.setattr(b.subprocess, "run", compiler)
+
+    def built():
+        ran.clear()
+        b.build(verbose=False)
+        return sorted(os.path.basename(cmd[cmd.index("-o") + 1]) for cmd in ran)
+    return built
+
+
+EVERYTHING = sorted([s.replace(".hip", ".o") for s in b.SOURCES] + ["_vits_ops.so", "libvits_amd.so"])
+
+
+def test_a_second_build_has_nothing_to_do(tree):
+    assert tree() == EVERYTHING
+    assert tree() == []
+
+
+def test_other_flags_build_again(tree, monkeypatch):
+    tree()
+    monkeypatch.setattr(b, "FLAGS", b.FLAGS + ["-DOTHER"])
+    assert tree() == sorted(x for x in EVERYTHING if x != "_vits_ops.so")
+    assert tree() == []
+    monkeypatch.setattr(b, "SOURCE_FLAGS", {"kernels_gl16.hip": ["-DONE"], **b.SOURCE_FLAGS})
+    assert tree() == ["kernels_gl16.o", "libvits_amd.so"]
+    monkeypatch.setattr(b, "CXX", "another-compiler")
+    assert tree() == ["_vits_ops.so"]
+    monkeypatch.setattr(b, "HIPCC", "another-hipcc")
+    assert tree() == sorted(x for x in EVERYTHING if x != "_vits_ops.so")
+
+
+def test_objects_of_an_unknown_command_are_built_again(tree):
+    """A folder that holds objects of an earlier build, which nothing says the flags of."""
+    for name in EVERYTHING:
+        with open(os.path.join(b.LIBDIR, name), "w") as f:
+            f.write("from before")
+    assert tree() == EVERYTHING

@@ -26,11 +26,25 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", 
 SOURCE_FLAGS = {"kernels_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
-def _stale(target: str, deps) -> bool:
-    if not os.path.exists(target):
+def _stale(target: str, deps, command: str) -> bool:
+    """Whether a target is missing, older than what it is made of, or made by another command than this one."""
+    try:
+        with open(target + ".cmd") as f:
+            if f.read() != command:
+                return True
+        t = os.path.getmtime(target)
+    except OSError:
         return True
-    t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _binding_command(source: str):
+    """(BUILT_FOR does nothing but make another torch another command.)"""
+    import torch
+    at = os.path.dirname(torch.__file__)
+    return [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            f'-DBUILT_FOR="{torch.__version__}"', "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(at, "include"), source,
+            "-o", BINDING, "-L" + os.path.join(at, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
 
 
 def build(force: bool = False, verbose: bool = True) -> str:
@@ -38,29 +52,31 @@ def build(force: bool = False, verbose: bool = True) -> str:
     headers = [os.path.join(CSRC, "common.h"), os.path.join(os.path.dirname(HERE), "include", "vits_amd.h")]
     paged = [os.path.join(CSRC, "paged.h")] + headers[1:]
     deps = {"kernels_paged.hip": paged, "model.hip": headers + paged}
-    objs, jobs = [], []
     bind = os.path.join(CSRC, "ops_binding.cpp")
-    if force or _stale(BINDING, [bind]):
-        import torch
-        at = os.path.dirname(torch.__file__)
-        jobs.append([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-                     "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(at, "include"), bind, "-o", BINDING,
-                     "-L" + os.path.join(at, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"])
+    targets = [(BINDING, [bind], _binding_command(bind))]
+    objs = []
     for src in SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(LIBDIR, src.replace(".hip", ".o"))
         objs.append(o)
-        if force or _stale(o, [s] + deps.get(src, headers[:1])):
-            jobs.append([HIPCC, *FLAGS, *SOURCE_FLAGS.get(src, []), "-c", s, "-o", o])
+        targets.append((o, [s] + deps.get(src, headers[:1]), [HIPCC, *FLAGS, *SOURCE_FLAGS.get(src, []), "-c", s, "-o", o]))
 
-    def run(cmd):
+    def make(target) -> bool:
+        path, made_of, cmd = target
+        line = " ".join(cmd)
+        if not force and not _stale(path, made_of, line):
+            return False
         if verbose:
-            print(" ".join(cmd), flush=True)
+            print(line, flush=True)
+        if os.path.exists(path + ".cmd"):            # (a build that fails leaves no target that passes for a built one)
+            os.remove(path + ".cmd")
         subprocess.run(cmd, check=True)
+        with open(path + ".cmd", "w") as f:
+            f.write(line)
+        return True
     with ThreadPoolExecutor(max_workers=4) as ex:
-        list(ex.map(run, jobs))
-    if jobs or force or _stale(LIB, objs):
-        run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs])
+        list(ex.map(make, targets))
+    make((LIB, objs, [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs]))
     return LIB
 
 
