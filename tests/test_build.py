@@ -55,3 +55,20 @@ def test_objects_of_an_unknown_command_are_built_again(tree):
         with open(os.path.join(b.LIBDIR, name), "w") as f:
             f.write("from before")
     assert tree() == EVERYTHING
+
+
+def test_the_binding_follows_the_header(tree):
+    """The binding's calls are declared by include/vits_amd.h alone: it includes it, and is built again with it."""
+    tree()
+    header = os.path.join(os.path.dirname(b.HERE), "include", "vits_amd.h")
+    with open(os.path.join(b.CSRC, "ops_binding.cpp")) as f:
+        source = f.read()
+    assert '#include "../../include/vits_amd.h"' in source and "decltype(&vits_op_paged_attention)" in source
+    later = os.path.getmtime(header) + 10
+    for name in EVERYTHING:
+        os.utime(os.path.join(b.LIBDIR, name), (later, later))
+    real = os.path.getmtime
+    b_getmtime = lambda path: later + 1 if path == header else real(path)      # noqa: E731
+    with pytest.MonkeyPatch.context() as m:
+        m.setattr(b.os.path, "getmtime", b_getmtime)
+        assert set(tree()) >= {"_vits_ops.so", "model.o", "kernels_paged.o", "libvits_amd.so"}

@@ -53,7 +53,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
     paged = [os.path.join(CSRC, "paged.h")] + headers[1:]
     deps = {"kernels_paged.hip": paged, "model.hip": headers + paged}
     bind = os.path.join(CSRC, "ops_binding.cpp")
-    targets = [(BINDING, [bind], _binding_command(bind))]
+    targets = [(BINDING, [bind, headers[1]], _binding_command(bind))]
     objs = []
     for src in SOURCES:
         s = os.path.join(CSRC, src)

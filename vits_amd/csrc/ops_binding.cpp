@@ -11,6 +11,8 @@
 
 #include <string>
 
+#include "../../include/vits_amd.h"
+
 namespace {
 
 using at::Tensor;
@@ -20,14 +22,12 @@ struct Refused {
   std::string why;
 };
 
-int (*plan_fn)(const int*, const int*, int, int*, int64_t, int, int*, int, const int64_t*, int, int*, int64_t*, int*, int*, int*, int64_t*, int,
-               int*, void*);
-int (*rotary_fn)(const void*, int64_t, int64_t, void*, int64_t, int64_t, int, const void*, int64_t, int64_t, const void*, int64_t, int64_t, void*,
-                 void*, int64_t, int, int, int, int, int, const int*, const int64_t*, int, const double*, int, float, int, int*, void*);
-int64_t (*workspace_fn)(int, int, int, int, int, int, int64_t);
-int (*attention_fn)(const void*, int64_t, int64_t, const void*, const void*, int64_t, int, int, const int*, int64_t, int, int, const int*,
-                    const int*, int, int, int, int, int, float, int, int64_t, void*, int64_t, int64_t, float*, int*, void*, int64_t, void*);
-const char* (*last_error_fn)();
+// the library's entry points, as its header declares them
+decltype(&vits_op_page_plan) plan_fn;
+decltype(&vits_op_rotary_store) rotary_fn;
+decltype(&vits_op_paged_attention_workspace_bytes) workspace_fn;
+decltype(&vits_op_paged_attention) attention_fn;
+decltype(&vits_last_error) last_error_fn;
 PyObject* vits_error;
 
 std::string describe(const Tensor& t) {
