@@ -72,3 +72,13 @@ def test_the_binding_follows_the_header(tree):
     with pytest.MonkeyPatch.context() as m:
         m.setattr(b.os.path, "getmtime", b_getmtime)
         assert set(tree()) >= {"_vits_ops.so", "model.o", "kernels_paged.o", "libvits_amd.so"}
+
+
+def test_the_build_check_compiles_everything(tree, monkeypatch):
+    """__graft_entry__.build() says whether the tree builds, so it compiles whatever is there already."""
+    import __graft_entry__ as entry
+    tree()
+    asked = []
+    monkeypatch.setattr(b, "build", lambda **kw: asked.append(kw) or os.path.join(b.LIBDIR, "libvits_amd.so"))
+    entry.build()
+    assert asked == [dict(force=True)]
