@@ -7,16 +7,27 @@ import pytest
 from vits_amd import build as b
 
 
+def remarks(*kernels):
+    """What the compiler says of its kernels' registers (-Rpass-analysis=kernel-resource-usage)."""
+    lines = []
+    for name, change in kernels:
+        says = {"TotalSGPRs": 90, "VGPRs": 256, "AGPRs": 0, "ScratchSize [bytes/lane]": 0, "Dynamic Stack": "False", "Occupancy [waves/SIMD]": 2,
+                "SGPRs Spill": 72, "VGPRs Spill": 0, "LDS Size [bytes/block]": 16852, **change}
+        lines += [f"remark: a.hip:52:0: {x} [-Rpass-analysis=kernel-resource-usage]" for x in
+                  (f"Function Name: {name}", *(f"    {k}: {v}" for k, v in says.items()))]
+    return "\n".join(lines) + "\n"
+
+
 @pytest.fixture
 def tree(tmp_path, monkeypatch):
     """The build in an empty library folder, with compilers that only write down what they were asked for."""
-    ran = []
+    ran, used = [], [("some_kernel", {})]
 
     def compiler(cmd, check=True, **kw):
         ran.append(cmd)
         with open(cmd[cmd.index("-o") + 1], "w") as f:
             f.write("built")
-        return subprocess.CompletedProcess(cmd, 0, "", "")
+        return subprocess.CompletedProcess(cmd, 0, "", remarks(*used))
     for name in ("LIBDIR", "LIB", "BINDING"):
         monkeypatch.setattr(b, name, str(tmp_path / os.path.basename(getattr(b, name))) if name != "LIBDIR" else str(tmp_path))
     monkeypatch.setattr(b.subprocess, "run", compiler)
@@ -25,6 +36,7 @@ def tree(tmp_path, monkeypatch):
         ran.clear()
         b.build(verbose=False)
         return sorted(os.path.basename(cmd[cmd.index("-o") + 1]) for cmd in ran)
+    built.used = used
     return built
 
 
@@ -82,3 +94,21 @@ def test_the_build_check_compiles_everything(tree, monkeypatch):
     monkeypatch.setattr(b, "build", lambda **kw: asked.append(kw) or os.path.join(b.LIBDIR, "libvits_amd.so"))
     entry.build()
     assert asked == [dict(force=True)]
+
+
+@pytest.mark.parametrize("change,word", [({"AGPRs": 2}, "AGPRs"), ({"VGPRs": 257}, "VGPRs"), ({"ScratchSize [bytes/lane]": 16}, "ScratchSize"),
+                                         ({"VGPRs Spill": 3}, "VGPRs Spill")])
+def test_a_build_of_too_many_registers_is_none(tree, change, word):
+    """The paged attention has to stay within 256 vector registers, without accumulator registers and scratch."""
+    tree.used[:] = [("one", {}), ("another", change)]
+    with pytest.raises(RuntimeError, match=f"another.*{word}"):
+        tree()
+    tree.used[:] = [("one", {}), ("another", {})]
+    assert {"kernels_paged.o", "libvits_amd.so"} <= set(tree())                     # what was refused is not taken for built
+    assert tree() == []
+
+
+def test_a_build_that_says_nothing_of_its_registers_is_none(tree):
+    tree.used.clear()
+    with pytest.raises(RuntimeError, match="registers"):
+        tree()

@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import os
+import re
 import subprocess
 import sys
 import sysconfig
@@ -23,7 +24,31 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", 
 
 # The paged attention keeps its accumulators in the registers that the vector unit reads too.  Left to choose, the compiler gives
 # builds with much LDS the other kind, moves values there, and has been seen to move only those of the lanes that were on.
-SOURCE_FLAGS = {"kernels_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# Where a build needs more than 256 registers it takes those too, whatever the flag says: so the compiler reports what it used, and a
+# build that has any, or scratch, is refused (the widest today: 256, none, none).
+USAGE = "-Rpass-analysis=kernel-resource-usage"
+SOURCE_FLAGS = {"kernels_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", USAGE]}
+MOST = {"VGPRs": 256, "AGPRs": 0, "ScratchSize": 0, "VGPRs Spill": 0}
+
+
+def _check_registers(source: str, report: str) -> str:
+    """Refuses a build whose kernels use more than MOST; returns what else the compiler said."""
+    kernel, seen, rest = "", set(), []
+    for line in report.splitlines():
+        if f"[{USAGE}]" not in line:
+            rest.append(line)
+            continue
+        name, _, value = re.sub(r"^.*?remark: \S+:\d+:\d+:\s*", "", line).replace(f"[{USAGE}]", "").strip().partition(": ")
+        name = name.split(" [")[0]
+        if name == "Function Name":
+            kernel = value
+        elif name in MOST:
+            seen.add(name)
+            if int(value) > MOST[name]:
+                raise RuntimeError(f"{source}: {kernel} uses {value} {name}, at most {MOST[name]} allowed")
+    if seen != set(MOST):
+        raise RuntimeError(f"{source}: the compiler did not say which registers its kernels use")
+    return "\n".join(rest)
 
 
 def _stale(target: str, deps, command: str) -> bool:
@@ -70,7 +95,14 @@ def build(force: bool = False, verbose: bool = True) -> str:
             print(line, flush=True)
         if os.path.exists(path + ".cmd"):            # (a build that fails leaves no target that passes for a built one)
             os.remove(path + ".cmd")
-        subprocess.run(cmd, check=True)
+        if USAGE in cmd:
+            done = subprocess.run(cmd, stderr=subprocess.PIPE, text=True)
+            if done.returncode:
+                sys.stderr.write(done.stderr)
+                done.check_returncode()
+            sys.stderr.write(_check_registers(os.path.basename(made_of[0]), done.stderr))
+        else:
+            subprocess.run(cmd, check=True)
         with open(path + ".cmd", "w") as f:
             f.write(line)
         return True

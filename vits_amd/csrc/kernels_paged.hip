@@ -801,9 +801,10 @@ __device__ __forceinline__ void att_leave(const PagedAttArgs& a, const AttPlan& 
 // a NaN in V would reach it.  So where rows differ and a result is not finite, the part is taken again row by row, with what
 // the row does not see left out of V.
 //
-// No lane is ever switched off in here before the last write: what a lane must not load it loads from where another may, and
-// drops.  With lanes off, the compiler (ROCm 7.2) has been seen to move whole-wave values between registers of the two kinds
-// for the lanes that were on alone, for which reason no build may need more than 256 registers either.
+// Lanes are switched off in here for the write of a result alone (which, row by row, other rows follow): what a lane must not load it
+// loads from where another may, and drops.  With lanes off, the compiler (ROCm 7.2) has been seen to move whole-wave values to
+// accumulator registers and back for the lanes that were on alone.  It has none to move to: builds that use them, or scratch, or
+// more than 256 vector registers are refused (vits_amd/build.py).
 template <typename T, int DIM>
 __device__ __forceinline__ bool att_part(const PagedAttArgs& a, const AttPlan& p, const Run& r, int unit, int t0, int t1, bool whole, float* slot) {
   using Tile = AttTile<T, DIM>;
