@@ -13,7 +13,7 @@ def remarks(*kernels):
     for name, change in kernels:
         says = {"TotalSGPRs": 90, "VGPRs": 256, "AGPRs": 0, "ScratchSize [bytes/lane]": 0, "Dynamic Stack": "False", "Occupancy [waves/SIMD]": 2,
                 "SGPRs Spill": 72, "VGPRs Spill": 0, "LDS Size [bytes/block]": 16852, **change}
-        lines += [f"remark: a.hip:52:0: {x} [-Rpass-analysis=kernel-resource-usage]" for x in
+        lines += [f"/a/b.hip:52:1: remark: {x} [-Rpass-analysis=kernel-resource-usage]\n   52 | __global__ void f() {{\n      | ^" for x in
                   (f"Function Name: {name}", *(f"    {k}: {v}" for k, v in says.items()))]
     return "\n".join(lines) + "\n"
 
@@ -112,3 +112,8 @@ def test_a_build_that_says_nothing_of_its_registers_is_none(tree):
     tree.used.clear()
     with pytest.raises(RuntimeError, match="registers"):
         tree()
+
+
+def test_other_messages_of_the_compiler_are_passed_on():
+    odd, end = "x.hip:3:4: warning: odd\n    3 | int x;\n      | ^\n", "1 warning generated.\n"
+    assert b._check_registers("x.hip", odd + remarks(("one", {})) + end) == odd + end

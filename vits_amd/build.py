@@ -33,12 +33,15 @@ MOST = {"VGPRs": 256, "AGPRs": 0, "ScratchSize": 0, "VGPRs Spill": 0}
 
 def _check_registers(source: str, report: str) -> str:
     """Refuses a build whose kernels use more than MOST; returns what else the compiler said."""
-    kernel, seen, rest = "", set(), []
+    kernel, seen, rest, quoted = "", set(), [], False
     for line in report.splitlines():
         if f"[{USAGE}]" not in line:
-            rest.append(line)
+            quoted = quoted and re.match(r"\s*\d*\s+\|", line) is not None            # the source line that a remark is about
+            if not quoted:
+                rest.append(line)
             continue
-        name, _, value = re.sub(r"^.*?remark: \S+:\d+:\d+:\s*", "", line).replace(f"[{USAGE}]", "").strip().partition(": ")
+        quoted = True
+        name, _, value = line.split("remark: ")[1].replace(f"[{USAGE}]", "").strip().partition(": ")
         name = name.split(" [")[0]
         if name == "Function Name":
             kernel = value
@@ -48,7 +51,7 @@ def _check_registers(source: str, report: str) -> str:
                 raise RuntimeError(f"{source}: {kernel} uses {value} {name}, at most {MOST[name]} allowed")
     if seen != set(MOST):
         raise RuntimeError(f"{source}: the compiler did not say which registers its kernels use")
-    return "\n".join(rest)
+    return "".join(x + "\n" for x in rest)
 
 
 def _stale(target: str, deps, command: str) -> bool:
