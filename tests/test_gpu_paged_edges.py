@@ -155,3 +155,58 @@ def test_what_is_written_counts_as_written(ops):
         ops.rotary_store(q, k, v, *caches, plan.position, plan.slot, freq)
     got = ops.rotary_store(q, k, v, *caches, plan.position, plan.slot, freq)      # an inference tensor outside that mode, as before
     assert torch.equal(caches[0], both[:, 0]) and got.shape == q.shape
+
+
+def two_term_bounds(t):
+    """Of a weight held in two terms of type t, the second of which is what the first leaves of it: each is off by half a step of what it
+    holds, so by 2^-22 of the weight in fp16 and 2^-16 in bf16.  fp16 holds nothing below 2^-24, where half a step is 2^-25: the largest
+    weight is at least 2^11 there, so that is 2^-36 of it."""
+    return {torch.float32: (0.0, 0.0), torch.float16: (2.0 ** -22, 2.0 ** -36), torch.bfloat16: (2.0 ** -16, 0.0)}[t]
+
+
+def cancelling(t, keys, rows, dim, seed):
+    """Rows whose weighted values nearly cancel: the sum is some 2^-9 of its terms, so its own rounding hides nothing of theirs.  Scores are
+    products of one channel each (the others are 0), at most 1.5; the last key takes away what the others sum up to."""
+    gen = torch.Generator().manual_seed(seed)
+    q = torch.zeros(rows, 1, dim)
+    q[:, 0, 0] = 1.0
+    k = torch.zeros(rows, keys, dim)
+    k[:, :, 0] = torch.rand(rows, keys, generator=gen) * 3 - 1.5
+    k = k.to(t)
+    v = torch.randn(rows, keys, dim, generator=gen).to(t)
+    weight = torch.softmax(k[:, :, 0].double(), 1)
+    v[:, -1] = (-(weight[:, :-1, None] * v[:, :-1].double()).sum(1) / weight[:, -1:]).to(t)
+    return q.to(t), k, v
+
+
+@pytest.mark.parametrize("max_keys", [32, 10 ** 9])
+@pytest.mark.parametrize("keys", [3, 32])
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_attention_weights_in_two_terms(ops, dtype, keys, max_keys):
+    """The weights enter the second product as exactly as two terms hold them; one alone is found out (planted in the oracle)."""
+    t, rows, dim = TYPES[dtype], 24, 64
+    q, k, v = cancelling(t, keys, rows, dim, seed=keys)
+    cache = Cache(t, [0] * rows, 1, dim, 16, seed=51, width=2, spare=2 * rows)
+    cache.table.copy_(torch.arange(2 * rows, dtype=torch.int32, device="cuda").view(rows, 2))
+    for r in range(rows):
+        for at in range(keys):
+            cache.k_cache[2 * r + at // 16, 0, at % 16] = k[r, at].cuda()
+            cache.v_cache[2 * r + at // 16, 0, at % 16] = v[r, at].cuda()
+    out = ops.paged_attention(q.cuda(), cache.k_cache, cache.v_cache, cache.table, gpu_i32(list(range(rows))), gpu_i32([keys - 1] * rows), scale=1.0,
+                              max_keys=max_keys).double().cpu()
+    score, values = k[:, :, 0].double(), v.double()
+    weight = torch.softmax(score, 1)
+    ref = torch.einsum("rn,rnd->rd", weight, values)
+    size, most = torch.einsum("rn,rnd->rd", weight, values.abs()), weight.amax(1)[:, None] * values.abs().sum(1)
+    held, least = two_term_bounds(t)
+    # a score is one product of two values of type t and zeros, exact in fp32; times log2 e and less the maximum: three roundings of at most
+    # 2 * 1.5 * log2 e < 8 (with the 11 that fp16 adds: 16), 2^-24 each, and the exponential's own 2^-23: below 2^-18.  Sums of at most 32 terms
+    # in fp32, twice, and their quotient: 66 * 2^-24.
+    tol = ref.abs() * (torch.finfo(t).eps / 2) + size * (2 * 2.0 ** -18 + 66 * 2.0 ** -24 + held) + least * most
+    if t == torch.float16:
+        tol = tol + 2.0 ** -25
+    assert bool(((out[:, 0] - ref).abs() <= tol).all()), float(((out[:, 0] - ref).abs() / tol).max())
+    if t != torch.float32:
+        w = torch.exp(score - score.amax(1, keepdim=True))
+        one = torch.einsum("rn,rnd->rd", w.to(t).double(), values) / w.sum(1, keepdim=True)
+        assert bool(((one - ref).abs() > tol).any(1).float().mean() > 0.5)                # most rows would tell
