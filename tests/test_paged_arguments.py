@@ -1,0 +1,25 @@
+"""Calls of the paged-cache operators whose arguments are unusual.  On the CPU a call that is not refused for them is refused for its device."""
+import pytest
+import torch
+
+from vits_amd import ops
+
+
+def i32(*values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+def test_caches_of_one_page_need_no_common_stride():
+    """Strides of dimensions of one element say nothing, so two caches may differ there; elsewhere they may not."""
+    both = torch.zeros(3, 2, 2, 16, 64)
+    q, k, v = torch.zeros(2, 4, 64), torch.zeros(2, 2, 64), torch.zeros(2, 2, 64)
+    freq = ops.rotary_frequencies(64, device="cpu")
+    for k_cache, v_cache, word in ((both[:1, 0], torch.zeros(1, 2, 16, 64), "GPU"), (both[:1, 0], both[1:2, 1], "GPU"), (both[:, 0], torch.zeros(3, 2, 16, 64), "alike")):
+        with pytest.raises(ValueError, match=word):
+            ops.paged_attention(q, k_cache, v_cache, i32(0)[None], i32(0, 0), i32(3, 4))
+        with pytest.raises(ValueError, match=word):
+            ops.rotary_store(q, k, v, k_cache, v_cache, i32(3, 4), torch.arange(2), freq)
+    one = torch.zeros(3, 1, 16, 64)
+    other = torch.zeros(3, 1024, dtype=torch.float32).as_strided((3, 1, 16, 64), (1024, 7, 64, 1))
+    with pytest.raises(ValueError, match="GPU"):
+        ops.paged_attention(q, one, other, i32(0)[None], i32(0, 0), i32(3, 4))

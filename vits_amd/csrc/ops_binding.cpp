@@ -73,7 +73,8 @@ void rows_of(const Tensor& t, at::ScalarType type, int64_t rows, int64_t heads, 
 }
 
 void caches_of(const Tensor& k, const Tensor& v, const char* what) {
-  const bool alike = k.dim() == 4 && v.scalar_type() == k.scalar_type() && v.sizes() == k.sizes() && v.strides() == k.strides();
+  bool alike = k.dim() == 4 && v.scalar_type() == k.scalar_type() && v.sizes() == k.sizes();
+  for (int i = 0; alike && i < 4; ++i) alike = k.size(i) <= 1 || v.stride(i) == k.stride(i);
   if (!alike || k.stride(3) != 1 || k.stride(2) != k.size(3) || (k.stride(1) != k.size(2) * k.size(3) && k.size(1) > 1))
     throw Refused{std::string(what) + ": k_cache and v_cache must be alike, [pages, kv_heads, page_size, dim], and contiguous within a page, got " +
                   describe(k) + " and " + describe(v)};
