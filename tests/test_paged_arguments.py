@@ -23,3 +23,20 @@ def test_caches_of_one_page_need_no_common_stride():
     other = torch.zeros(3, 1024, dtype=torch.float32).as_strided((3, 1, 16, 64), (1024, 7, 64, 1))
     with pytest.raises(ValueError, match="GPU"):
         ops.paged_attention(q, one, other, i32(0)[None], i32(0, 0), i32(3, 4))
+
+
+def rotary_arguments():
+    q, k, v = torch.zeros(2, 4, 64), torch.zeros(2, 2, 64), torch.zeros(2, 2, 64)
+    caches = torch.zeros(2, 3, 2, 16, 64)
+    return dict(q=q, k=k, v=v, k_cache=caches[0], v_cache=caches[1], position=i32(3, 4), slot=torch.arange(2), freq=ops.rotary_frequencies(64, device="cpu"))
+
+
+def test_an_error_of_an_argument_is_that_error():
+    class Odd:
+        def __bool__(self):
+            raise KeyError("odd")
+    with pytest.raises(KeyError):
+        ops.rotary_store(**rotary_arguments(), interleaved=Odd())
+    for bad in ("1.5", None, [1.0]):
+        with pytest.raises(TypeError):
+            ops.rotary_store(**rotary_arguments(), scale=bad)

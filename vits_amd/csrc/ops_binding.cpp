@@ -115,6 +115,11 @@ long long integer(PyObject* o) {
   return x;
 }
 int integer32(PyObject* o, const char* what) { return narrow(integer(o), what); }
+bool truth(PyObject* o) {
+  const int x = PyObject_IsTrue(o);
+  if (x < 0) throw std::exception();
+  return x > 0;
+}
 double real(PyObject* o) {
   const double x = PyFloat_AsDouble(o);
   if (x == -1.0 && PyErr_Occurred()) throw std::exception();
@@ -190,6 +195,8 @@ PyObject* rotary_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor *kc = maybe(a[3], what, "k_cache"), *vc = maybe(a[4], what, "v_cache"), *slot = maybe(a[6], what, "slot");
     const Tensor *out = maybe(a[10], what, "out"), *flag = maybe(a[11], what, "err_flag");
     const Tensor &position = tensor(a[5], what, "position"), &freq = tensor(a[7], what, "freq");
+    const bool interleaved = truth(a[8]);
+    const float scale = (float)real(a[9]);
     if (!q && !k) throw Refused{"rotary_store: neither queries nor keys"};
     if (!q && out) throw Refused{"rotary_store: out without q"};
     if (k ? !(v && kc && vc && slot) : v || kc || vc) throw Refused{"rotary_store: keys, values, both caches and slots go together"};
@@ -219,7 +226,7 @@ PyObject* rotary_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
                           v ? v->stride(1) : 0, at_(kc), at_(vc), kc ? page_stride(*kc) : 0, kc ? narrow(kc->size(0), what) : 0,
                           kc ? narrow(kc->size(2), what) : 0, kc ? narrow(kc->size(1), what) : 0, narrow(dim, what), type,
                           (int*)position.data_ptr(), (int64_t*)at_(slot), narrow(rows, what), (double*)freq.data_ptr(),
-                          narrow(freq.numel(), what), (float)real(a[9]), PyObject_IsTrue(a[8]) > 0, (int*)at_(flag), address(a[12])),
+                          narrow(freq.numel(), what), scale, interleaved, (int*)at_(flag), address(a[12])),
                 what, {kc, vc, out, flag});
   });
 }
