@@ -40,3 +40,23 @@ def test_an_error_of_an_argument_is_that_error():
     for bad in ("1.5", None, [1.0]):
         with pytest.raises(TypeError):
             ops.rotary_store(**rotary_arguments(), scale=bad)
+
+
+def test_what_is_no_tensor_is_a_value_error():
+    """The first argument too, whose shape and device the functions look at themselves."""
+    r = rotary_arguments()
+    pages = ops.new_pages(3, 4, 20, device="cpu")
+    for bad in (None, [1.0, 2.0], 3):
+        with pytest.raises(ValueError, match="q must be a tensor"):
+            ops.paged_attention(bad, r["k_cache"], r["v_cache"], i32(0)[None], i32(0, 0), i32(3, 4))
+        with pytest.raises(ValueError, match="lengths must be a tensor"):
+            ops.page_plan(bad, i32(1, 1, 1), pages.table, pages.ring, pages.cursor, 16, rows=4)
+        if bad is not None:
+            with pytest.raises(ValueError, match="q must be a tensor"):
+                ops.rotary_store(**{**r, "q": bad})
+            with pytest.raises(ValueError, match="k must be a tensor"):
+                ops.rotary_store(**{**r, "q": None, "k": bad})
+    with pytest.raises(ValueError, match="q must be"):
+        ops.paged_attention(torch.zeros(()), r["k_cache"], r["v_cache"], i32(0)[None], i32(0, 0), i32(3, 4))
+    with pytest.raises(ValueError, match="out"):
+        ops.page_plan(pages.lengths, i32(1, 1, 1), pages.table, pages.ring, pages.cursor, 16, out=[None] * 7)

@@ -75,6 +75,11 @@ def new_pages(requests: int, width: int, pages: int, device="cuda") -> Pages:
                  torch.tensor([0, pages], dtype=torch.int64, device=device))
 
 
+def _need_tensor(x, what: str) -> None:
+    if not isinstance(x, torch.Tensor):
+        raise ValueError(what + " must be a tensor")
+
+
 def _call(first: torch.Tensor, fn, *args) -> None:
     """fn(*args, stream) on the current stream of the first tensor's GPU.  (The two private functions are what torch.cuda.current_device and
     current_stream come down to; those take 2 us a call, as much as the rest of it.)"""
@@ -95,6 +100,7 @@ def page_plan(lengths: torch.Tensor, grow: torch.Tensor, table: torch.Tensor, ri
     `rows` is how many there may be (default: as `out` holds).  table and ring are changed in place; the new lengths and
     cursor are returned beside the old ones, so the caller decides when the step counts.  Where the step does not fit,
     `status` says why and nothing is changed."""
+    _need_tensor(lengths, "page_plan: lengths")
     if out is None:
         if rows is None:
             raise ValueError("page_plan: give rows or out")
@@ -106,7 +112,10 @@ def page_plan(lengths: torch.Tensor, grow: torch.Tensor, table: torch.Tensor, ri
         if len(out) != 7:
             raise ValueError("page_plan: out must hold a PagePlan's seven tensors")
         out = PagePlan._make(out)
-    _call(lengths, _bound.page_plan, lengths, grow, table, ring, cursor, page_size, out.request.numel() if rows is None else rows, out)
+    if rows is None:
+        _need_tensor(out.request, "page_plan: out.request")
+        rows = out.request.numel()
+    _call(lengths, _bound.page_plan, lengths, grow, table, ring, cursor, page_size, rows, out)
     return out
 
 
@@ -146,6 +155,10 @@ def rotary_store(q: Optional[torch.Tensor], k: Optional[torch.Tensor], v: Option
     into k_cache at the rows' slots, where v goes too, unturned.  The first 2 * freq.numel() channels of a head turn.
     Rows of slot < 0 are left as they were.  q may be None (nothing is returned), or k, v and the caches (then slot may be
     too).  With q alone and -freq it is its own gradient.  The slots of one call have to differ."""
+    if q is not None:
+        _need_tensor(q, "rotary_store: q")
+    elif k is not None:
+        _need_tensor(k, "rotary_store: k")
     if q is not None and out is None:
         # rows that are no rows are left as they were: not as the allocator found them
         out = (torch.empty if slot is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
@@ -165,8 +178,12 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     that sees nothing gives 0, a row of request < 0 is left as it was (0 in an `out` made here).  lse (fp32 [rows, heads],
     optional) receives the log of the sum of the exponentials.  max_keys: the most tokens a row can see as far as the host
     knows, which guides how the work is split; the result does not depend on it beyond rounding."""
+    _need_tensor(q, "paged_attention: q")
     if out is None:
         out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-    _call(q, _bound.paged_attention, q, k_cache, v_cache, table, request, position, 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale,
-          window, 0 if max_keys is None else max_keys, out, lse, err_flag)
+    if scale is None:
+        if q.dim() != 3 or q.shape[-1] == 0:
+            raise ValueError(f"paged_attention: q must be [rows, heads, dim], got {tuple(q.shape)}")
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    _call(q, _bound.paged_attention, q, k_cache, v_cache, table, request, position, scale, window, 0 if max_keys is None else max_keys, out, lse, err_flag)
     return out
