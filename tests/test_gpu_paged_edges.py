@@ -210,3 +210,18 @@ def test_attention_weights_in_two_terms(ops, dtype, keys, max_keys):
         w = torch.exp(score - score.amax(1, keepdim=True))
         one = torch.einsum("rn,rnd->rd", w.to(t).double(), values) / w.sum(1, keepdim=True)
         assert bool(((one - ref).abs() > tol).any(1).float().mean() > 0.5)                # most rows would tell
+
+
+def test_the_documented_example_runs(ops):
+    """The lines of the module's docstring, with a model of one layer."""
+    import textwrap
+    code = textwrap.dedent("\n".join(x for x in ops.__doc__.splitlines() if x.startswith("    ")))
+    assert "page_plan" in code and "paged_attention" in code
+    kv_heads, dim, R = 2, 64, 96
+    gen = torch.Generator(device="cuda").manual_seed(61)
+    q, k, v = (torch.randn(R, h, dim, generator=gen, device="cuda").to(torch.bfloat16) for h in (4, kv_heads, kv_heads))
+    names = dict(ops=ops, torch=torch, kv_heads=kv_heads, dim=dim, R=R, q=q, k=k, v=v, grow=torch.ones(64, dtype=torch.int32, device="cuda"))
+    exec(code, names)
+    assert names["lengths"].tolist() == [1] * 64 and names["plan"].status.item() == 0
+    # one token each: it sees itself alone
+    assert torch.equal(names["o"][:64], v[:64].repeat_interleave(2, 1)) and not names["o"][64:].any()

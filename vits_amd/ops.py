@@ -1,7 +1,7 @@
 """Operators around a paged key-value cache, on torch tensors: what an autoregressive model needs that is served beside
 the synthesiser (a text or prosody model whose tokens, durations or pitch go to `SynthesizerTrn.infer_batches`).
 
-    pages = ops.new_pages(requests=64, width=512, pages=20000, page_size=16, device="cuda")  # table, ring, cursor, lengths
+    lengths, table, ring, cursor = ops.new_pages(requests=64, width=512, pages=20000, device="cuda")       # no request holds anything
     k_cache, v_cache = (torch.empty(20000, kv_heads, 16, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))   # a layer
     freq = ops.rotary_frequencies(dim, device="cuda")
     ...
