@@ -299,7 +299,8 @@ int vits_op_attention_prec(const float* qkv, const float* emb_k, const float* em
  * row_position (0 for a request's first token) and row_slot, -1 behind the last; requests' rows follow each other in
  * order, and so do the pages they take.  status [1]: 0, or the OR of VITS_PLAN_*; then nothing is taken: lengths_out and
  * cursor_out repeat the inputs, row_start is 0, every row is -1, table and ring are left as they were.
- * At most 65535 requests, 2^30 rows and 2^30 pages. */
+ * At most 65535 requests, 2^30 rows and 2^30 pages.  Made for some thousand requests: the time grows with their square
+ * beyond (4096: 17 us, 16384: 120 us, 65535: 1.9 ms). */
 #define VITS_PLAN_BAD_LENGTH 1 /* a length below 0, a growth below -1, or their sum beyond int32 */
 #define VITS_PLAN_TABLE_FULL 2 /* a request needs more pages than its row of the table has       */
 #define VITS_PLAN_ROWS_FULL 4  /* more new tokens than rows                                      */
@@ -334,7 +335,8 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
  * tokens of its window that the table holds count, the others are left out.
  * dim: 32, 64, ... 256; at most 2^23 rows and, by the table, 2^30 tokens a request; caches, pages and the heads of q begin
  * on 16-byte addresses.  max_keys: how many tokens the host knows a row to see at most (0: unknown; a window bounds it too);
- * it only guides how the work is split, a row that sees more is right all the same.  ws (16-byte address, may be NULL for 0
+ * it only guides how the work is split, a row that sees more is right all the same; so do rows and requests (the table's size): 16
+ * and more rows a request of the table are taken for prompts, which are split otherwise than single rows.  ws (16-byte address, may be NULL for 0
  * bytes): vits_op_paged_attention_workspace_bytes of the same numbers (-1 for a shape that is refused); calls that may run at
  * the same time need one each. */
 int64_t vits_op_paged_attention_workspace_bytes(int requests, int rows, int heads, int kv_heads, int dim, int dtype,

@@ -25,7 +25,8 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 // pages than the ring, so no place is read by one block and written by another.
 // Bound by latency, not by its bytes: a launch, one dependent load, a scan and a barrier for the sums, the same again for the
 // rows, one table entry.  One block would do for the sums, but its rows would then wait for a second launch.  48 requests, a row
-// each: 4.9 us; 700 requests, 62 k rows (1.06 MB): 7.4 us; 256 prompts, 254 k rows (4.2 MB): 6.6 us (0.6 TB/s).
+// each: 4.9 us; 700 requests, 62 k rows (1.06 MB): 7.4 us; 256 prompts, 254 k rows (4.2 MB): 6.6 us (0.6 TB/s).  Every block reads every
+// request, and a block serves 32 of them at most, so many requests cost their square: 4096 take 17 us, 16384 120 us, 65535 1.9 ms.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int PLAN_THREADS = 256;
 constexpr int PLAN_ROWS = 1024;              // rows of a block: four consecutive ones a thread, 16-byte stores
@@ -211,7 +212,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PagePlanArgs a)
 // rotary rows, stored to the cache.  A pair of channels (a, b) turns to (a cos - b sin, b cos + a sin); every value is read and
 // written once, so a prompt is bound by memory: 8192 rows of 32 + 8 + 8 heads of 128 in bf16, 201 MB, take 43.8 us, 4.6 TB/s
 // (a plain copy: 4.9).  A block computes the angles of its rows once, in LDS, for all their heads: a transcendental a pair and
-// row instead of one a value.  Few rows are bound by the chain launch - position - angle - barrier - slot - values: one row 2.4
+// row instead of one a value.  Few rows are bound by the chain launch - position - angle - barrier - slot - values: one row 2.5
 // us, 192 rows of 48 heads of 128 (4.45 MB) 3.9 us; loading the values before the angles was no faster there (the longer code
 // costs as much as it hides) and slower on prompts (51 us).
 // ---------------------------------------------------------------------------------------------------------
@@ -1279,11 +1280,21 @@ __global__ __launch_bounds__(ATT_THREADS) void paged_join_kernel(PagedAttArgs a,
 //   fp16 of 256       500: 15/16           800: 21/20        1200: 29/34       3000: 91/92
 //   fp32 of 96, 128   384: 15/15           384: 15/17        600: 21/17        1200: 43/42
 //   fp32 of 32, 64    400: 15/14           600: 19/16        600: 21/20        750: 28/24 (32), 34/38 (64)
+// Beyond 128 steps the pieces even out more than their start costs, but for steps of 4 KiB; block / split at units x steps:
+//   bf16 of 128   240 x 128 50/54   240 x 200 102/95   512 x 128 115/115   512 x 160 137/130   512 x 250 229/195   1024 x 128 216/217   1024 x 250 393/389
+//   fp16 of 64    256 x 128 30/37   256 x 200 46/53    256 x 300 81/78     512 x 128 57/56     512 x 200 102/94    1024 x 128 117/118   1024 x 200 173/163
+//   bf16 of 32    56 x 128 16/18    56 x 160 19/20     128 x 160 21/24     128 x 200 25/26     512 x 160 32/42     512 x 200 41/48
+// 512 units of one or two steps take a wave each, more steps a block: wave / block at 1, 2, 3, 4 steps
+//   bf16 of 128, 512 units   9.8/11.4 10.6/11.2 12.2/12.2 13.3/12.0      1024 units   9.4/20 11.6/21 12.0/23 15/26
+//   fp16 of 64, 512 units    7.3/6.3 8.0/7.1 8.3/6.8 9.5/7.3             1024 units   6.7/11 7.9/12 8.7/12 9.8/12
+// (from 1024 units on a wave would be the faster one for up to 8 steps: 21 / 30 and 14 / 17 us there.)
 // More units than the chip has SIMDs need no splitting while they are short (fp16, 8 heads of 64, rows x steps, wave / block / split):
 //   256 x 19 37/38/48   512 x 19 77/79/95   512 x 47 177/149/170   2048 x 8 116/210/176   2048 x 19 257/293/295
 // Rows of prompts (16 and more a request: more cannot be told here) stand in runs, and a block or wave for every row of a run but
 // the first has nothing to do, which costs a block of eight waves its start all the same.  One prompt, bf16, 32 / 8 heads of 128:
 //   256 rows 26/55/30   512 rows 63/119/52   2048 rows 647/909/412   4096 rows 2340/2940/1220
+// `requests` is the table's size, the only number of requests that the host has: a prompt of 2048 rows with a table of 129 requests and
+// more is not told from single rows, and takes 901 us for 409.
 enum AttForm { ATT_WAVE, ATT_BLOCK, ATT_SPLIT };
 
 AttPlan att_plan(int requests, int rows, int heads, int kv_heads, int dim, int dtype, long long max_keys, AttForm& form) {

@@ -154,7 +154,8 @@ def rotary_store(q: Optional[torch.Tensor], k: Optional[torch.Tensor], v: Option
     """Turns q [rows, heads, dim] by its rows' positions into `out` (new, given, or q itself), and k [rows, kv_heads, dim]
     into k_cache at the rows' slots, where v goes too, unturned.  The first 2 * freq.numel() channels of a head turn.
     Rows of slot < 0 are left as they were.  q may be None (nothing is returned), or k, v and the caches (then slot may be
-    too).  With q alone and -freq it is its own gradient.  The slots of one call have to differ."""
+    too).  With q alone and -freq it is its own gradient.  The slots of one call have to differ, and the caches share no cell; q turned
+    in place may have k and v between its rows and heads.  An `out` made here with slots is filled with zeros first, by a launch of its own."""
     if q is not None:
         _need_tensor(q, "rotary_store: q")
     elif k is not None:
@@ -175,7 +176,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     err_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Every row of q [rows, heads, dim] attends to its request's tokens up to and with its own position (the last `window` of
     them, where that is not 0); heads / kv_heads query heads share a key-value head.  scale: 1 / sqrt(dim) by default.  A row
-    that sees nothing gives 0, a row of request < 0 is left as it was (0 in an `out` made here).  lse (fp32 [rows, heads],
+    that sees nothing gives 0, a row of request < 0 is left as it was (0 in an `out` made here, by a launch of its own).  lse (fp32 [rows, heads],
     optional) receives the log of the sum of the exponentials.  max_keys: the most tokens a row can see as far as the host
     knows, which guides how the work is split; the result does not depend on it beyond rounding."""
     _need_tensor(q, "paged_attention: q")
