@@ -330,15 +330,15 @@ int vits_op_rotary_store(const void* q, int64_t q_row, int64_t q_head, void* out
  * r's request with position - window < t <= position (window 0: from the first token on), keys and values of head
  * h / (heads / kv_heads).  A row that sees no token (position < 0, or none of its pages is one of the cache's) gives 0.  A row
  * whose scores are all -inf has no value and gives NaN.  lse [rows][heads] fp32 or NULL: log of the sum of
- * exp(scale * q . k_t), -inf for both.  Scores, softmax and sums in fp32.  What lies in the cache behind a row's position,
- * and in pages the table does not name for it, has no influence whatever it holds.  A position beyond the table's last token: the
- * tokens of its window that the table holds count, the others are left out.
+ * exp(scale * q . k_t), -inf for both, +inf for a row with a score of +inf (whose out is NaN).  Scores, softmax and sums in
+ * fp32.  What lies in the cache behind a row's position, and in pages the table does not name for it, has no influence whatever it
+ * holds.  A position beyond the table's last token: the tokens of its window that the table holds count, the others are left out.
  * dim: 32, 64, ... 256; at most 2^23 rows and, by the table, 2^30 tokens a request; caches, pages and the heads of q begin
  * on 16-byte addresses.  max_keys: how many tokens the host knows a row to see at most (0: unknown; a window bounds it too);
- * it only guides how the work is split, a row that sees more is right all the same; so do rows and requests (the table's size): 16
- * and more rows a request of the table are taken for prompts, which are split otherwise than single rows.  ws (16-byte address, may be NULL for 0
- * bytes): vits_op_paged_attention_workspace_bytes of the same numbers (-1 for a shape that is refused); calls that may run at
- * the same time need one each. */
+ * it only guides how the work is split, a row that sees more is right all the same; so do rows and requests (the table's size):
+ * 16 and more rows a request of the table are taken for prompts, which are split otherwise than single rows.  ws (16-byte
+ * address, may be NULL for 0 bytes): vits_op_paged_attention_workspace_bytes of the same numbers (-1 for a shape that is
+ * refused); calls that may run at the same time need one each. */
 int64_t vits_op_paged_attention_workspace_bytes(int requests, int rows, int heads, int kv_heads, int dim, int dtype,
                                                 int64_t max_keys);
 int vits_op_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, const void* v_cache,

@@ -225,3 +225,30 @@ def test_the_documented_example_runs(ops):
     assert names["lengths"].tolist() == [1] * 64 and names["plan"].status.item() == 0
     # one token each: it sees itself alone
     assert torch.equal(names["o"][:64], v[:64].repeat_interleave(2, 1)) and not names["o"][64:].any()
+
+
+FORMS = [(80, 1, 32), (1, 2, 32), (1, 2, 10 ** 9)]          # copies of the rows, key-value heads, max_keys: a wave a unit, a block, equal pieces
+
+
+@pytest.mark.parametrize("copies,hk,max_keys", FORMS)
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_attention_of_infinitely_high_scores(ops, dtype, copies, hk, max_keys):
+    """A score of +inf: the row has no value (inf / inf), and the log of its sum is +inf; with a NaN beside it that is NaN too."""
+    t = TYPES[dtype]
+    cache = Cache(t, [32, 32, 32] * copies, hk, 64, 16, seed=72)
+    for s in range(3 * copies):
+        if s % 3 != 2:
+            cache.k_cache[cache.table[s, 1], :, 5] = math.inf
+        if s % 3 == 1:
+            cache.k_cache[cache.table[s, 0], :, 2] = math.nan
+    request = [s for c in range(copies) for s in (3 * c, 3 * c + 1, 3 * c + 2, 3 * c, 3 * c)]
+    position = [31, 31, 31, 20, 21] * copies
+    q = rows_q(cache, len(request), 3 * hk, 64, t, gain=1.0).abs()
+    lse = torch.empty(len(request), 3 * hk, device="cuda")
+    out = ops.paged_attention(q, cache.k_cache, cache.v_cache, cache.table, gpu_i32(request), gpu_i32(position), max_keys=max_keys, lse=lse).double().cpu()
+    for r, kind in enumerate(["inf", "nan", "", "", "inf"] * copies):
+        if kind:
+            assert bool(torch.isnan(out[r]).all()) and bool((lse[r] == math.inf).all() if kind == "inf" else torch.isnan(lse[r]).all()), (r, lse[r])
+        else:
+            ref, ref_lse, tol, tol_lse = attend_by_hand(q[r], cache.k[request[r]], cache.v[request[r]], position[r], 1 / 8, 0)
+            assert bool(((out[r] - ref).abs() <= tol).all()) and bool(((lse[r].double().cpu() - ref_lse).abs() <= tol_lse).all()), r

@@ -740,7 +740,8 @@ struct AttTile {
       for (int c = 0; c < CH; ++c) o[c] *= keep;
       top = next;
     }
-    const float base = top == -INFINITY ? 0.f : top - LIFT;
+    // (of an infinite score nothing is taken away, so that it is the sum that becomes infinite, not a NaN)
+    const float base = fabsf(top) == INFINITY ? 0.f : top - LIFT;
 #pragma unroll
     for (int u = 0; u < SUB; ++u)
 #pragma unroll
@@ -1012,7 +1013,7 @@ __device__ __forceinline__ void att_join(const PagedAttArgs& a, const AttPlan& p
     float top = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int j = 0; j < N; ++j) top = part[j] ? fmaxf(top, tops[j]) : top;
-    const float base = top == -INFINITY ? 0.f : top;
+    const float base = fabsf(top) == INFINITY ? 0.f : top;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -1232,7 +1233,7 @@ __global__ __launch_bounds__(ATT_THREADS) void paged_join_kernel(PagedAttArgs a,
       for (int k = me % WAVE; k < parts; k += WAVE) top = fmaxf(top, part(k)[a.dim]);
 #pragma unroll
       for (int d = 1; d < WAVE; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, WAVE));
-      base = top == -INFINITY ? 0.f : top;
+      base = fabsf(top) == INFINITY ? 0.f : top;
       for (int k0 = 0; k0 < parts; k0 += AHEAD * at_once) {
         if (k0 > 0) load(k0);
 #pragma unroll
