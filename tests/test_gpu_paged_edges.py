@@ -227,7 +227,49 @@ def test_the_documented_example_runs(ops):
     assert torch.equal(names["o"][:64], v[:64].repeat_interleave(2, 1)) and not names["o"][64:].any()
 
 
+def definition(q, k, v, scale):
+    """Softmax attention of one row as its formula has it, in 64 bits, infinities and all: q [heads, dim], k and v [keys, kv_heads, dim]."""
+    group = q.shape[0] // k.shape[1]
+    q, k, v = q.double().cpu(), k.double().cpu().repeat_interleave(group, 1), v.double().cpu().repeat_interleave(group, 1)
+    score = torch.stack([(q * x).sum(-1) for x in k]) * scale                                            # [keys, heads]
+    weight = torch.softmax(score, 0)
+    return torch.stack([(weight[:, h, None] * v[:, h]).sum(0) for h in range(q.shape[0])]), torch.logsumexp(score, 0)
+
+
 FORMS = [(80, 1, 32), (1, 2, 32), (1, 2, 10 ** 9)]          # copies of the rows, key-value heads, max_keys: a wave a unit, a block, equal pieces
+
+
+@pytest.mark.parametrize("copies,hk,max_keys", FORMS)
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_attention_of_infinite_values_that_are_seen(ops, dtype, copies, hk, max_keys):
+    """A weight times an infinity is that infinity; the two of them together, or a NaN, are NaN; the other channels keep their values.
+    Rows alone and beside rows of the same request that do not see it."""
+    t = TYPES[dtype]
+    cache = Cache(t, [32, 32, 32, 20] * copies, hk, 64, 16, seed=71)
+    heads = 3 * hk
+    inf = math.inf
+    for s in range(4 * copies):
+        for at, channel, x in ((17, 3, inf), (17, 9, -inf), (4, 40, inf), (17, 40, -inf), (18, 63, math.nan)):
+            if s % 4 != 1:
+                cache.v[s][at, :, channel] = x
+                cache.v_cache[cache.table[s, at // 16], :, at % 16, channel] = x
+    request = [s for c in range(copies) for s in (4 * c, 4 * c + 1, 4 * c + 2, 4 * c + 2, 4 * c + 2, 4 * c + 3)]
+    position = [31, 31, 16, 17, 30, 19] * copies
+    q = rows_q(cache, len(request), heads, 64, t, gain=1.0)
+    lse = torch.empty(len(request), heads, device="cuda")
+    out = ops.paged_attention(q, cache.k_cache, cache.v_cache, cache.table, gpu_i32(request), gpu_i32(position), max_keys=max_keys, lse=lse).double().cpu()
+    for r, (s, p) in enumerate(zip(request, position)):
+        if r >= 12 and r % 31:                             # (the oracle takes its time)
+            continue
+        ref, ref_lse = definition(q[r], cache.k[s][:p + 1], cache.v[s][:p + 1], 1 / 8)
+        wild = ~torch.isfinite(ref)
+        assert bool(wild.any()) == (s % 4 != 1 and p > 3)
+        assert torch.equal(out[r][wild].nan_to_num(7.0, 8.0, 9.0), ref[wild].nan_to_num(7.0, 8.0, 9.0)), (r, out[r][wild], ref[wild])
+        v = cache.v[s].clone()
+        v[~torch.isfinite(v)] = 0.0                        # for the bounds of the channels that have a value
+        near, _, tol, tol_lse = attend_by_hand(q[r], cache.k[s], v, p, 1 / 8, 0)
+        assert bool(((out[r] - near).abs() <= tol)[~wild].all()), r
+        assert bool(((lse[r].double().cpu() - ref_lse).abs() <= tol_lse).all())
 
 
 @pytest.mark.parametrize("copies,hk,max_keys", FORMS)

@@ -659,7 +659,8 @@ struct AttTile {
     f32x4 f;                                            // fp32
     unsigned hi[2 * SUB], lo[2 * SUB];                  // 16 bits: two keys each; lo is what 16 bits leave of a weight
   };
-  static __device__ __forceinline__ Weights weights(const f32x4 (&p)[SUB]) {
+  // lifted: no second term is 0 or negative where the first is not 0 (see att_part); the weight then holds one bit less
+  static __device__ __forceinline__ Weights weights(const f32x4 (&p)[SUB], bool lifted) {
     Weights w;
     w.f = p[0];
     if constexpr (HALF) {
@@ -670,6 +671,12 @@ struct AttTile {
         const Two h = __builtin_convertvector(x, Two);
         w.hi[i] = __builtin_bit_cast(unsigned, h);
         w.lo[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(x - __builtin_convertvector(h, f32x2), Two));
+        if (lifted) {                                    // the number before it as the first term
+          const Two l = __builtin_bit_cast(Two, w.lo[i]);
+          if (!((float)l[0] > 0.f) && (w.hi[i] & 0xffffu)) w.hi[i] -= 1;
+          if (!((float)l[1] > 0.f) && (w.hi[i] >> 16)) w.hi[i] -= 0x10000u;
+          w.lo[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(x - __builtin_convertvector(__builtin_bit_cast(Two, w.hi[i]), f32x2), Two));
+        }
       }
     }
     return w;
@@ -801,7 +808,9 @@ __device__ __forceinline__ void att_leave(const PagedAttArgs& a, const AttPlan& 
 //
 // A key that one row of the run sees and another does not has a weight of 0 in the other's column, and 0 times an infinity or
 // a NaN in V would reach it.  So where rows differ and a result is not finite, the part is taken again row by row, with what
-// the row does not see left out of V.
+// the row does not see left out of V.  And 16-bit weights have a second term that may be 0 or negative, which times an infinity in V is
+// a NaN beside the first term's infinity: a row that is not finite by itself is taken once more, with two terms above 0.  (A weight
+// of fp16 below 2^-34 of the largest is 0 in its first term all the same, and 0 times an infinity a NaN.)
 //
 // Lanes are switched off in here for the write of a result alone (which, row by row, other rows follow): what a lane must not load it
 // loads from where another may, and drops.  With lanes off, the compiler (ROCm 7.2) has been seen to move whole-wave values to
@@ -852,6 +861,7 @@ __device__ __forceinline__ bool att_part(const PagedAttArgs& a, const AttPlan& p
   const T *kc = (const T*)a.k_cache, *vc = (const T*)a.v_cache;
   constexpr int ROUND = WAVE / SUB;                      // steps that one call of locate() serves
 
+  bool lifted = false;
   for (int alone = -1;;) {                               // -1: all rows together, else the row that is taken
     // keys that any and that every column in question sees
     const bool mine = real && (alone < 0 || my_row == alone);
@@ -934,7 +944,7 @@ __device__ __forceinline__ bool att_part(const PagedAttArgs& a, const AttPlan& p
           for (int e = 0; e < 4; ++e) s[u][e] = m >> (4 * u + e) & 1 ? s[u][e] : -INFINITY;
       }
       w.soften(s);
-      const typename Tile::Weights x = Tile::weights(s);
+      const typename Tile::Weights x = Tile::weights(s, lifted);
 #pragma unroll
       for (int pass = 0; pass < PASSES; ++pass) {
         if (pass > 0) {
@@ -956,14 +966,15 @@ __device__ __forceinline__ bool att_part(const PagedAttArgs& a, const AttPlan& p
     for (int c = 0; c < CH; ++c) ATT_SETTLE(w.o[c]);
     w.sum = col_sum(w.sum);
     w.top -= Tile::LIFT;                                  // from here on what a weight of 1 stands for
-    if (alone < 0 && r.n > 1) {
+    if ((alone < 0 && r.n > 1) || (Tile::HALF && !lifted)) {
       bool wild = false;
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) wild |= !(fabsf(w.o[c][e]) < INFINITY);
-      if (__ballot(wild && real)) {
-        alone = 0;
+      if (__ballot(wild && mine)) {
+        lifted = r.n == 1 || alone >= 0;
+        alone = max(alone, 0);
         continue;
       }
     }
@@ -979,6 +990,7 @@ __device__ __forceinline__ bool att_part(const PagedAttArgs& a, const AttPlan& p
     }
     if (mine) att_leave<T, DIM>(a, p, w, col, lg, r.row + my_row, hk * group + my_head, none, whole, slot);
     if (alone < 0 || ++alone == r.n) return stray != 0;
+    lifted = false;
   }
 }
 
