@@ -294,3 +294,80 @@ def test_attention_of_infinitely_high_scores(ops, dtype, copies, hk, max_keys):
         else:
             ref, ref_lse, tol, tol_lse = attend_by_hand(q[r], cache.k[request[r]], cache.v[request[r]], position[r], 1 / 8, 0)
             assert bool(((out[r] - ref).abs() <= tol).all()) and bool(((lse[r].double().cpu() - ref_lse).abs() <= tol_lse).all()), r
+
+
+@pytest.mark.parametrize("max_keys", [None, 10 ** 9])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("heads,hk,dim,page", [(1024, 1, 32, 16), (1024, 1024, 32, 16), (1000, 8, 64, 16), (33, 33, 64, 16), (2, 1, 32, 65536), (48, 3, 96, 4096)])
+def test_attention_of_the_largest_heads_and_pages(ops, dtype, heads, hk, dim, page, max_keys):
+    t = TYPES[dtype]
+    cache = Cache(t, [1, 40, 70], hk, dim, page, seed=81)
+    request, position = [2, -1, 0, 1, 1, -1, 1, 2, 2, 2], [69, 3, 0, 38, -1, -1, 39, 5, -1, 60]
+    q = rows_q(cache, len(request), heads, dim, t)
+    lse, out = torch.full((len(request), heads), 4.0, device="cuda"), torch.full_like(q, 4.0)
+    ops.paged_attention(q, cache.k_cache, cache.v_cache, cache.table, gpu_i32(request), gpu_i32(position), max_keys=max_keys, out=out, lse=lse)
+    out, lse = out.double().cpu(), lse.double().cpu()
+    for r, (s, p) in enumerate(zip(request, position)):
+        if s < 0:
+            assert bool((out[r] == 4.0).all() and (lse[r] == 4.0).all())
+        else:
+            ref, ref_lse, tol, tol_lse = attend_by_hand(q[r], cache.k[s], cache.v[s], p, 1 / math.sqrt(dim), 0)
+            assert bool(((out[r] - ref).abs() <= tol).all()), r
+            assert bool((lse[r] == -math.inf).all()) if p < 0 else bool(((lse[r] - ref_lse).abs() <= tol_lse).all())
+
+
+def test_rows_beyond_32_bits_of_elements(ops):
+    """2^19 + 5 rows of 32 heads of 256: 4.3e9 elements of q and of out, few of them live, the last among them."""
+    t, rows, heads, dim = torch.bfloat16, (1 << 19) + 5, 32, 256
+    cache = Cache(t, [40, 100], 2, dim, 16, seed=82)
+    live = [0, 12345, rows - 3, rows - 2, rows - 1]
+    q = torch.zeros(rows, heads, dim, dtype=t, device="cuda")
+    q[live] = rows_q(cache, len(live), heads, dim, t)
+    request, position = torch.full((rows,), -1, dtype=torch.int32, device="cuda"), torch.zeros(rows, dtype=torch.int32, device="cuda")
+    request[live], position[live] = gpu_i32([0, 1, 1, 1, 0]), gpu_i32([39, 99, 7, 8, 20])
+    out = torch.full_like(q, 4.0)
+    ops.paged_attention(q, cache.k_cache, cache.v_cache, cache.table, request, position, max_keys=100, out=out)
+    for r in live:
+        s, p = int(request[r]), int(position[r])
+        ref, _, tol, _ = attend_by_hand(q[r], cache.k[s], cache.v[s], p, 1 / 16, 0)
+        assert bool(((out[r].double().cpu() - ref).abs() <= tol).all()), r
+    assert bool((out[1] == 4.0).all() and (out[rows - 4] == 4.0).all())
+    slot = torch.full((rows,), -1, dtype=torch.int64, device="cuda")
+    slot[live] = torch.arange(len(live), device="cuda")
+    freq, few = ops.rotary_frequencies(dim), torch.tensor(live, device="cuda")
+    want = ops.rotary_store(q[few].contiguous(), None, None, None, None, position[few].contiguous(), None, freq)
+    ops.rotary_store(q, None, None, None, None, position, slot, freq, out=out)
+    assert torch.equal(out[few], want) and bool((out[1] == 4.0).all() and (out[rows - 4] == 4.0).all())
+
+
+def test_rotary_of_many_rows(ops):
+    gen = torch.Generator(device="cuda").manual_seed(83)
+    rows = (1 << 23) - 3
+    q = torch.randn(rows, 1, 2, generator=gen, device="cuda")
+    position = torch.randint(0, 1 << 20, (rows,), generator=gen, dtype=torch.int32, device="cuda")
+    freq = ops.rotary_frequencies(2)
+    out = ops.rotary_store(q, None, None, None, None, position, None, freq)
+    angle = position.double() * freq
+    a, b = q[:, 0, 0].double(), q[:, 0, 1].double()
+    ref = torch.stack((a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()), 1)
+    bound = ((a.abs() + b.abs()) * 2.0 ** -21 + 2.0 ** -51 * angle * (a.abs() + b.abs()))[:, None] + ref.abs() * 2.0 ** -24
+    assert bool(((out[:, 0].double() - ref).abs() <= bound).all())
+
+
+def test_plan_of_the_farthest_positions(ops):
+    """Lengths up to 2^31 - 1 in pages of 65536, and page ids whose slots need 64 bits."""
+    page, width, last = 65536, 32768, 2 ** 31 - 1
+    pages = 1 << 20
+    table = torch.full((2, width), -1, dtype=torch.int32, device="cuda")
+    table[0, :] = torch.arange(width, device="cuda")
+    ring = torch.full((pages,), -1, dtype=torch.int32, device="cuda")
+    ring[5] = pages - 1
+    cursor = torch.tensor([5, 6], dtype=torch.int64, device="cuda")
+    plan = ops.page_plan(gpu_i32([last - 3, 0]), gpu_i32([3, 2]), table, ring, cursor, page, rows=6)
+    assert plan.status.item() == 0 and plan.lengths.tolist() == [last, 2] and plan.start.tolist() == [0, 3, 5] and plan.cursor.tolist() == [6, 6]
+    assert plan.request.tolist() == [0, 0, 0, 1, 1, -1] and plan.position.tolist() == [last - 3, last - 2, last - 1, 0, 1, -1]
+    top = (width - 1) * page
+    assert plan.slot.tolist() == [top + 65532, top + 65533, top + 65534, (pages - 1) * page, (pages - 1) * page + 1, -1]
+    assert table[1, 0].item() == pages - 1
+    plan = ops.page_plan(gpu_i32([last, 0]), gpu_i32([1, 0]), table, ring, cursor, page, rows=6)
+    assert plan.status.item() == 1 and plan.slot.eq(-1).all()
