@@ -25,7 +25,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 // pages than the ring, so no place is read by one block and written by another.
 // Bound by latency, not by its bytes: a launch, one dependent load, a scan and a barrier for the sums, the same again for the
 // rows, one table entry.  One block would do for the sums, but its rows would then wait for a second launch.  48 requests, a row
-// each: 4.9 us; 700 requests, 62 k rows (1.06 MB): 7.4 us; 256 prompts, 254 k rows (4.2 MB): 6.6 us (0.6 TB/s).  Every block reads every
+// each: 4.8 us; 700 requests, 62 k rows (1.06 MB): 7.5 us; 256 prompts, 254 k rows (4.2 MB): 6.6 us (0.6 TB/s).  Every block reads every
 // request, and a block serves 32 of them at most, so many requests cost their square: 4096 take 17 us, 16384 120 us, 65535 1.9 ms.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int PLAN_THREADS = 256;
@@ -212,8 +212,8 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PagePlanArgs a)
 // rotary rows, stored to the cache.  A pair of channels (a, b) turns to (a cos - b sin, b cos + a sin); every value is read and
 // written once, so a prompt is bound by memory: 8192 rows of 32 + 8 + 8 heads of 128 in bf16, 201 MB, take 43.8 us, 4.6 TB/s
 // (a plain copy: 4.9).  A block computes the angles of its rows once, in LDS, for all their heads: a transcendental a pair and
-// row instead of one a value.  Few rows are bound by the chain launch - position - angle - barrier - slot - values: one row 2.5
-// us, 192 rows of 48 heads of 128 (4.45 MB) 3.9 us; loading the values before the angles was no faster there (the longer code
+// row instead of one a value.  Few rows are bound by the chain launch - position - angle - barrier - slot - values: one row 2.4
+// us, 192 rows of 48 heads of 128 (4.45 MB) 4.0 us; loading the values before the angles was no faster there (the longer code
 // costs as much as it hides) and slower on prompts (51 us).
 // ---------------------------------------------------------------------------------------------------------
 template <typename T> struct Conv;
@@ -408,11 +408,11 @@ hipError_t start_rotary_t(RotaryArgs a, hipStream_t s) {
 // 2.6e-4 of the result, now 2.1e-4, which is the rounding of the result itself, in the same time).
 //
 // What bounds it: the cache is read once for all rows and heads of a unit, so long and many rows are bound by memory (64 rows of up
-// to 4096 tokens, 8 heads of 128 in bf16, 603 MB: 121 us, 5.0 TB/s; one row over 131 k tokens, 537 MB: 105 us, 5.1; 512 rows of up to
-// 1500, fp16, 841 MB: 149 us, 5.6, part of it from the last-level cache).  Short ones are bound by latency: a wave takes 1.3 us for a
+// to 4096 tokens, 8 heads of 128 in bf16, 603 MB: 121 us, 5.0 TB/s; one row over 131 k tokens, 537 MB: 107 us, 5.0; 512 rows of up to
+// 1500, fp16, 841 MB: 150 us, 5.6, part of it from the last-level cache).  Short ones are bound by latency: a wave takes 1.3 us for a
 // step of 32 keys by itself, so a row alone is spread over the waves of a block.  fp32 rows alone are bound by the matrix rate of
 // the few CUs that they reach (16x16x4: 1536 cycles for 16 keys of 96 channels, of whose 16 columns one row of a head of its
-// own fills one): one row of 500 tokens, 2 heads of 96: 14.3 us.
+// own fills one): one row of 500 tokens, 2 heads of 96: 14.6 us.
 // ---------------------------------------------------------------------------------------------------------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x3a __attribute__((ext_vector_type(3), aligned(4)));
@@ -1204,7 +1204,7 @@ __global__ __launch_bounds__(ATT_THREADS, DIM <= 128 ? 2 : 1) void paged_attenti
 // a wave each, where there are many units and so, as a rule, few parts of each (where one has many after all, the block takes
 // them one after the other); one, where few units have many parts (one row over a long context).  dim / 4 threads hold a part, the
 // team as many parts as that leaves threads for and eight times that in flight, each its parts in the order of the keys, so that
-// the result does not depend on which block was done first.  Latency: 5.0 us for 200 units of 2 to 3 parts, 7.5 us for 8 units of 64
+// the result does not depend on which block was done first.  Latency: 5.0 us for 200 units of 2 to 3 parts, 8.1 us for 8 units of 64
 // parts each; as an "all parts, then the last block joins" in the kernel before, it would need a counter to be cleared by a launch
 // of its own and a release of every part to the other dies' caches.
 constexpr int JOIN_FEW = 16;
