@@ -25,7 +25,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", 
 # The paged attention keeps its accumulators in the registers that the vector unit reads too.  Left to choose, the compiler gives
 # builds with much LDS the other kind, moves values there, and has been seen to move only those of the lanes that were on.
 # Where a build needs more than 256 registers it takes those too, whatever the flag says: so the compiler reports what it used, and a
-# build that has any, or scratch, is refused (the widest today: 256, none, none).
+# build that has any, or scratch, is refused (the widest today: 252, none, none).
 USAGE = "-Rpass-analysis=kernel-resource-usage"
 SOURCE_FLAGS = {"kernels_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", USAGE]}
 MOST = {"VGPRs": 256, "AGPRs": 0, "ScratchSize": 0, "VGPRs Spill": 0}
